@@ -399,6 +399,124 @@ int lnsb_rope_qkv(int fmt, const lnsb_rope_qkv_args * args, lnsb_stream_t stream
 int lnsb_f32_to_f16(const float * src, uint16_t * dst, int64_t n, lnsb_stream_t stream);
 int lnsb_f16_to_f32(const uint16_t * src, float * dst, int64_t n, lnsb_stream_t stream);
 
+/* ---- Serving many sequences from a paged KV cache (no counterpart in the
+ * reference; ordinary floating point, no LNS involved: these are the ops a
+ * host runs outside LNS, as LNS_DISABLE_OPS does for rope, kq, kq_soft_max and
+ * kqv).  Keys and values of all sequences lie in pages of page_size rows; a
+ * sequence's row i is row i % page_size of page page_table[s][i / page_size].
+ * A call takes the new tokens of all its sequences at once, one after the
+ * other: tokens q_start[s] .. q_start[s + 1] - 1 belong to sequence s and are
+ * the last of its kv_len[s] cached rows, so token t sits at row
+ * kv_len[s] - (q_start[s + 1] - t).  A sequence may have no new token; a token
+ * whose row would be negative has no row: it is not stored and its attention
+ * is zero.
+ *
+ * The three plan arrays are read on the device, so a captured graph can be
+ * replayed with new lengths; the host gives bounds.  kv_len above max_kv is
+ * taken as max_kv, q_start is taken within [0, n_tokens].  A page id outside
+ * [0, n_pages) that a visible row needs is never followed: its rows are not
+ * stored and read as zeros, and it is counted (lnsb_paged_errors). ---- */
+typedef struct {
+    void *          k_cache;      /* page p, row r, kv head h at p * page_stride + r * row_stride + h * head_stride, */
+    void *          v_cache;      /*   counted in elements; head_dim elements contiguous */
+    int64_t         page_stride, row_stride, head_stride;   /* multiples of 8; both caches 16-byte aligned */
+    const int32_t * page_table;   /* [n_seqs][table_ld] */
+    const int32_t * q_start;      /* [n_seqs + 1] */
+    const int32_t * kv_len;       /* [n_seqs] */
+    int64_t         table_ld, n_pages, n_tokens, max_kv;    /* max_kv <= table_ld * page_size */
+    int             n_seqs;
+    int             type;         /* LNSB_TYPE_F16 | LNSB_TYPE_BF16 */
+    int             page_size;    /* a power of two, 8 .. 1024 */
+    int             n_head_kv;
+    int             head_dim;     /* 16, 32, 64, 128 or 256 */
+} lnsb_paged_kv;
+
+/* k and v of the new tokens into the cache, k rotated on the way, and q
+ * rotated beside it.  Pair j of a head turns by the angle whose (cos, sin) is
+ * cos_sin[(row * n_dims/2 + j) * 2 + {0, 1}] (lnsb_rope's table, by cache row;
+ * max_kv rows at least): (2j, 2j+1), or (j, j + n_dims/2) with neox; elements
+ * from n_dims on are copied.  Computed in 32 bits, rounded once to the cache's
+ * type.  A token's heads are contiguous; rows are *_ld elements apart. */
+typedef struct {
+    lnsb_paged_kv kv;
+    const void *  k;              /* [n_tokens][n_head_kv][head_dim] of in_type */
+    const void *  v;              /* the same */
+    const void *  q;              /* [n_tokens][n_head][head_dim] of in_type, or NULL */
+    void *        q_out;          /* of the cache's type; NULL with q */
+    const float * cos_sin;        /* NULL with n_dims == 0: nothing is turned */
+    int64_t       k_ld, v_ld, q_ld, q_out_ld;
+    int           in_type;        /* LNSB_TYPE_F32 | LNSB_TYPE_F16 | LNSB_TYPE_BF16 */
+    int           n_head;         /* of q */
+    int           n_dims;         /* even, <= head_dim */
+    int           neox;
+} lnsb_paged_append_args;
+int lnsb_paged_append(const lnsb_paged_append_args * args, lnsb_stream_t stream);
+
+/* attention of the new tokens over the cache (after lnsb_paged_append of
+ * them): the token at row i of its sequence sees rows j <= i, and j > i -
+ * window when window > 0; with query head h on kv head h / (n_head /
+ * n_head_kv)
+ *   dst = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale * q.k_j - max)
+ * and 0 where no row is visible.  Rows of the cache at or beyond kv_len, and
+ * those before the window of a sequence's first new token, may hold anything.
+ * Any other non-finite row may reach all of the call's tokens of its sequence.
+ * q and dst are of the cache's type, rows 16-byte aligned (pointers, q_ld and
+ * dst_ld multiples of 8).  Products and the softmax's sums are 32-bit floats;
+ * the weights p are rounded to the cache's type for the product with v.
+ *
+ * work: lnsb_paged_attn_work_bytes() bytes of device memory, 16-byte aligned,
+ * zero before its first use; every call leaves it ready for the next.  Calls
+ * that can overlap on the GPU need one each. */
+typedef struct {
+    lnsb_paged_kv kv;
+    const void *  q;              /* [n_tokens][n_head][head_dim] */
+    void *        dst;            /* [n_tokens][n_head][head_dim] */
+    void *        work;
+    int64_t       work_bytes;
+    int64_t       q_ld, dst_ld;
+    int64_t       max_q;          /* the most new tokens of one sequence: chooses the kernels, limits nothing */
+    int64_t       window;         /* 0: none */
+    int           n_head;
+    float         scale;
+} lnsb_paged_attn_args;
+int lnsb_paged_attn(const lnsb_paged_attn_args * args, lnsb_stream_t stream);
+int64_t lnsb_paged_attn_work_bytes(void);
+
+/* since the last call, on the current device: page ids outside the cache met
+ * by lnsb_paged_append and lnsb_paged_attn, and waits inside lnsb_paged_attn
+ * that ran out (its output is then invalid); either may be NULL.  Reads and
+ * clears both counts (synchronises with the device). */
+int lnsb_paged_errors(int64_t * bad_pages, int64_t * timeouts);
+
+/* The next token of every row of logits from one given random number per row.
+ * With x = logits[r] (NaN counts as -inf), t = temperature[r] and
+ *   w_i = exp((x_i - max x) * (1 / t)),  w_i = 1 where x_i is the maximum,
+ * the tokens in falling order of x, equal ones in order of their index, are
+ * cut to the first top_k, of these to the shortest prefix whose sum of w is
+ * at least top_p times theirs (one token at least), of these to those with
+ * w >= min_p.  token is the first kept one, in order of index, at which the
+ * running sum of w passes u[r] times the kept ones' sum; prob is its w over
+ * that sum.  t <= 0 takes the largest logit, the first of equal ones, with
+ * prob 1.  A row without a logit above -inf gives token -1 and prob 0.
+ * w is a 32-bit float, its sums are exact integers of 2^-40 (the remainder of
+ * each w below that is dropped), so nothing hangs on an order of additions.
+ * temperature, top_k, top_p, min_p: per row, in device memory; NULL, or
+ * top_k <= 0, top_p >= 1, min_p <= 0 in a row, leaves that filter out (NULL
+ * temperature: 1).  u in [0, 1). */
+typedef struct {
+    const void *    logits;       /* [n_rows][ld] of type, n_vocab used */
+    const float *   temperature;
+    const int32_t * top_k;
+    const float *   top_p;
+    const float *   min_p;
+    const float *   u;
+    int32_t *       token;        /* [n_rows] */
+    float *         prob;         /* [n_rows] or NULL */
+    int64_t         ld, n_rows, n_vocab;   /* n_vocab <= 2^20 */
+    int             type;         /* LNSB_TYPE_F32 | LNSB_TYPE_F16 | LNSB_TYPE_BF16 */
+} lnsb_sample_args;
+int lnsb_sample(const lnsb_sample_args * args, lnsb_stream_t stream);
+
 /* ---- Monte state: one LFSR per process, seed 7 (ggml-lns.h:13-24).  All
  *      return 0 on success, LNSB_E_UNSUPPORTED outside a monte build;
  *      set_state rejects 0 (absorbing). ---- */

@@ -1,7 +1,9 @@
 """Builds the B200 LNS libraries in-tree: lib/liblnsb200_<mode>.so, one per
 xlns16 summation mode, exactly as the reference builds one tree per
 GGML_LNS16_SUM mode (lns-backend/common/lns-common.cmake:24-46).  Every
-library also carries the xlns32 (LNSCUDA32) kernels.
+library also carries the xlns32 (LNSCUDA32) kernels, and the serving kernels
+(lnsb_serve.cu), which no summation mode enters: they are compiled once, to an
+object that every library links.
 
     python xlns-ggml-backend_b200/build.py            # all modes
     python xlns-ggml-backend_b200/build.py base sum32 # some
@@ -20,7 +22,8 @@ LIB = os.path.join(HERE, "lib")
 MODES = {"base": 0, "monte": 1, "monte_bylpvip": 2, "lpvip": 3, "sum32": 4}
 
 SOURCES = ["lnsb_kernels.cu", "lnsb_tables.cpp", "lnsb_graph.cpp"]
-HEADERS = ["lnsb_arith.cuh", "lnsb_tables.h", os.path.join(ROOT, "include", "lnsb200.h"),
+SHARED_SOURCES = ["lnsb_serve.cu"]
+HEADERS = ["lnsb_arith.cuh", "lnsb_launch.cuh", "lnsb_tables.h", os.path.join(ROOT, "include", "lnsb200.h"),
            os.path.join(ROOT, "include", "lnsb200_graph.h")]
 
 
@@ -35,39 +38,58 @@ def lib_path(mode):
     return os.path.join(LIB, "liblnsb200_%s.so" % mode)
 
 
-def _stale(out):
+def _path(name):
+    return name if os.path.isabs(name) else os.path.join(CSRC, name)
+
+
+def _stale(out, sources):
     if not os.path.exists(out):
         return True
     t = os.path.getmtime(out)
-    deps = [os.path.join(CSRC, s) for s in SOURCES] + [h if os.path.isabs(h) else os.path.join(CSRC, h) for h in HEADERS]
-    return any(os.path.getmtime(d) > t for d in deps)
+    return any(os.path.getmtime(_path(d)) > t for d in sources + HEADERS)
 
 
-def build_mode(mode, force=False, verbose=False):
-    out = lib_path(mode)
-    if not force and not _stale(out):
-        return out
-    os.makedirs(LIB, exist_ok=True)
-    cmd = [
-        nvcc(), "-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "-std=c++17",
-        "-Xcompiler", "-fPIC,-ffp-contract=off", "-shared",
-        "-DLNSB_SUM_MODE=%d" % MODES[mode],
-        "-I", os.path.join(ROOT, "include"),
-        "-o", out + ".tmp",
-    ] + [os.path.join(CSRC, s) for s in SOURCES]
-    if verbose:
-        cmd.insert(1, "-Xptxas=-v")
+def _flags(verbose=False):
+    return [nvcc()] + (["-Xptxas=-v"] if verbose else []) + [
+        "-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "-std=c++17",
+        "-Xcompiler", "-fPIC,-ffp-contract=off", "-I", os.path.join(ROOT, "include")]
+
+
+def _run(what, cmd):
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
-        raise RuntimeError("nvcc failed for mode %s:\n%s\n%s" % (mode, " ".join(cmd), r.stderr))
+        raise RuntimeError("nvcc failed for %s:\n%s\n%s" % (what, " ".join(cmd), r.stderr))
+
+
+def build_shared(force=False, verbose=False):
+    """the objects that do not depend on the summation mode"""
+    outs = []
+    os.makedirs(LIB, exist_ok=True)
+    for src in SHARED_SOURCES:
+        out = os.path.join(LIB, os.path.splitext(src)[0] + ".o")
+        if force or _stale(out, [src]):
+            _run(src, _flags(verbose) + ["-c", "-o", out + ".tmp", _path(src)])
+            os.replace(out + ".tmp", out)
+        outs.append(out)
+    return outs
+
+
+def build_mode(mode, force=False, verbose=False, objects=None):
+    out = lib_path(mode)
+    if not force and not _stale(out, SOURCES + SHARED_SOURCES):
+        return out
+    objects = objects if objects is not None else build_shared(force, verbose)
+    _run("mode " + mode, _flags(verbose) + ["-shared", "-DLNSB_SUM_MODE=%d" % MODES[mode], "-o", out + ".tmp"] +
+         [_path(s) for s in SOURCES] + objects)
     os.replace(out + ".tmp", out)
     return out
 
 
 def build_all(modes=None, force=False):
     modes = list(modes or MODES)
+    objects = build_shared(force)
     with concurrent.futures.ThreadPoolExecutor(max_workers=len(modes)) as ex:
-        return list(ex.map(lambda m: build_mode(m, force), modes))
+        return list(ex.map(lambda m: build_mode(m, force, objects=objects), modes))
 
 
 if __name__ == "__main__":

@@ -1,0 +1,857 @@
+// Serving many sequences from a paged KV cache: appending rotated keys and
+// values, attention of the new tokens over the cache, sampling.  Ordinary
+// floating point, no LNS: the ops a host runs outside LNS.  The code does not
+// depend on the summation mode; every library of the build carries it.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+
+#include "lnsb200.h"
+#include "lnsb_launch.cuh"
+
+namespace lnsb {
+namespace {
+
+// page ids outside the cache, waits that ran out: lnsb_paged_errors
+__device__ unsigned long long g_paged_errors[2];
+
+constexpr int k_sms = 148;                      // of one B200
+
+template <class T> struct num;
+template <> struct num<float> {
+    static __device__ __forceinline__ float to(float v) { return v; }
+    static __device__ __forceinline__ float from(float v) { return v; }
+};
+template <> struct num<__half> {
+    static __device__ __forceinline__ float to(__half v) { return __half2float(v); }
+    static __device__ __forceinline__ __half from(float v) { return __float2half_rn(v); }
+    static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+        const __half2 h = __floats2half2_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    }
+    static constexpr uint32_t one2 = 0x3C003C00u;
+};
+template <> struct num<__nv_bfloat16> {
+    static __device__ __forceinline__ float to(__nv_bfloat16 v) { return __bfloat162float(v); }
+    static __device__ __forceinline__ __nv_bfloat16 from(float v) { return __float2bfloat16_rn(v); }
+    static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    }
+    static constexpr uint32_t one2 = 0x3F803F80u;
+};
+
+// ============================ the plan =====================================
+
+// the device's view of lnsb_paged_kv
+struct paged {
+    const int32_t * table;
+    const int32_t * q_start;
+    const int32_t * kv_len;
+    int64_t         table_ld, n_pages, n_tokens, max_kv;
+    int64_t         page_stride, row_stride, head_stride;
+    int             n_seqs, page_shift, n_head_kv;
+};
+
+struct seq_span {
+    int64_t first, n, kv;      // first new token, how many, visible rows
+};
+__device__ __forceinline__ seq_span span_of(const paged & P, int s) {
+    const int64_t a = min(max((int64_t) P.q_start[s], (int64_t) 0), P.n_tokens);
+    const int64_t b = min(max((int64_t) P.q_start[s + 1], a), P.n_tokens);
+    return { a, b - a, min(max((int64_t) P.kv_len[s], (int64_t) 0), P.max_kv) };
+}
+// page id of a row below kv_len, or -1 (counted) for one outside the cache
+__device__ __forceinline__ int64_t page_of(const paged & P, int s, int64_t row) {
+    const int64_t id = P.table[s * P.table_ld + (row >> P.page_shift)];
+    if (id >= 0 && id < P.n_pages) return id;
+    atomicAdd(&g_paged_errors[0], 1ull);
+    return -1;
+}
+
+// ============================ append =======================================
+
+// One thread per rotated pair, copied element or v element.
+template <class TI, class TC>
+__global__ void k_paged_append(paged P, const TI * __restrict__ k, const TI * __restrict__ v, const TI * __restrict__ q,
+                               TC * __restrict__ q_out, const float * __restrict__ cos_sin, int64_t k_ld, int64_t v_ld,
+                               int64_t q_ld, int64_t q_out_ld, int n_head, int D, int n_dims, int neox,
+                               TC * __restrict__ kc, TC * __restrict__ vc) {
+    pdl_entry();
+    const int half = n_dims / 2, per = half + (D - n_dims);
+    const int64_t row_work = (int64_t) (n_head + P.n_head_kv) * per + (int64_t) P.n_head_kv * D;
+    const int64_t n = P.n_tokens * row_work;
+    for (int64_t i = (int64_t) blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t) blockDim.x * gridDim.x) {
+        const int64_t t = i / row_work;
+        int64_t r = i - t * row_work;
+        int lo = 0, hi = P.n_seqs;                       // the last sequence that starts at or before t
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) / 2;
+            if (P.q_start[mid] <= t) lo = mid; else hi = mid;
+        }
+        const seq_span S = span_of(P, lo);
+        const int64_t row = S.kv - S.n + (t - S.first);
+        if (t < S.first || t >= S.first + S.n || row < 0) continue;
+        const int64_t heads = n_head + P.n_head_kv;
+        const bool is_v = r >= heads * per;
+        const int64_t h = is_v ? (r - heads * per) / D : r / per;
+        const bool to_cache = is_v || h >= n_head;
+        int64_t at = 0;
+        if (to_cache) {
+            const int64_t id = page_of(P, lo, row);
+            if (id < 0) continue;
+            at = id * P.page_stride + (row & ((1 << P.page_shift) - 1)) * P.row_stride +
+                 (is_v ? h : h - n_head) * P.head_stride;
+        }
+        if (is_v) {
+            const int64_t d = (r - heads * per) % D;
+            vc[at + d] = num<TC>::from(num<TI>::to(v[t * v_ld + h * D + d]));
+            continue;
+        }
+        const int j = (int) (r - h * per);
+        const TI * src = h < n_head ? q + t * q_ld + h * D : k + t * k_ld + (h - n_head) * D;
+        TC * dst = h < n_head ? q_out + t * q_out_ld + h * D : kc + at;
+        if (j >= half) {
+            const int d = n_dims + j - half;
+            dst[d] = num<TC>::from(num<TI>::to(src[d]));
+            continue;
+        }
+        const int d0 = neox ? j : 2 * j, d1 = neox ? j + half : 2 * j + 1;
+        const float c = cos_sin[(row * half + j) * 2], s = cos_sin[(row * half + j) * 2 + 1];
+        const float x0 = num<TI>::to(src[d0]), x1 = num<TI>::to(src[d1]);
+        dst[d0] = num<TC>::from(x0 * c - x1 * s);
+        dst[d1] = num<TC>::from(x0 * s + x1 * c);
+    }
+}
+
+// ===================== attention: few rows a sequence ======================
+//
+// The rows of one (sequence, kv head) are its (token, head of the group)
+// pairs, row r = token r / G, head r % G.  A CTA takes 16 of them -- the
+// height of one mma.sync tile -- over a range of 64-key tiles: warp w
+// computes keys 16 w .. 16 w + 15 of each tile, with its own maximum, sum and
+// output, so the four warps never wait for one another inside the range and
+// join at its end.
+//
+// What bounds it is the cache's bytes.  All (sequence, row tile, kv head, key
+// tile) units form one line that the CTAs cut into equal shares, whatever the
+// lengths: a share that ends inside an item leaves a partial result in `work`,
+// and the CTA that comes last to an item joins its partials in the order of
+// the line, so the result does not hang on who came when.
+//
+// The maximum is a reference that moves only when a score passes it by more
+// than 8 (in log2): exp2 of the rest stays below 2^8, which both types hold,
+// and the quotient does not see the reference.  The sum of the weights comes
+// from the same product as the output, against a column of ones, so it is of
+// the weights as rounded.
+
+constexpr int ROWS = 16, KEYS = 64, A_CTAS = 2 * k_sms;
+constexpr int MAX_DIM = 256;
+constexpr float k_lag = 8.0f;
+constexpr float k_none = -1e30f;               // the reference of a row that has seen nothing
+
+// work: [counters A_CTAS int32][partials A_CTAS * 2 * (ROWS * MAX_DIM + 2 * ROWS) float]
+constexpr int64_t A_PART = ROWS * MAX_DIM + 2 * ROWS;
+constexpr int64_t A_COUNT_BYTES = (A_CTAS * 4 + 255) / 256 * 256;
+constexpr int64_t A_WORK = A_COUNT_BYTES + (int64_t) A_CTAS * 2 * A_PART * 4;
+
+__device__ __forceinline__ uint32_t smem_addr(const void * p) { return (uint32_t) __cvta_generic_to_shared(p); }
+__device__ __forceinline__ void cp16(uint32_t dst, const void * src, bool valid) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" :: "r"(dst), "l"(src), "r"(valid ? 16 : 0));
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;\n" ::); }
+template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;\n" :: "n"(N) : "memory"); }
+__device__ __forceinline__ void ldsm4(uint32_t a, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];\n"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a));
+}
+__device__ __forceinline__ void ldsm4t(uint32_t a, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];\n"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a));
+}
+template <class T>
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (std::is_same<T, __half>::value)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// units of one sequence in the line: row tiles x kv heads x key tiles
+struct seq_units {
+    int64_t row_tiles, key_tiles, first_tile;   // key tiles from first_tile on
+};
+__device__ __forceinline__ seq_units units_of(const seq_span & S, int G, int64_t window) {
+    seq_units u;
+    u.row_tiles = (S.n * G + ROWS - 1) / ROWS;
+    int64_t lo = 0;
+    if (window > 0) lo = max((int64_t) 0, S.kv - S.n - window + 1);
+    u.first_tile = lo / KEYS;
+    u.key_tiles = max((int64_t) 1, (S.kv + KEYS - 1) / KEYS - u.first_tile);
+    return u;
+}
+// smem of one CTA: the warps' rings, reused for joining the warps
+template <int D> __host__ __device__ constexpr int a_stages() { return D <= 128 ? 3 : 2; }
+template <int D> __host__ __device__ constexpr int a_stage_bytes() { return 16 * D * 2 * 2; }
+template <int D> __host__ __device__ constexpr int a_smem() {
+    const int ring = 4 * a_stages<D>() * a_stage_bytes<D>();
+    const int join = 4 * (ROWS * (D + 4) + 2 * ROWS) * 4;
+    return ring > join ? ring : join;
+}
+// 16-byte chunk c of row r in a [rows][D] tile: the rows that one ldmatrix
+// reads together lie in different banks
+template <int D> __device__ __forceinline__ uint32_t chunk_at(int r, int c) {
+    constexpr int CPR = D / 8;
+    const int x = CPR >= 8 ? (r & 7) : CPR == 4 ? ((r >> 1) & 3) : ((r >> 2) & 1);
+    return (uint32_t) (r * CPR + (c ^ x)) * 16;
+}
+
+template <class T, int D>
+__global__ void __launch_bounds__(128)
+k_paged_attn_rows(paged P, const T * __restrict__ q, T * __restrict__ dst, const T * __restrict__ kc,
+                  const T * __restrict__ vc, int64_t q_ld, int64_t dst_ld, int G, float scale_log2, int64_t window,
+                  int * __restrict__ counters, float * __restrict__ parts) {
+    constexpr int ST = a_stages<D>(), SB = a_stage_bytes<D>(), CPR = D / 8, KS = D / 16;
+    extern __shared__ __align__(128) unsigned char sm[];
+    __shared__ int64_t s_scan[128];
+    __shared__ int s_last;
+    pdl_entry();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int c = blockIdx.x;
+
+    // the line's length: thread t sums the sequences of its share
+    const int per = (P.n_seqs + 127) / 128;
+    const int s_lo = min(tid * per, P.n_seqs), s_hi = min(s_lo + per, P.n_seqs);
+    int64_t mine = 0;
+    for (int s = s_lo; s < s_hi; s++) {
+        const seq_units u = units_of(span_of(P, s), G, window);
+        mine += u.row_tiles * u.key_tiles * P.n_head_kv;
+    }
+    s_scan[tid] = mine;
+    __syncthreads();
+    int64_t W = 0;
+    for (int i = 0; i < 128; i++) W += s_scan[i];
+    const int64_t N = min((int64_t) gridDim.x, W);                // CTAs that get a share: one unit at least
+    if (c >= N) return;
+    int64_t x = W * c / N;
+    const int64_t x_end = W * (c + 1) / N;
+    // the sequence that holds unit x, and the line's position where it begins
+    int s = 0;
+    int64_t base = 0;
+    {
+        int b = 0;
+        while (base + s_scan[b] <= x) base += s_scan[b++];
+        s = b * per;
+    }
+    const uint32_t ring = smem_addr(sm) + warp * ST * SB;
+    float * join = reinterpret_cast<float *>(sm);
+
+    while (x < x_end) {
+        seq_span S = span_of(P, s);
+        seq_units u = units_of(S, G, window);
+        int64_t len = u.row_tiles * u.key_tiles * P.n_head_kv;
+        while (base + len <= x) {
+            base += len;
+            S = span_of(P, ++s);
+            u = units_of(S, G, window);
+            len = u.row_tiles * u.key_tiles * P.n_head_kv;
+        }
+        const int64_t item = (x - base) / u.key_tiles;           // (row tile, kv head) of the sequence
+        const int64_t item0 = base + item * u.key_tiles;         // its place on the line
+        const int64_t t0 = x - item0, t1 = min(u.key_tiles, x_end - item0);
+        const int h = (int) (item % P.n_head_kv);
+        const int64_t r0 = item / P.n_head_kv * ROWS, R = S.n * G;
+        const int64_t pos0 = S.kv - S.n;                         // row of the sequence's first new token
+        // keys that some row of the tile sees
+        const int64_t last_row = min(r0 + ROWS, R) - 1;
+        const int64_t key_end = min(S.kv, pos0 + last_row / G + 1);
+        const int64_t key_lo = window > 0 ? max((int64_t) 0, pos0 + r0 / G - window + 1) : 0;
+
+        // rows lane/4 and lane/4 + 8 of the tile
+        int64_t pos[2], lo[2];
+        const T * qp[2];
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const int64_t r = r0 + lane / 4 + 8 * i;
+            pos[i] = r < R ? pos0 + r / G : -1;
+            lo[i] = window > 0 ? pos[i] - window + 1 : 0;
+            qp[i] = r < R ? q + (S.first + r / G) * q_ld + ((int64_t) h * G + r % G) * D + (lane % 4) * 2 : nullptr;
+        }
+        uint32_t qf[KS][4];
+#pragma unroll
+        for (int k = 0; k < KS; k++)
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                qf[k][i] = qp[i & 1] ? *reinterpret_cast<const uint32_t *>(qp[i & 1] + k * 16 + (i >> 1) * 8) : 0u;
+
+        float o[D / 8][4], l[4] = { 0, 0, 0, 0 }, m[2] = { k_none, k_none };
+#pragma unroll
+        for (int i = 0; i < D / 8; i++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) o[i][e] = 0.0f;
+
+        const T * kh = kc + (int64_t) h * P.head_stride;
+        const T * vh = vc + (int64_t) h * P.head_stride;
+        // the keys of tile t that this warp takes
+        auto load = [&](int64_t t, int stage) {
+            const int64_t k0 = (u.first_tile + t) * KEYS + warp * 16;
+            const uint32_t ks = ring + stage * SB, vs = ks + 16 * D * 2;
+            int64_t id[2];
+#pragma unroll
+            for (int i = 0; i < 2; i++) {                        // page_size >= 8: eight keys share a page
+                const int64_t key = k0 + 8 * i;
+                id[i] = t < t1 && key < key_end && key + 8 > key_lo ? page_of(P, s, key) : -1;
+            }
+#pragma unroll
+            for (int j = 0; j < 16 * CPR / 32; j++) {
+                const int idx = j * 32 + lane, r = idx / CPR, ch = idx % CPR;
+                const int64_t key = k0 + r, pid = id[r >> 3];
+                const bool ok = pid >= 0 && key < key_end && key >= key_lo;
+                const int64_t off = ok ? pid * P.page_stride + (key & ((1 << P.page_shift) - 1)) * P.row_stride + ch * 8 : 0;
+                cp16(ks + chunk_at<D>(r, ch), kh + off, ok);
+                cp16(vs + chunk_at<D>(r, ch), vh + off, ok);
+            }
+            cp_commit();
+        };
+        for (int i = 0; i < ST - 1; i++) load(t0 + i, i);
+        int stage = 0;
+        for (int64_t t = t0; t < t1; t++) {
+            load(t + ST - 1, stage == 0 ? ST - 1 : stage - 1);
+            cp_wait<ST - 1>();
+            __syncwarp();
+            const uint32_t ks = ring + stage * SB, vs = ks + 16 * D * 2;
+            float sc[2][4] = {};
+#pragma unroll
+            for (int k = 0; k < KS; k++) {
+                uint32_t b[4];                                    // keys 0-7 and 8-15, halves of 16 dims
+                ldsm4(ks + chunk_at<D>((lane & 7) + ((lane >> 4) << 3), 2 * k + ((lane >> 3) & 1)), b);
+                mma16816<T>(sc[0], qf[k], b[0], b[1]);
+                mma16816<T>(sc[1], qf[k], b[2], b[3]);
+            }
+            const int64_t k0 = (u.first_tile + t) * KEYS + warp * 16;
+            float top[2] = { -INFINITY, -INFINITY };
+#pragma unroll
+            for (int n = 0; n < 2; n++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int64_t key = k0 + n * 8 + (lane % 4) * 2 + (e & 1);
+                    const int i = e >> 1;
+                    sc[n][e] = key <= pos[i] && key >= lo[i] ? sc[n][e] * scale_log2 : -INFINITY;
+                    top[i] = fmaxf(top[i], sc[n][e]);
+                }
+            if (__any_sync(0xFFFFFFFFu, top[0] > m[0] + k_lag || top[1] > m[1] + k_lag)) {
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    top[i] = fmaxf(top[i], __shfl_xor_sync(0xFFFFFFFFu, top[i], 1));
+                    top[i] = fmaxf(top[i], __shfl_xor_sync(0xFFFFFFFFu, top[i], 2));
+                    const float mn = fmaxf(m[i], top[i]), f = ex2(m[i] - mn);
+                    m[i] = mn;
+                    l[2 * i] *= f;
+#pragma unroll
+                    for (int d = 0; d < D / 8; d++) {
+                        o[d][2 * i] *= f;
+                        o[d][2 * i + 1] *= f;
+                    }
+                }
+            }
+            uint32_t p[4];
+#pragma unroll
+            for (int n = 0; n < 2; n++)
+#pragma unroll
+                for (int i = 0; i < 2; i++)
+                    p[2 * n + i] = num<T>::pack(ex2(sc[n][2 * i] - m[i]), ex2(sc[n][2 * i + 1] - m[i]));
+            mma16816<T>(l, p, num<T>::one2, num<T>::one2);
+#pragma unroll
+            for (int d = 0; d < D / 16; d++) {
+                uint32_t b[4];
+                ldsm4t(vs + chunk_at<D>((lane & 7) + (((lane >> 3) & 1) << 3), 2 * d + (lane >> 4)), b);
+                mma16816<T>(o[2 * d], p, b[0], b[1]);
+                mma16816<T>(o[2 * d + 1], p, b[2], b[3]);
+            }
+            __syncwarp();
+            stage = stage + 1 == ST ? 0 : stage + 1;
+        }
+        cp_wait<0>();
+        __syncthreads();
+
+        // join the four warps: [warp][row][D + 4] outputs, then maxima and sums
+        float * jm = join + 4 * ROWS * (D + 4), * jl = jm + 4 * ROWS;
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const int r = lane / 4 + 8 * i;
+            if (lane % 4 == 0) {
+                jm[warp * ROWS + r] = m[i];
+                jl[warp * ROWS + r] = l[2 * i];
+            }
+#pragma unroll
+            for (int d = 0; d < D / 8; d++)
+                *reinterpret_cast<float2 *>(join + (warp * ROWS + r) * (D + 4) + d * 8 + (lane % 4) * 2) =
+                    make_float2(o[d][2 * i], o[d][2 * i + 1]);
+        }
+        __syncthreads();
+        const int rows = (int) min((int64_t) ROWS, R - r0);
+        const bool whole = t0 == 0 && t1 == u.key_tiles;
+        float * part = parts + ((int64_t) c * 2 + (t0 == 0)) * A_PART;   // an item that began here, or before
+        for (int i = tid; i < rows * D; i += 128) {
+            const int r = i / D, d = i % D;
+            float mx = jm[r];
+#pragma unroll
+            for (int w = 1; w < 4; w++) mx = fmaxf(mx, jm[w * ROWS + r]);
+            float num_ = 0, den = 0;
+#pragma unroll
+            for (int w = 0; w < 4; w++) {
+                const float f = ex2(jm[w * ROWS + r] - mx);
+                num_ += f * join[(w * ROWS + r) * (D + 4) + d];
+                den += f * jl[w * ROWS + r];
+            }
+            if (whole) {
+                const int64_t gr = r0 + r;
+                dst[(S.first + gr / G) * dst_ld + ((int64_t) h * G + gr % G) * D + d] = num<T>::from(den > 0 ? num_ / den : 0.0f);
+            } else {
+                part[r * D + d] = num_;
+                if (d == 0) {
+                    part[ROWS * MAX_DIM + r] = mx;
+                    part[ROWS * MAX_DIM + ROWS + r] = den;
+                }
+            }
+        }
+        if (!whole) {
+            // CTA b holds unit y where W b / N <= y: the ones that share the item
+            const int64_t y1 = item0 + u.key_tiles - 1;
+            const int c0 = (int) (((item0 + 1) * N - 1) / W), c1 = (int) (((y1 + 1) * N - 1) / W);
+            __threadfence();
+            __syncthreads();
+            if (tid == 0) s_last = atomicAdd(&counters[c0], 1) == c1 - c0;
+            __syncthreads();
+            if (s_last) {
+                __threadfence();
+                for (int i = tid; i < rows * D; i += 128) {
+                    const int r = i / D, d = i % D;
+                    float mx = k_none, num_ = 0, den = 0;
+                    for (int b = c0; b <= c1; b++) {
+                        const float * pb = parts + ((int64_t) b * 2 + (b == c0)) * A_PART;
+                        const float mb = __ldcg(pb + ROWS * MAX_DIM + r), mn = fmaxf(mx, mb);
+                        const float f = ex2(mx - mn), g = ex2(mb - mn);
+                        num_ = num_ * f + g * __ldcg(pb + r * D + d);
+                        den = den * f + g * __ldcg(pb + ROWS * MAX_DIM + ROWS + r);
+                        mx = mn;
+                    }
+                    const int64_t gr = r0 + r;
+                    dst[(S.first + gr / G) * dst_ld + ((int64_t) h * G + gr % G) * D + d] =
+                        num<T>::from(den > 0 ? num_ / den : 0.0f);
+                }
+                if (tid == 0) counters[c0] = 0;
+            }
+        }
+        __syncthreads();                                          // the ring is free again
+        x = item0 + t1;
+    }
+}
+
+// ============================ sampling =====================================
+//
+// One CTA a row.  The cut of the sorted order -- a key, and how many of the
+// tokens that share it -- is found without sorting: by radix selection over
+// the 32-bit order-preserving keys, by count for top-k, by mass for top-p.
+
+constexpr int S_THREADS = 512, S_WARPS = S_THREADS / 32;
+
+__device__ __forceinline__ uint32_t order_key(float x) {          // x is no NaN, -0 is +0
+    const uint32_t b = __float_as_uint(x);
+    return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+// w in units of 2^-40; w in [0, 1]
+__device__ __forceinline__ unsigned long long mass_of(float w) {
+    const uint32_t b = __float_as_uint(w);
+    const int e = (int) (b >> 23) - 110;                          // w = mant * 2^(e - 40)
+    const unsigned long long mant = (b & 0x7FFFFFu) | 0x800000u;
+    if (e >= 0) return mant << e;
+    return e > -24 ? mant >> -e : 0ull;
+}
+
+struct sample_par {
+    float    inv_t, top_p, min_p, u;
+    int      k;
+    bool     greedy;
+};
+
+template <class T>
+__global__ void __launch_bounds__(S_THREADS)
+k_sample(const T * __restrict__ logits, int64_t ld, int V, const float * __restrict__ temperature,
+         const int32_t * __restrict__ top_k, const float * __restrict__ top_p, const float * __restrict__ min_p,
+         const float * __restrict__ u, int32_t * __restrict__ token, float * __restrict__ prob) {
+    using ull = unsigned long long;
+    __shared__ ull s_mass[256];
+    __shared__ float s_f[S_WARPS];
+    __shared__ ull s_w[S_WARPS];
+    __shared__ int s_i[S_WARPS];
+    __shared__ uint32_t s_key;
+    __shared__ ull s_above;
+    pdl_entry();
+    const int64_t row = blockIdx.x;
+    const T * x = logits + row * ld;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    sample_par p;
+    const float t = temperature ? temperature[row] : 1.0f;
+    p.greedy = !(t > 0.0f);
+    p.inv_t = 1.0f / t;
+    p.k = top_k ? top_k[row] : 0;
+    if (p.k <= 0 || p.k > V) p.k = V;
+    p.top_p = top_p ? top_p[row] : 1.0f;
+    p.min_p = min_p ? fminf(min_p[row], 1.0f) : 0.0f;             // the largest always stays
+    if (p.min_p != p.min_p) p.min_p = 0.0f;
+    p.u = u[row];
+    auto value = [&](int i) {
+        const float v = num<T>::to(x[i]);
+        return v != v ? -INFINITY : v + 0.0f;
+    };
+    // the maximum
+    float top = -INFINITY;
+    for (int i = tid; i < V; i += S_THREADS) top = fmaxf(top, value(i));
+#pragma unroll
+    for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
+    if (lane == 0) s_f[warp] = top;
+    __syncthreads();
+    for (int w = 0; w < S_WARPS; w++) top = fmaxf(top, s_f[w]);
+    if (top == -INFINITY) {
+        if (tid == 0) {
+            token[row] = -1;
+            if (prob) prob[row] = 0.0f;
+        }
+        return;
+    }
+    auto weight = [&](float v) { return v == top ? 1.0f : expf((v - top) * p.inv_t); };
+    uint32_t cut = 0;                         // kept: key > cut, and the first `ties` of key == cut
+    ull ties = (ull) V;
+    if (p.greedy) {
+        cut = order_key(top);
+        ties = 1;
+    } else {
+        // selection by count, then by mass: the largest key at which what lies above is < need
+        ull whole = 0;
+        for (int by_mass = 0; by_mass < 2; by_mass++) {
+            if (by_mass == 0 ? p.k >= V : !(p.top_p < 1.0f)) continue;
+            if (by_mass) {                                        // the mass of what top-k left
+                ull m = 0;
+                for (int i = tid; i < V; i += S_THREADS) {
+                    const float v = value(i);
+                    if (order_key(v) > cut) m += mass_of(weight(v));
+                }
+#pragma unroll
+                for (int d = 16; d; d >>= 1) m += __shfl_xor_sync(0xFFFFFFFFu, m, d);
+                __syncthreads();
+                if (lane == 0) s_w[warp] = m;
+                __syncthreads();
+                whole = 0;
+                for (int w = 0; w < S_WARPS; w++) whole += s_w[w];
+                if (p.k < V) {
+                    const float vc = __uint_as_float(cut & 0x80000000u ? cut & 0x7FFFFFFFu : ~cut);
+                    whole += ties * mass_of(weight(vc));
+                }
+            }
+            uint32_t prefix = 0, mask = 0;
+            // what lies above must be <= limit (count: k - 1; mass: below top_p * whole)
+            ull limit = (ull) (p.k - 1);
+            if (by_mass) {
+                const double want = (double) p.top_p * (double) whole;
+                limit = want > 0 ? (ull) ceil(want) - (ceil(want) > 0 ? 1 : 0) : 0;
+            }
+            ull above = 0;
+            for (int shift = 24; shift >= 0; shift -= 8) {
+                __syncthreads();
+                for (int i = tid; i < 256; i += S_THREADS) s_mass[i] = 0;
+                __syncthreads();
+                for (int i = tid; i < V; i += S_THREADS) {
+                    const float v = value(i);
+                    const uint32_t k = order_key(v);
+                    if ((k & mask) == prefix && k >= cut) {
+                        const ull a = by_mass ? mass_of(weight(v)) : 1ull;
+                        if (a) atomicAdd(&s_mass[(k >> shift) & 255], a);
+                    }
+                }
+                __syncthreads();
+                if (tid == 0) {
+                    // the lowest bucket that what lies above it still allows
+                    int b = 255;
+                    ull run = above, at = above;
+                    int best = -1;
+                    for (; b >= 0; b--) {
+                        if (s_mass[b]) {
+                            if (run > limit) break;
+                            best = b;
+                            at = run;
+                        }
+                        run += s_mass[b];
+                    }
+                    s_key = prefix | ((uint32_t) best << shift);
+                    s_above = at;
+                }
+                __syncthreads();
+                prefix = s_key;
+                above = s_above;
+                mask |= 255u << shift;
+            }
+            ull n = limit - above + 1;                            // by count
+            if (by_mass) {
+                const float vc = __uint_as_float(prefix & 0x80000000u ? prefix & 0x7FFFFFFFu : ~prefix);
+                const ull w = mass_of(weight(vc));
+                n = (limit - above) / w + 1;
+            }
+            if (prefix > cut) {
+                cut = prefix;
+                ties = n;
+            } else {
+                ties = min(ties, n);
+            }
+        }
+    }
+    // in order of index: warp w takes a contiguous part of the row
+    const int part = (V + S_WARPS - 1) / S_WARPS;
+    const int i0 = min(warp * part, V), i1 = min(i0 + part, V);
+    int eq = 0;
+    for (int i = i0 + lane; i < i1; i += 32) eq += order_key(value(i)) == cut;
+#pragma unroll
+    for (int d = 16; d; d >>= 1) eq += __shfl_xor_sync(0xFFFFFFFFu, eq, d);
+    if (lane == 0) s_i[warp] = eq;
+    __syncthreads();
+    ull before = 0;
+    for (int w = 0; w < warp; w++) before += s_i[w];
+    auto kept = [&](int i, bool in, ull & rank, float & w) {       // all lanes; rank: ties before this step
+        float v = -INFINITY;
+        uint32_t k = 0;
+        if (in) {
+            v = value(i);
+            k = order_key(v);
+        }
+        const uint32_t tie = __ballot_sync(0xFFFFFFFFu, in && k == cut);
+        const bool keep = in && (k > cut || (k == cut && rank + __popc(tie & ((1u << lane) - 1)) < ties));
+        rank += __popc(tie);
+        w = keep ? weight(v) : 0.0f;
+        return keep && (p.greedy || w >= p.min_p) ? (p.greedy ? 1ull : mass_of(w)) : 0ull;
+    };
+    ull sum = 0, rank = before;
+    for (int i = i0; i < i1; i += 32) {
+        float w;
+        sum += kept(i + lane, i + lane < i1, rank, w);
+    }
+#pragma unroll
+    for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
+    __syncthreads();
+    if (lane == 0) s_w[warp] = sum;
+    __syncthreads();
+    ull total = 0, base = 0;
+    for (int w = 0; w < S_WARPS; w++) {
+        if (w < warp) base += s_w[w];
+        total += s_w[w];
+    }
+    const float uu = fminf(fmaxf(p.u, 0.0f), 1.0f);
+    ull goal = (ull) ((double) uu * (double) total);
+    if (goal >= total) goal = total - 1;
+    if (goal < base || goal >= base + sum) return;
+    // the warp that holds the token
+    rank = before;
+    for (int i = i0; i < i1; i += 32) {
+        float w;
+        ull a = kept(i + lane, i + lane < i1, rank, w), run = a;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const ull o = __shfl_up_sync(0xFFFFFFFFu, run, d);
+            if (lane >= d) run += o;
+        }
+        const bool hit = a && goal >= base + run - a && goal < base + run;
+        if (hit) {
+            token[row] = i + lane;
+            if (prob) prob[row] = p.greedy ? 1.0f : (float) ((double) w / ((double) total * 0x1p-40));
+        }
+        if (__any_sync(0xFFFFFFFFu, hit)) return;
+        base += __shfl_sync(0xFFFFFFFFu, run, 31);
+    }
+}
+
+// ============================ host =========================================
+
+bool paged_ok(const lnsb_paged_kv & a, int * st) {
+    *st = LNSB_E_INVALID;
+    const bool pow2 = a.page_size > 0 && (a.page_size & (a.page_size - 1)) == 0;
+    if (a.type != LNSB_TYPE_F16 && a.type != LNSB_TYPE_BF16) return false;
+    if (!pow2 || a.page_size < 8 || a.page_size > 1024) return false;
+    if (a.head_dim != 16 && a.head_dim != 32 && a.head_dim != 64 && a.head_dim != 128 && a.head_dim != 256) return false;
+    if (a.n_seqs < 0 || a.n_tokens < 0 || a.n_head_kv <= 0 || a.n_pages < 0 || a.table_ld < 0) return false;
+    if (a.max_kv < 0 || a.max_kv > a.table_ld * a.page_size) return false;
+    if (a.row_stride < a.head_dim || a.head_stride < a.head_dim || a.page_stride < a.head_dim) return false;
+    if (a.page_stride % 8 || a.row_stride % 8 || a.head_stride % 8) return false;
+    if ((reinterpret_cast<uintptr_t>(a.k_cache) | reinterpret_cast<uintptr_t>(a.v_cache)) % 16) return false;
+    if (a.n_tokens > 0 && a.n_seqs > 0 &&
+        (a.k_cache == nullptr || a.v_cache == nullptr || a.page_table == nullptr || a.q_start == nullptr || a.kv_len == nullptr))
+        return false;
+    *st = LNSB_E_TOO_LARGE;
+    if (a.max_kv > 0x7FFFFFFF || a.n_pages > 0x7FFFFFFF || a.n_tokens > 0x7FFFFFFF || a.n_seqs > 65536 || a.n_head_kv > 65535)
+        return false;
+    *st = 0;
+    return true;
+}
+paged view_of(const lnsb_paged_kv & a) {
+    paged P;
+    P.table = a.page_table;
+    P.q_start = a.q_start;
+    P.kv_len = a.kv_len;
+    P.table_ld = a.table_ld;
+    P.n_pages = a.n_pages;
+    P.n_tokens = a.n_tokens;
+    P.max_kv = a.max_kv;
+    P.page_stride = a.page_stride;
+    P.row_stride = a.row_stride;
+    P.head_stride = a.head_stride;
+    P.n_seqs = a.n_seqs;
+    P.page_shift = 31 - __builtin_clz((unsigned) a.page_size);
+    P.n_head_kv = a.n_head_kv;
+    return P;
+}
+
+template <class TI, class TC>
+void launch_append(const lnsb_paged_append_args & a, cudaStream_t s) {
+    const lnsb_paged_kv & c = a.kv;
+    const int64_t per = a.n_dims / 2 + (c.head_dim - a.n_dims);
+    const int64_t n = c.n_tokens * ((int64_t) (a.n_head + c.n_head_kv) * per + (int64_t) c.n_head_kv * c.head_dim);
+    const int64_t blocks = std::min<int64_t>((n + 255) / 256, k_sms * 64);
+    launch_k(k_paged_append<TI, TC>, dim3((unsigned) blocks), dim3(256), 0, s, view_of(c), static_cast<const TI *>(a.k),
+             static_cast<const TI *>(a.v), static_cast<const TI *>(a.q), static_cast<TC *>(a.q_out), a.cos_sin, a.k_ld, a.v_ld,
+             a.q_ld, a.q_out_ld, a.n_head, c.head_dim, a.n_dims, a.neox, static_cast<TC *>(c.k_cache),
+             static_cast<TC *>(c.v_cache));
+}
+
+constexpr int k_max_devices = 64;
+
+template <class T, int D>
+int launch_rows(const lnsb_paged_attn_args & a, cudaStream_t s) {
+    auto kern = k_paged_attn_rows<T, D>;
+    static bool attr[k_max_devices] = {};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return (int) e;
+    if (dev < 0 || dev >= k_max_devices) return LNSB_E_NO_DEVICE;
+    if (!attr[dev]) {
+        e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, a_smem<D>());
+        if (e != cudaSuccess) return (int) e;
+        attr[dev] = true;
+    }
+    unsigned char * w = static_cast<unsigned char *>(a.work);
+    launch_k(kern, dim3(A_CTAS), dim3(128), (size_t) a_smem<D>(), s, view_of(a.kv), static_cast<const T *>(a.q),
+             static_cast<T *>(a.dst), static_cast<const T *>(a.kv.k_cache), static_cast<const T *>(a.kv.v_cache), a.q_ld,
+             a.dst_ld, a.n_head / a.kv.n_head_kv, a.scale * 1.44269504088896340736f, a.window, reinterpret_cast<int *>(w),
+             reinterpret_cast<float *>(w + A_COUNT_BYTES));
+    return launch_status();
+}
+template <class T>
+int launch_attn(const lnsb_paged_attn_args & a, cudaStream_t s) {
+    switch (a.kv.head_dim) {
+        case 16:  return launch_rows<T, 16>(a, s);
+        case 32:  return launch_rows<T, 32>(a, s);
+        case 64:  return launch_rows<T, 64>(a, s);
+        case 128: return launch_rows<T, 128>(a, s);
+        default:  return launch_rows<T, 256>(a, s);
+    }
+}
+
+}  // namespace
+}  // namespace lnsb
+
+using namespace lnsb;
+
+extern "C" {
+
+int lnsb_paged_append(const lnsb_paged_append_args * a, lnsb_stream_t stream) {
+    if (a == nullptr) return LNSB_E_INVALID;
+    int st = 0;
+    if (!paged_ok(a->kv, &st)) return st;
+    const lnsb_paged_kv & c = a->kv;
+    const int nh = a->q != nullptr ? a->n_head : 0;
+    if ((a->q == nullptr) != (a->q_out == nullptr) || a->n_head < 0 || (a->q != nullptr && a->n_head == 0)) return LNSB_E_INVALID;
+    if (a->n_dims < 0 || a->n_dims % 2 != 0 || a->n_dims > c.head_dim || (a->n_dims > 0 && a->cos_sin == nullptr))
+        return LNSB_E_INVALID;
+    if (a->in_type != LNSB_TYPE_F32 && a->in_type != LNSB_TYPE_F16 && a->in_type != LNSB_TYPE_BF16) return LNSB_E_INVALID;
+    const int64_t kvw = (int64_t) c.n_head_kv * c.head_dim, qw = (int64_t) nh * c.head_dim;
+    if (a->k_ld < kvw || a->v_ld < kvw || (nh > 0 && (a->q_ld < qw || a->q_out_ld < qw))) return LNSB_E_INVALID;
+    if (c.n_tokens == 0 || c.n_seqs == 0) return 0;
+    if (a->k == nullptr || a->v == nullptr) return LNSB_E_INVALID;
+    lnsb_paged_append_args b = *a;
+    b.n_head = nh;
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const bool f16 = c.type == LNSB_TYPE_F16;
+    switch (a->in_type) {
+        case LNSB_TYPE_F32:
+            if (f16) launch_append<float, __half>(b, s); else launch_append<float, __nv_bfloat16>(b, s);
+            break;
+        case LNSB_TYPE_F16:
+            if (f16) launch_append<__half, __half>(b, s); else launch_append<__half, __nv_bfloat16>(b, s);
+            break;
+        default:
+            if (f16) launch_append<__nv_bfloat16, __half>(b, s); else launch_append<__nv_bfloat16, __nv_bfloat16>(b, s);
+    }
+    return launch_status();
+}
+
+int64_t lnsb_paged_attn_work_bytes(void) { return A_WORK; }
+
+int lnsb_paged_attn(const lnsb_paged_attn_args * a, lnsb_stream_t stream) {
+    if (a == nullptr) return LNSB_E_INVALID;
+    int st = 0;
+    if (!paged_ok(a->kv, &st)) return st;
+    const lnsb_paged_kv & c = a->kv;
+    if (a->n_head <= 0 || a->n_head % c.n_head_kv != 0 || a->max_q < 0 || a->window < 0) return LNSB_E_INVALID;
+    const int64_t w = (int64_t) a->n_head * c.head_dim;
+    if (a->q_ld < w || a->dst_ld < w || a->q_ld % 8 || a->dst_ld % 8) return LNSB_E_INVALID;
+    if ((reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->dst) | reinterpret_cast<uintptr_t>(a->work)) % 16)
+        return LNSB_E_INVALID;
+    if (c.n_tokens == 0 || c.n_seqs == 0) return 0;
+    if (a->q == nullptr || a->dst == nullptr || a->work == nullptr || a->work_bytes < lnsb_paged_attn_work_bytes())
+        return LNSB_E_INVALID;
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    return c.type == LNSB_TYPE_F16 ? launch_attn<__half>(*a, s) : launch_attn<__nv_bfloat16>(*a, s);
+}
+
+int lnsb_paged_errors(int64_t * bad_pages, int64_t * timeouts) {
+    unsigned long long v[2] = {}, zero[2] = {};
+    cudaError_t e = cudaDeviceSynchronize();
+    if (e == cudaSuccess) e = cudaMemcpyFromSymbol(v, g_paged_errors, sizeof(v));
+    if (e == cudaSuccess) e = cudaMemcpyToSymbol(g_paged_errors, zero, sizeof(zero));
+    if (e != cudaSuccess) return (int) e;
+    if (bad_pages) *bad_pages = (int64_t) v[0];
+    if (timeouts) *timeouts = (int64_t) v[1];
+    return 0;
+}
+
+int lnsb_sample(const lnsb_sample_args * a, lnsb_stream_t stream) {
+    if (a == nullptr || a->n_rows < 0 || a->n_vocab <= 0 || a->ld < a->n_vocab) return LNSB_E_INVALID;
+    if (a->type != LNSB_TYPE_F32 && a->type != LNSB_TYPE_F16 && a->type != LNSB_TYPE_BF16) return LNSB_E_INVALID;
+    if (a->n_rows == 0) return 0;
+    if (a->logits == nullptr || a->u == nullptr || a->token == nullptr) return LNSB_E_INVALID;
+    if (a->n_vocab > (1 << 20) || a->n_rows > 0x7FFFFFFF) return LNSB_E_TOO_LARGE;
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const dim3 grid((unsigned) a->n_rows);
+    const int V = (int) a->n_vocab;
+    if (a->type == LNSB_TYPE_F32)
+        launch_k(k_sample<float>, grid, dim3(S_THREADS), 0, s, static_cast<const float *>(a->logits), a->ld, V, a->temperature,
+                 a->top_k, a->top_p, a->min_p, a->u, a->token, a->prob);
+    else if (a->type == LNSB_TYPE_F16)
+        launch_k(k_sample<__half>, grid, dim3(S_THREADS), 0, s, static_cast<const __half *>(a->logits), a->ld, V,
+                 a->temperature, a->top_k, a->top_p, a->min_p, a->u, a->token, a->prob);
+    else
+        launch_k(k_sample<__nv_bfloat16>, grid, dim3(S_THREADS), 0, s, static_cast<const __nv_bfloat16 *>(a->logits), a->ld, V,
+                 a->temperature, a->top_k, a->top_p, a->min_p, a->u, a->token, a->prob);
+    return launch_status();
+}
+
+}  // extern "C"

@@ -252,6 +252,122 @@ class KernelSet:
         _lib.check(self.lib, "lnsb_f16_to_f32", self.lib.lnsb_f16_to_f32(_ptr(src), _ptr(dst), n, _stream(stream)))
 
 
+    # ---- serving many sequences from a paged KV cache (no LNS: any format, any mode) ----
+    def _paged(self, k_cache, v_cache, page_table, q_start, kv_len, max_kv, n_tokens):
+        """lnsb_paged_kv of caches [n_pages][page_size][n_head_kv][head_dim] (any strides, dims contiguous), F16 or
+        BF16, with the plan arrays page_table [n_seqs][pages], q_start [n_seqs + 1], kv_len [n_seqs] (int32)"""
+        ty = _type_id(k_cache)
+        n_pages, page_size, n_head_kv, head_dim = k_cache.shape
+        st = k_cache.stride()
+        _want(v_cache.dtype == k_cache.dtype and v_cache.shape == k_cache.shape and v_cache.stride() == st and st[3] == 1,
+              "k_cache and v_cache must have the same type, shape and strides, with contiguous heads")
+        n_seqs, table_ld = page_table.shape
+        _want(page_table.dtype == q_start.dtype == kv_len.dtype == _int32() and page_table.is_contiguous()
+              and q_start.is_contiguous() and kv_len.is_contiguous() and q_start.numel() == n_seqs + 1
+              and kv_len.numel() == n_seqs, "page_table [n_seqs][pages], q_start [n_seqs + 1] and kv_len [n_seqs] must be "
+              "contiguous int32")
+        return (k_cache.data_ptr(), v_cache.data_ptr(), st[0], st[1], st[2], page_table.data_ptr(), q_start.data_ptr(),
+                kv_len.data_ptr(), table_ld, n_pages, n_tokens, max_kv, n_seqs, ty, page_size, n_head_kv, head_dim, 0)
+
+    def paged_append(self, k, v, k_cache, v_cache, page_table, q_start, kv_len, max_kv, q=None, q_out=None, cos_sin=None,
+                     neox=False, stream=None):
+        """lnsb_paged_append: k, v [n_tokens][n_head_kv][head_dim] (F32, F16 or BF16; token rows any distance apart) into
+        the caches, k turned by cos_sin [rows][n_dims / 2][2] (F32; None: not turned); q [n_tokens][n_head][head_dim]
+        turned into q_out (of the caches' type)"""
+        T = k.shape[0]
+        _want(v.shape == k.shape and v.dtype == k.dtype and k.shape[1:] == k_cache.shape[2:] and _heads(k) and _heads(v),
+              "k and v must be [n_tokens][n_head_kv][head_dim] of one type, heads contiguous")
+        n_dims = 0
+        if cos_sin is not None:
+            n_dims = 2 * cos_sin.shape[1]
+            _want(cos_sin.dtype == _f32() and cos_sin.is_contiguous() and cos_sin.shape[0] >= max_kv
+                  and cos_sin.shape[2] == 2, "cos_sin must be contiguous F32 [rows >= max_kv][n_dims / 2][2]")
+        n_head = q_ld = qo_ld = 0
+        if q is not None:
+            n_head, q_ld = q.shape[1], q.stride(0)
+            _want(q_out is not None and q_out.shape == q.shape and q.dtype == k.dtype and q_out.dtype == k_cache.dtype
+                  and q.shape[0] == T and q.shape[2] == k.shape[2] and _heads(q) and _heads(q_out),
+                  "q must be [n_tokens][n_head][head_dim] of k's type, q_out the same of the caches' type")
+            qo_ld = q_out.stride(0)
+        a = _lib.PagedAppendArgs(*self._paged(k_cache, v_cache, page_table, q_start, kv_len, max_kv, T), k.data_ptr(),
+                                 v.data_ptr(), q.data_ptr() if n_head else None, q_out.data_ptr() if n_head else None,
+                                 cos_sin.data_ptr() if n_dims else None, k.stride(0), v.stride(0), q_ld, qo_ld,
+                                 _type_id(k), n_head, n_dims, 1 if neox else 0)
+        _lib.check(self.lib, "lnsb_paged_append", self.lib.lnsb_paged_append(ctypes.byref(a), _stream(stream)))
+
+    def paged_attn_work(self, device=None):
+        """a workspace for paged_attn on one stream (zeroed, as its first use wants it)"""
+        import torch
+        return torch.zeros(self.lib.lnsb_paged_attn_work_bytes(), dtype=torch.uint8, device=device or "cuda")
+
+    def paged_attn(self, q, k_cache, v_cache, page_table, q_start, kv_len, max_q, max_kv, dst, work, scale=None, window=0,
+                   stream=None):
+        """lnsb_paged_attn: q, dst [n_tokens][n_head][head_dim] of the caches' type; scale None: 1 / sqrt(head_dim);
+        window 0: every earlier row is visible"""
+        _want(q.dtype == dst.dtype == k_cache.dtype and q.shape == dst.shape and q.shape[2] == k_cache.shape[3]
+              and _heads(q) and _heads(dst), "q and dst must be [n_tokens][n_head][head_dim] of the caches' type, heads "
+              "contiguous")
+        T, n_head, D = q.shape
+        a = _lib.PagedAttnArgs(*self._paged(k_cache, v_cache, page_table, q_start, kv_len, max_kv, T), q.data_ptr(),
+                               dst.data_ptr(), work.data_ptr(), work.numel() * work.element_size(), q.stride(0),
+                               dst.stride(0), max_q, window, n_head, D ** -0.5 if scale is None else scale)
+        _lib.check(self.lib, "lnsb_paged_attn", self.lib.lnsb_paged_attn(ctypes.byref(a), _stream(stream)))
+
+    def paged_errors(self):
+        """(page ids outside the cache, waits that ran out) since the last call, on the current device"""
+        b, t = ctypes.c_int64(), ctypes.c_int64()
+        _lib.check(self.lib, "lnsb_paged_errors", self.lib.lnsb_paged_errors(ctypes.byref(b), ctypes.byref(t)))
+        return b.value, t.value
+
+    def sample(self, logits, u, token, prob=None, temperature=None, top_k=None, top_p=None, min_p=None, stream=None):
+        """lnsb_sample: the next token of every row of logits [n_rows][n_vocab] (F32, F16 or BF16; rows any distance
+        apart) from one number u [n_rows] in [0, 1); token int32 [n_rows], prob F32 [n_rows] or None; temperature,
+        top_p, min_p F32 [n_rows] and top_k int32 [n_rows], each or None"""
+        R, V = logits.shape
+        _want(logits.stride(1) == 1 or V == 1, "logits must have contiguous rows")
+        for t, d in ((u, _f32()), (token, _int32()), (prob, _f32()), (temperature, _f32()), (top_k, _int32()),
+                     (top_p, _f32()), (min_p, _f32())):
+            _want(t is None or (t.dtype == d and t.numel() == R and t.is_contiguous()),
+                  "u, prob, temperature, top_p, min_p must be F32 [n_rows], token and top_k int32 [n_rows]")
+        a = _lib.SampleArgs(logits.data_ptr(), *(t.data_ptr() if t is not None else None
+                                                 for t in (temperature, top_k, top_p, min_p, u, token, prob)),
+                            logits.stride(0) if R > 1 else V, R, V, _type_id(logits))
+        _lib.check(self.lib, "lnsb_sample", self.lib.lnsb_sample(ctypes.byref(a), _stream(stream)))
+
+
+def _want(ok, what):
+    if not ok:
+        raise ValueError(what)
+
+
+def _int32():
+    import torch
+    return torch.int32
+
+
+def _f32():
+    import torch
+    return torch.float32
+
+
+def _heads(t):
+    """[tokens][heads][dim] with a token's heads contiguous"""
+    return t.dim() == 3 and (t.stride(2) == 1 or t.shape[2] == 1) and (t.stride(1) == t.shape[2] or t.shape[1] == 1)
+
+
+_TYPE_IDS = {}
+
+
+def _type_id(t):
+    if not _TYPE_IDS:
+        import torch
+        _TYPE_IDS.update({torch.float32: _lib.TYPES["f32"], torch.float16: _lib.TYPES["f16"],
+                          torch.bfloat16: _lib.TYPES["bf16"]})
+    if t.dtype not in _TYPE_IDS:
+        raise ValueError("%s is none of F32, F16 and BF16" % t.dtype)
+    return _TYPE_IDS[t.dtype]
+
+
 def kernels(fmt=XLNS16, mode="base"):
     return KernelSet(fmt, mode)
 

@@ -72,6 +72,37 @@ class RopeArgs(ctypes.Structure):
                 ("neox", ctypes.c_int), ("dst", ctypes.c_void_p)]
 
 
+# lnsb_paged_kv, the first member of the two paged calls' arguments
+_PAGED_KV = [("k_cache", ctypes.c_void_p), ("v_cache", ctypes.c_void_p), ("page_stride", ctypes.c_int64),
+             ("row_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64), ("page_table", ctypes.c_void_p),
+             ("q_start", ctypes.c_void_p), ("kv_len", ctypes.c_void_p), ("table_ld", ctypes.c_int64),
+             ("n_pages", ctypes.c_int64), ("n_tokens", ctypes.c_int64), ("max_kv", ctypes.c_int64),
+             ("n_seqs", ctypes.c_int), ("type", ctypes.c_int), ("page_size", ctypes.c_int), ("n_head_kv", ctypes.c_int),
+             ("head_dim", ctypes.c_int), ("_pad", ctypes.c_int)]
+
+
+class PagedAppendArgs(ctypes.Structure):
+    _fields_ = _PAGED_KV + [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("q", ctypes.c_void_p),
+                            ("q_out", ctypes.c_void_p), ("cos_sin", ctypes.c_void_p), ("k_ld", ctypes.c_int64),
+                            ("v_ld", ctypes.c_int64), ("q_ld", ctypes.c_int64), ("q_out_ld", ctypes.c_int64),
+                            ("in_type", ctypes.c_int), ("n_head", ctypes.c_int), ("n_dims", ctypes.c_int),
+                            ("neox", ctypes.c_int)]
+
+
+class PagedAttnArgs(ctypes.Structure):
+    _fields_ = _PAGED_KV + [("q", ctypes.c_void_p), ("dst", ctypes.c_void_p), ("work", ctypes.c_void_p),
+                            ("work_bytes", ctypes.c_int64), ("q_ld", ctypes.c_int64), ("dst_ld", ctypes.c_int64),
+                            ("max_q", ctypes.c_int64), ("window", ctypes.c_int64), ("n_head", ctypes.c_int),
+                            ("scale", ctypes.c_float)]
+
+
+class SampleArgs(ctypes.Structure):
+    _fields_ = [("logits", ctypes.c_void_p), ("temperature", ctypes.c_void_p), ("top_k", ctypes.c_void_p),
+                ("top_p", ctypes.c_void_p), ("min_p", ctypes.c_void_p), ("u", ctypes.c_void_p), ("token", ctypes.c_void_p),
+                ("prob", ctypes.c_void_p), ("ld", ctypes.c_int64), ("n_rows", ctypes.c_int64), ("n_vocab", ctypes.c_int64),
+                ("type", ctypes.c_int)]
+
+
 # (name, restype, argtypes) for every function of include/lnsb200.h
 _I64 = ctypes.c_int64
 _VP = ctypes.c_void_p
@@ -125,6 +156,11 @@ SIGNATURES = [
     ("lnsb_rope_qkv", ctypes.c_int, [ctypes.c_int, ctypes.POINTER(RopeQkvArgs), _VP]),
     ("lnsb_f32_to_f16", ctypes.c_int, [_VP, _VP, _I64, _VP]),
     ("lnsb_f16_to_f32", ctypes.c_int, [_VP, _VP, _I64, _VP]),
+    ("lnsb_paged_append", ctypes.c_int, [ctypes.POINTER(PagedAppendArgs), _VP]),
+    ("lnsb_paged_attn", ctypes.c_int, [ctypes.POINTER(PagedAttnArgs), _VP]),
+    ("lnsb_paged_attn_work_bytes", _I64, []),
+    ("lnsb_paged_errors", ctypes.c_int, [ctypes.POINTER(_I64), ctypes.POINTER(_I64)]),
+    ("lnsb_sample", ctypes.c_int, [ctypes.POINTER(SampleArgs), _VP]),
     ("lnsb_monte_get_state", ctypes.c_int, [ctypes.POINTER(ctypes.c_uint16)]),
     ("lnsb_monte_set_state", ctypes.c_int, [ctypes.c_uint16]),
     ("lnsb_monte_reserve", ctypes.c_int, [ctypes.c_uint64, ctypes.POINTER(ctypes.c_uint16)]),
