@@ -2,12 +2,15 @@
 // values, attention of the new tokens over the cache, sampling.  Ordinary
 // floating point, no LNS: the ops a host runs outside LNS.  The code does not
 // depend on the summation mode; every library of the build carries it.
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 #include <cstdint>
+#include <type_traits>
 
 #include "lnsb200.h"
 #include "lnsb_launch.cuh"
@@ -156,7 +159,7 @@ constexpr float k_none = -1e30f;               // the reference of a row that ha
 // work: [counters A_CTAS int32][partials A_CTAS * 2 * (ROWS * MAX_DIM + 2 * ROWS) float]
 constexpr int64_t A_PART = ROWS * MAX_DIM + 2 * ROWS;
 constexpr int64_t A_COUNT_BYTES = (A_CTAS * 4 + 255) / 256 * 256;
-constexpr int64_t A_WORK = A_COUNT_BYTES + (int64_t) A_CTAS * 2 * A_PART * 4;
+constexpr int64_t A_WORK = A_COUNT_BYTES + ((int64_t) A_CTAS * 2 * A_PART * 4 + 255) / 256 * 256;
 
 __device__ __forceinline__ uint32_t smem_addr(const void * p) { return (uint32_t) __cvta_generic_to_shared(p); }
 __device__ __forceinline__ void cp16(uint32_t dst, const void * src, bool valid) {
@@ -189,13 +192,18 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
+template <class T>
+__device__ __forceinline__ uint32_t pack2(uint32_t lo, uint32_t hi) {
+    return num<T>::pack(__uint_as_float(lo), __uint_as_float(hi));
+}
+
 // units of one sequence in the line: row tiles x kv heads x key tiles
 struct seq_units {
     int64_t row_tiles, key_tiles, first_tile;   // key tiles from first_tile on
 };
-__device__ __forceinline__ seq_units units_of(const seq_span & S, int G, int64_t window) {
+__device__ __forceinline__ seq_units units_of(const seq_span & S, int G, int64_t window, int64_t rows_most) {
     seq_units u;
-    u.row_tiles = (S.n * G + ROWS - 1) / ROWS;
+    u.row_tiles = S.n * G > rows_most ? 0 : (S.n * G + ROWS - 1) / ROWS;
     int64_t lo = 0;
     if (window > 0) lo = max((int64_t) 0, S.kv - S.n - window + 1);
     u.first_tile = lo / KEYS;
@@ -222,7 +230,7 @@ template <class T, int D>
 __global__ void __launch_bounds__(128)
 k_paged_attn_rows(paged P, const T * __restrict__ q, T * __restrict__ dst, const T * __restrict__ kc,
                   const T * __restrict__ vc, int64_t q_ld, int64_t dst_ld, int G, float scale_log2, int64_t window,
-                  int * __restrict__ counters, float * __restrict__ parts) {
+                  int64_t rows_most, int * __restrict__ counters, float * __restrict__ parts) {
     constexpr int ST = a_stages<D>(), SB = a_stage_bytes<D>(), CPR = D / 8, KS = D / 16;
     extern __shared__ __align__(128) unsigned char sm[];
     __shared__ int64_t s_scan[128];
@@ -236,7 +244,7 @@ k_paged_attn_rows(paged P, const T * __restrict__ q, T * __restrict__ dst, const
     const int s_lo = min(tid * per, P.n_seqs), s_hi = min(s_lo + per, P.n_seqs);
     int64_t mine = 0;
     for (int s = s_lo; s < s_hi; s++) {
-        const seq_units u = units_of(span_of(P, s), G, window);
+        const seq_units u = units_of(span_of(P, s), G, window, rows_most);
         mine += u.row_tiles * u.key_tiles * P.n_head_kv;
     }
     s_scan[tid] = mine;
@@ -260,12 +268,12 @@ k_paged_attn_rows(paged P, const T * __restrict__ q, T * __restrict__ dst, const
 
     while (x < x_end) {
         seq_span S = span_of(P, s);
-        seq_units u = units_of(S, G, window);
+        seq_units u = units_of(S, G, window, rows_most);
         int64_t len = u.row_tiles * u.key_tiles * P.n_head_kv;
         while (base + len <= x) {
             base += len;
             S = span_of(P, ++s);
-            u = units_of(S, G, window);
+            u = units_of(S, G, window, rows_most);
             len = u.row_tiles * u.key_tiles * P.n_head_kv;
         }
         const int64_t item = (x - base) / u.key_tiles;           // (row tile, kv head) of the sequence
@@ -458,6 +466,658 @@ k_paged_attn_rows(paged P, const T * __restrict__ q, T * __restrict__ dst, const
         __syncthreads();                                          // the ring is free again
         x = item0 + t1;
     }
+}
+
+// ===================== attention: chunks ===================================
+//
+// Sequences with more than 16 rows (token, head of the group) go to the
+// tensor cores in tiles of 256 rows, two groups of 128, over tiles of 128
+// keys.  S = Q K^T of a group lands in 128 columns of TMEM, one row a lane;
+// the group's 128 threads read one row each, so maximum and sum need no other
+// thread, and write the weights back into the same columns as the 16-bit A
+// operand of P V, whose sum O stays in TMEM.
+//
+//   warps 0-3, 4-7  group 0, group 1: Q into shared memory, softmax, output
+//   warp 8          one thread issues every MMA: PV of a group's tile j, then
+//                   its QK of tile j + 1, one group after the other, so one
+//                   group's softmax runs under the other's products
+//   warp 9          TMA of K and V pages through a ring of 128-key tiles
+//   warp 10         walks the CTA's share of the line and hands out its items
+//   warp 11         nothing: it completes the warpgroup that gives registers to
+//                   the softmax (168 x 384 at launch = 208 x 256 + 88 x 128)
+//
+// TMEM operations of one thread run in the order of their issue: QK of tile
+// j + 1 may overwrite the weights that PV of tile j reads.  As with few rows,
+// the (row tile, kv head, key tile) units of all sequences form a line that
+// the CTAs cut into equal shares; each warp joins its own 32 rows of a cut
+// item, so no warp waits for another outside the mbarriers.
+//
+// Every wait gives up after k_wait_cycles: the CTA then drains what it has in
+// flight, frees its TMEM and counts a timeout.
+
+constexpr int B_ROWS = 128, B_TILE = 256, B_KEYS = 128, B_THREADS = 384, B_SUMS = 256, B_ITEMS = 4, B_CTAS = k_sms;
+constexpr long long k_wait_cycles = 1ll << 31;
+
+// partials: [slot][group][warp][d / 4][lane] float4, then [warp][lane] (m, l)
+constexpr int64_t B_PART = (int64_t) B_TILE * (128 + 2);
+constexpr int64_t B_COUNT_BYTES = ((int64_t) B_CTAS * 8 * 4 + 255) / 256 * 256;
+constexpr int64_t B_WORK = B_COUNT_BYTES + (int64_t) B_CTAS * 2 * B_PART * 4;
+
+// ---- mbarriers, TMA, tcgen05 ----
+__device__ __forceinline__ void bar_init(uint32_t bar, uint32_t count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;\n" :: "r"(bar), "r"(count) : "memory");
+}
+__device__ __forceinline__ void bar_arrive(uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" :: "r"(bar) : "memory");
+}
+__device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" :: "r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}\n"
+                 : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return ok != 0;
+}
+// false: the CTA gives up (this wait ran out, or another one did)
+__device__ __forceinline__ bool bar_wait_slow(uint32_t bar, uint32_t parity, volatile int * stop) {
+    const long long t0 = clock64();
+    while (!bar_try(bar, parity)) {
+        if (*stop) return false;
+        if (clock64() - t0 > k_wait_cycles) {
+            *stop = 1;
+            return false;
+        }
+    }
+    return true;
+}
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int * stop) {
+    return bar_try(bar, parity) || bar_wait_slow(bar, parity, stop);
+}
+// the same for a whole warp: all its lanes go on, or none
+__device__ __forceinline__ bool bar_wait_warp(uint32_t bar, uint32_t parity, volatile int * stop) {
+    return __all_sync(0xFFFFFFFFu, bar_wait(bar, parity, stop));
+}
+__device__ __forceinline__ void tma_page(uint32_t dst, const CUtensorMap * map, int d, int row, int head, int page, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];\n"
+                 :: "r"(dst), "l"(map), "r"(d), "r"(row), "r"(head), "r"(page), "r"(bar) : "memory");
+}
+// operand in shared memory, 128-byte swizzle: start, stride between the
+// 64-element halves (major dimension outside), stride between groups of 8 rows
+__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lead, uint32_t stride) {
+    return (uint64_t) ((addr & 0x3FFFF) >> 4) | ((uint64_t) (lead >> 4) << 16) | ((uint64_t) (stride >> 4) << 32) |
+           (1ull << 46) | (2ull << 61);
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n"
+                 :: "r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t) add) : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n"
+                 :: "r"(d), "r"(a), "l"(b), "r"(idesc), "r"((uint32_t) add) : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n" :: "r"(bar) : "memory");
+}
+__device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory"); }
+__device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory"); }
+// the loads of v are complete; v is used only behind this
+template <int N> __device__ __forceinline__ void tc_wait_ld(uint32_t (&v)[N]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < N; i++) asm volatile("" : "+r"(v[i]));
+}
+__device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory"); }
+#define LNSB_R4(v, i) "=r"(v[i]), "=r"(v[i + 1]), "=r"(v[i + 2]), "=r"(v[i + 3])
+#define LNSB_W4(v, i) "r"(v[i]), "r"(v[i + 1]), "r"(v[i + 2]), "r"(v[i + 3])
+// 32 columns of the warp's 32 lanes
+__device__ __forceinline__ void tc_ld32(uint32_t a, uint32_t * v) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+                 "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n"
+                 : LNSB_R4(v, 0), LNSB_R4(v, 4), LNSB_R4(v, 8), LNSB_R4(v, 12), LNSB_R4(v, 16), LNSB_R4(v, 20), LNSB_R4(v, 24),
+                   LNSB_R4(v, 28) : "r"(a));
+}
+__device__ __forceinline__ void tc_st32(uint32_t a, const uint32_t * v) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
+                 "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};\n"
+                 :: "r"(a), LNSB_W4(v, 0), LNSB_W4(v, 4), LNSB_W4(v, 8), LNSB_W4(v, 12), LNSB_W4(v, 16), LNSB_W4(v, 20),
+                    LNSB_W4(v, 24), LNSB_W4(v, 28) : "memory");
+}
+#undef LNSB_R4
+#undef LNSB_W4
+
+// ---- the line ----
+struct tile_plan {
+    int64_t rows_above, window;      // sequences of more rows than this
+    int     G;
+};
+// key tiles [lo, hi) of row tile rt of a sequence; one at least
+__device__ __forceinline__ void tile_keys(const tile_plan & L, const seq_span & S, int64_t rt, int64_t & lo, int64_t & n) {
+    const int64_t R = S.n * L.G, pos0 = S.kv - S.n;
+    const int64_t last = (min((rt + 1) * B_TILE, R) - 1) / L.G, first = rt * B_TILE / L.G;
+    const int64_t hi = (max(min(S.kv, pos0 + last + 1), (int64_t) 0) + B_KEYS - 1) / B_KEYS;
+    lo = L.window > 0 ? max((int64_t) 0, pos0 + first - L.window + 1) / B_KEYS : 0;
+    n = max((int64_t) 1, hi - lo);
+}
+__device__ __forceinline__ int64_t row_tiles_of(const tile_plan & L, const seq_span & S) {
+    const int64_t R = S.n * L.G;
+    return R > L.rows_above ? (R + B_TILE - 1) / B_TILE : 0;
+}
+// units of one kv head of a sequence, summed by the whole warp
+__device__ __forceinline__ int64_t units_by_warp(const tile_plan & L, const seq_span & S) {
+    const int64_t nr = row_tiles_of(L, S);
+    int64_t sum = 0;
+    for (int64_t rt = threadIdx.x & 31; rt < nr; rt += 32) {
+        int64_t lo, n;
+        tile_keys(L, S, rt, lo, n);
+        sum += n;
+    }
+#pragma unroll
+    for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
+    return sum;
+}
+// a CTA's part of one item
+struct tile_item {
+    int seq, head;                   // kv head
+    int first, kv, pos0;             // the sequence's first new token, its cached rows, cache row of the first new token
+    int r0, rows;                    // first row of the tile; all rows of the sequence
+    int key0, n;                     // first key, and how many key tiles (0: the share is done)
+    int cut, c0, others;             // part of an item that others share: their first CTA, and how many more there are
+};
+// walks the CTA's share [x, x_end) of the line; the whole warp takes part
+struct line_walk {
+    const int64_t * sums;            // units of each run of `per` sequences
+    int64_t per, W, N, x, x_end, base, run_base, seq_len;   // seq_len: units of sequence s, from base on
+    int     run, s;
+
+    __device__ void next(const paged & P, const tile_plan & L, tile_item & I) {
+        I.n = 0;
+        if (x >= x_end) return;
+        const int lane = threadIdx.x & 31;
+        // the run of sequences, then the sequence, that holds unit x
+        bool moved = seq_len < 0;
+        while (run_base + sums[run] <= x) {
+            run_base += sums[run++];
+            moved = true;
+        }
+        if (moved) {
+            s = (int) (run * per);
+            base = run_base;
+            seq_len = units_by_warp(L, span_of(P, s)) * P.n_head_kv;
+        }
+        while (base + seq_len <= x) {
+            base += seq_len;
+            seq_len = units_by_warp(L, span_of(P, ++s)) * P.n_head_kv;
+        }
+        const int64_t per_head = seq_len / P.n_head_kv;
+        const seq_span S = span_of(P, s);
+        I.seq = s;
+        I.head = (int) ((x - base) / per_head);
+        int64_t at = base + I.head * per_head, len = 1, lo0 = 0;   // the row tile's place on the line, its key tiles
+        const int64_t nr = row_tiles_of(L, S);
+        int64_t rt = 0;
+        for (int64_t r = 0; r < nr; r += 32) {
+            int64_t lo = 0, n = 0;
+            if (r + lane < nr) tile_keys(L, S, r + lane, lo, n);
+            int64_t upto = n;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const int64_t o = __shfl_up_sync(0xFFFFFFFFu, upto, d);
+                if (lane >= d) upto += o;
+            }
+            const uint32_t hit = __ballot_sync(0xFFFFFFFFu, r + lane < nr && at + upto > x);
+            if (hit) {
+                const int l = __ffs(hit) - 1;
+                rt = r + l;
+                lo0 = __shfl_sync(0xFFFFFFFFu, lo, l);
+                len = __shfl_sync(0xFFFFFFFFu, n, l);
+                at += __shfl_sync(0xFFFFFFFFu, upto, l) - len;
+                break;
+            }
+            at += __shfl_sync(0xFFFFFFFFu, upto, 31);
+        }
+        const int64_t t0 = x - at, t1 = min(len, x_end - at);
+        I.first = (int) S.first;
+        I.kv = (int) S.kv;
+        I.pos0 = (int) (S.kv - S.n);
+        I.r0 = (int) (rt * B_TILE);
+        I.rows = (int) (S.n * L.G);
+        I.key0 = (int) ((lo0 + t0) * B_KEYS);
+        I.n = (int) (t1 - t0);
+        I.cut = t0 > 0 || t1 < len;
+        // CTA b holds unit y where W b / N <= y
+        I.c0 = (int) (((at + 1) * N - 1) / W);
+        I.others = (int) (((at + len) * N - 1) / W) - I.c0;
+        x = at + t1;
+    }
+};
+
+// the first cache row that the sequence still owns: the window's of its first new token
+__device__ __forceinline__ int first_owned(const tile_item & I, const tile_plan & L) {
+    return L.window > 0 ? (int) max((int64_t) 0, I.pos0 - L.window + 1) : 0;
+}
+
+// shared memory of one CTA
+template <int D> __host__ __device__ constexpr int b_tile_bytes() { return B_KEYS * D * 2; }
+template <int D> __host__ __device__ constexpr int b_ring() { return D == 128 ? 5 : 10; }
+struct tile_control {                // behind the tiles
+    int64_t   sums[B_SUMS];
+    tile_item item[B_ITEMS];
+    uint64_t  bar[2 * 10 + 2 * B_ITEMS + 9];
+    uint32_t  tmem;
+    int       stop;
+};
+template <int D> __host__ __device__ constexpr int b_smem() {
+    return (2 + b_ring<D>()) * b_tile_bytes<D>() + (int) sizeof(tile_control);
+}
+static_assert(b_smem<128>() <= 227 * 1024 && b_smem<64>() <= 227 * 1024, "shared memory of one CTA");
+
+template <class T, int D>
+__global__ void __launch_bounds__(B_THREADS, 1)
+k_paged_attn_tiles(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, paged P, tile_plan L,
+                   const T * __restrict__ q, T * __restrict__ dst, int64_t q_ld, int64_t dst_ld, float scale_log2,
+                   int * __restrict__ counters, float * __restrict__ parts, int after_rows) {
+    constexpr int ST = b_ring<D>(), TB = b_tile_bytes<D>(), HB = B_KEYS * 128, HALVES = D / 64;
+    constexpr bool BF = std::is_same<T, __nv_bfloat16>::value;
+    // f32 sums of 16-bit operands, 128 rows; B of PV is [key][dim], keys outside
+    constexpr uint32_t fmt = (1u << 4) | ((BF ? 1u : 0u) << 7) | ((BF ? 1u : 0u) << 10) | (8u << 24);
+    constexpr uint32_t idesc_qk = fmt | ((B_KEYS / 8) << 17), idesc_pv = fmt | (1u << 16) | ((D / 8) << 17);
+    constexpr uint32_t S_COL = 0, O_COL = 256;              // + 128 g, + D g
+
+    extern __shared__ __align__(1024) unsigned char tile_sm[];     // swizzled tiles: 1024-byte boundaries
+    tile_control & C = *reinterpret_cast<tile_control *>(tile_sm + (2 + ST) * TB);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const uint32_t q_sm = smem_addr(tile_sm), ring = q_sm + 2 * TB;
+    const uint32_t bars = smem_addr(C.bar);
+    const uint32_t kv_full = bars, kv_empty = bars + 8 * ST, q_full = kv_empty + 8 * ST, s_full = q_full + 16,
+                   p_ready = s_full + 16, o_full = p_ready + 16, it_full = o_full + 16, it_empty = it_full + 8 * B_ITEMS, drained = it_empty + 8 * B_ITEMS;
+    volatile int * stop = &C.stop;
+
+    if (tid == 0) {
+        for (int i = 0; i < ST; i++) {
+            bar_init(kv_full + 8 * i, 1);
+            bar_init(kv_empty + 8 * i, 1);
+        }
+        for (int g = 0; g < 2; g++) {
+            bar_init(q_full + 8 * g, B_ROWS);
+            bar_init(s_full + 8 * g, 1);
+            bar_init(p_ready + 8 * g, B_ROWS);
+            bar_init(o_full + 8 * g, 1);
+        }
+        for (int i = 0; i < B_ITEMS; i++) {
+            bar_init(it_full + 8 * i, 1);
+            bar_init(it_empty + 8 * i, 10);                  // warps 0 .. 9
+        }
+        bar_init(drained, 1);
+        C.stop = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+    }
+    // behind k_paged_attn_rows of the same call this grid needs not wait at its
+    // start: that kernel let it launch after its own wait, and the two write
+    // different rows
+    if (!after_rows) asm volatile("griddepcontrol.wait;\n" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;\n" :::);
+
+    // the line's length
+    const int64_t per = (P.n_seqs + B_SUMS - 1) / B_SUMS;
+    int64_t mine = 0;
+    for (int64_t j = 0; j < (tid < B_SUMS ? per : 0); j++) {
+        const int64_t s = tid * per + j;
+        seq_span S = { 0, 0, 0 };
+        if (s < P.n_seqs) S = span_of(P, (int) s);
+        const int64_t nr = row_tiles_of(L, S);
+        int64_t u = 0;
+        if (nr <= 4)
+            for (int64_t rt = 0; rt < nr; rt++) {
+                int64_t lo, n;
+                tile_keys(L, S, rt, lo, n);
+                u += n;
+            }
+        for (uint32_t big = __ballot_sync(0xFFFFFFFFu, nr > 4); big; big &= big - 1) {
+            const int l = __ffs(big) - 1;
+            const seq_span X = { 0, __shfl_sync(0xFFFFFFFFu, S.n, l), __shfl_sync(0xFFFFFFFFu, S.kv, l) };
+            const int64_t sum = units_by_warp(L, X);
+            if (lane == l) u = sum;
+        }
+        mine += u;
+    }
+    if (tid < B_SUMS) C.sums[tid] = mine * P.n_head_kv;
+    __syncthreads();
+    int64_t W = 0;
+    for (int i = lane; i < B_SUMS; i += 32) W += C.sums[i];
+#pragma unroll
+    for (int d = 16; d; d >>= 1) W += __shfl_xor_sync(0xFFFFFFFFu, W, d);
+    const int64_t N = min((int64_t) gridDim.x, W);            // CTAs that get a share: one unit at least
+    const bool work = blockIdx.x < N;
+    if (work && warp == 8) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;\n" :: "r"(smem_addr(&C.tmem)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n");
+    }
+    tc_before();
+    __syncthreads();
+    tc_after();
+    if (work) {
+        const uint32_t tmem = C.tmem;
+        uint32_t items = 0;                                   // handed out
+        tile_item I;
+        // the next item of warps 0 .. 9; false: the share is done, or the CTA gives up
+        auto next_item = [&]() {
+            const uint32_t i = items % B_ITEMS;
+            if (!bar_wait_warp(it_full + 8 * i, (items / B_ITEMS) & 1, stop)) return false;
+            I = C.item[i];
+            __syncwarp();
+            if (lane == 0) bar_arrive(it_empty + 8 * i);
+            items++;
+            return I.n > 0;
+        };
+        if (warp >= 8) {
+            asm volatile("setmaxnreg.dec.sync.aligned.u32 88;\n" ::);
+        if (warp == 10) {
+            // ------------------------------------------------ items
+            line_walk walk;
+            walk.sums = C.sums;
+            walk.per = per;
+            walk.W = W;
+            walk.N = N;
+            walk.x = W * blockIdx.x / N;
+            walk.x_end = W * (blockIdx.x + 1) / N;
+            walk.base = walk.run_base = 0;
+            walk.seq_len = -1;
+            walk.run = walk.s = 0;
+            do {
+                const uint32_t i = items % B_ITEMS;
+                walk.next(P, L, I);
+                if (!bar_wait_warp(it_empty + 8 * i, ((items / B_ITEMS) & 1) ^ 1, stop)) break;
+                if (lane == 0) {
+                    C.item[i] = I;
+                    bar_arrive(it_full + 8 * i);
+                }
+                __syncwarp();
+                items++;
+            } while (I.n > 0);
+        } else if (warp == 9) {
+            // ------------------------------------------------ K and V pages
+            const int box = min(1 << P.page_shift, B_KEYS), boxes = B_KEYS / box;
+            uint32_t n = 0;                                  // buffers filled
+            bool ok = true;
+            while (ok && next_item()) {
+                const int seen = first_owned(I, L);
+                for (int t = 0; ok && t < I.n; t++) {
+                    const int64_t key = (int64_t) I.key0 + t * B_KEYS + lane * box;
+                    int64_t page = -1;
+                    if (lane < boxes && key < I.kv && key + box > seen) page = page_of(P, I.seq, key);
+                    if (page < 0) page = P.n_pages;          // out of bounds: zeros
+                    const int row = (int) (key & ((1 << P.page_shift) - 1));
+#pragma unroll
+                    for (int kv = 0; kv < 2; kv++, n++) {
+                        const uint32_t b = n % ST;
+                        if (!(ok = bar_wait_warp(kv_empty + 8 * b, ((n / ST) & 1) ^ 1, stop))) break;
+                        if (lane == 0) bar_expect(kv_full + 8 * b, TB);
+                        __syncwarp();
+                        if (lane < boxes)
+#pragma unroll
+                            for (int i = 0; i < HALVES; i++)
+                                tma_page(ring + b * TB + i * HB + lane * box * 128, kv ? &vmap : &kmap, 64 * i, row, I.head,
+                                         (int) page, kv_full + 8 * b);
+                    }
+                }
+            }
+            // nothing of this CTA's may be in flight when it ends
+            int none = 0;
+            for (uint32_t i = n > ST ? n - ST : 0; i < n; i++) (void) bar_wait(kv_full + 8 * (i % ST), (i / ST) & 1, &none);
+        } else if (warp == 8) {
+            // ------------------------------------------------ MMA
+            uint32_t n = 0;                                  // ring position of the item's first K
+            uint32_t np[2] = { 0, 0 }, nq[2] = { 0, 0 };     // phases of p_ready and q_full
+            bool ok = true;
+            while (ok && next_item()) {
+                const int groups = I.rows - I.r0 > B_ROWS ? 2 : 1;
+                const uint32_t nt = (uint32_t) I.n;
+                if (lane == 0) {
+                    auto qk = [&](int g, uint32_t i) {
+                        const uint32_t kb = ring + (i % ST) * TB, qb = q_sm + g * TB;
+#pragma unroll
+                        for (int k = 0; k < D / 16; k++) {
+                            const uint32_t off = (k / 4) * HB + (k % 4) * 32;
+                            mma_ss(tmem + S_COL + 128 * g, smem_desc(qb + off, 16, 1024), smem_desc(kb + off, 16, 1024),
+                                   idesc_qk, k > 0);
+                        }
+                        mma_commit(s_full + 8 * g);
+                    };
+                    ok = bar_wait(kv_full + 8 * (n % ST), (n / ST) & 1, stop);
+                    for (int g = 0; ok && g < groups; g++) {
+                        ok = bar_wait(q_full + 8 * g, nq[g]++ & 1, stop);
+                        tc_after();
+                        if (ok) qk(g, n);
+                    }
+                    if (ok) mma_commit(kv_empty + 8 * (n % ST));
+                    for (uint32_t j = 0; ok && j < nt; j++) {
+                        const uint32_t v = n + 2 * j + 1, k = v + 1;
+                        const uint32_t vb = ring + (v % ST) * TB;
+                        ok = bar_wait(kv_full + 8 * (v % ST), (v / ST) & 1, stop);
+                        for (int g = 0; ok && g < groups; g++) {
+                            if (!(ok = bar_wait(p_ready + 8 * g, np[g]++ & 1, stop))) break;
+                            tc_after();
+#pragma unroll
+                            for (int kk = 0; kk < B_KEYS / 16; kk++)
+                                mma_ts(tmem + O_COL + D * g, tmem + S_COL + 128 * g + 8 * kk,
+                                       smem_desc(vb + kk * 2048, HB, 1024), idesc_pv, j > 0 || kk > 0);
+                            if (j + 1 < nt) {
+                                if (g == 0 && !(ok = bar_wait(kv_full + 8 * (k % ST), (k / ST) & 1, stop))) break;
+                                qk(g, k);
+                            } else {
+                                mma_commit(o_full + 8 * g);
+                            }
+                        }
+                        if (ok) {
+                            mma_commit(kv_empty + 8 * (v % ST));
+                            if (j + 1 < nt) mma_commit(kv_empty + 8 * (k % ST));
+                        }
+                    }
+                }
+                n += 2 * nt;
+                ok = __shfl_sync(0xFFFFFFFFu, ok, 0);
+            }
+            if (lane == 0) {
+                int none = 0;
+                mma_commit(drained);
+                (void) bar_wait(drained, 0, &none);
+            }
+            __syncwarp();
+        }
+        } else {
+            asm volatile("setmaxnreg.inc.sync.aligned.u32 208;\n" ::);
+            // ------------------------------------------------ softmax and output
+            const int g = warp >> 2, row = tid & 127;
+            const uint32_t lanes = (uint32_t) (warp & 3) << 21;      // TMEM lane 32 (warp % 4)
+            const uint32_t s_at = tmem + lanes + S_COL + 128 * g, o_at = tmem + lanes + O_COL + D * g;
+            uint32_t ns = 0, no = 0;                                 // phases of s_full and o_full
+            uint32_t n = 0;
+            bool ok = true;
+            while (ok && next_item()) {
+                const uint32_t nt = (uint32_t) I.n, ring0 = n;
+                n += 2 * nt;
+                const int r = I.r0 + B_ROWS * g + row;
+                if (I.r0 + B_ROWS * g >= I.rows) continue;           // no rows for this group
+                const bool live = r < I.rows;
+                const int64_t tok = I.first + r / L.G;
+                const int head = I.head * L.G + r % L.G;
+                {
+                    const uint4 * src = reinterpret_cast<const uint4 *>(q + tok * q_ld + (int64_t) head * D);
+                    const uint32_t qb = q_sm + g * TB + row * 128;
+                    uint4 v[D / 8];
+#pragma unroll
+                    for (int i = 0; i < D / 8; i++) v[i] = live ? __ldg(src + i) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+                    for (int i = 0; i < D / 8; i++)
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n"
+                                     :: "r"(qb + (i / 8) * HB + (((i % 8) ^ (row & 7)) << 4)), "r"(v[i].x), "r"(v[i].y),
+                                        "r"(v[i].z), "r"(v[i].w) : "memory");
+                    asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+                    bar_arrive(q_full + 8 * g);
+                }
+                // the tile's first and last row, and this thread's
+                const int pos_a = I.pos0 + (I.r0 + B_ROWS * g) / L.G;
+                const int pos_z = I.pos0 + (min(I.r0 + B_ROWS * g + B_ROWS, I.rows) - 1) / L.G;
+                const int pos = I.pos0 + r / L.G;
+                const int seen = first_owned(I, L);
+                float m = k_none, l = 0.0f;
+                for (uint32_t j = 0; j < nt; j++) {
+                    const int k0 = I.key0 + (int) j * B_KEYS;
+                    if (!(ok = bar_wait_warp(s_full + 8 * g, ns++ & 1, stop))) break;
+                    tc_after();
+                    uint32_t sv[128];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) tc_ld32(s_at + 32 * i, sv + 32 * i);
+                    tc_wait_ld(sv);
+                    if (k0 + B_KEYS - 1 > pos_a || (L.window > 0 && k0 <= pos_z - L.window)) {
+                        const int hi = pos - k0;                     // columns lo .. hi
+                        const int lo = L.window > 0 ? (int) max(pos - L.window + 1 - k0, (int64_t) 0) : 0;
+#pragma unroll
+                        for (int i = 0; i < 128; i++)
+                            if (i > hi || i < lo) sv[i] = 0xFF800000u;
+                    }
+                    float top = __uint_as_float(sv[0]);
+#pragma unroll
+                    for (int i = 1; i < 128; i++) top = fmaxf(top, __uint_as_float(sv[i]));
+                    top *= scale_log2;
+                    if (__any_sync(0xFFFFFFFFu, top > m + k_lag)) {
+                        const float mn = fmaxf(m, top), f = ex2(m - mn);
+                        m = mn;
+                        l *= f;
+                        if (j > 0) {
+#pragma unroll
+                            for (int i = 0; i < D / 32; i++) {
+                                uint32_t ov[32];
+                                tc_ld32(o_at + 32 * i, ov);
+                                tc_wait_ld(ov);
+#pragma unroll
+                                for (int e = 0; e < 32; e++) ov[e] = __float_as_uint(__uint_as_float(ov[e]) * f);
+                                tc_st32(o_at + 32 * i, ov);
+                            }
+                        }
+                    }
+                    float add[4] = { 0, 0, 0, 0 };
+#pragma unroll
+                    for (int i = 0; i < 2; i++) {
+                        uint32_t pv[32];
+#pragma unroll
+                        for (int e = 0; e < 32; e++) {
+                            const float a = ex2(fmaf(__uint_as_float(sv[64 * i + 2 * e]), scale_log2, -m));
+                            const float b = ex2(fmaf(__uint_as_float(sv[64 * i + 2 * e + 1]), scale_log2, -m));
+                            add[2 * (e & 1)] += a;
+                            add[2 * (e & 1) + 1] += b;
+                            pv[e] = num<T>::pack(a, b);
+                        }
+                        tc_st32(s_at + 32 * i, pv);
+                    }
+                    l += (add[0] + add[1]) + (add[2] + add[3]);
+                    // rows of V that the sequence does not own may hold anything: weight 0 must meet 0
+                    if (k0 + B_KEYS > I.kv || k0 < seen) {
+                        const uint32_t i = ring0 + 2 * j + 1;
+                        if (!(ok = bar_wait_warp(kv_full + 8 * (i % ST), (i / ST) & 1, stop))) break;
+                        if (k0 + row >= I.kv || k0 + row < seen) {
+                            const uint32_t vb = ring + (i % ST) * TB + row * 128;
+#pragma unroll
+                            for (int c = 0; c < D / 8; c++)
+                                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};\n"
+                                             :: "r"(vb + (c / 8) * HB + (c % 8) * 16), "r"(0) : "memory");
+                        }
+                        asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+                    }
+                    tc_wait_st();
+                    tc_before();
+                    bar_arrive(p_ready + 8 * g);
+                }
+                if (!ok || !(ok = bar_wait_warp(o_full + 8 * g, no++ & 1, stop))) break;
+                tc_after();
+                // 32 dims at a time: o becomes the row's outputs
+                auto put = [&](int i, uint32_t (&o)[32], float inv) {
+                    uint4 * out = reinterpret_cast<uint4 *>(dst + tok * dst_ld + (int64_t) head * D + 32 * i);
+#pragma unroll
+                    for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * inv);
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        out[e] = make_uint4(pack2<T>(o[8 * e], o[8 * e + 1]), pack2<T>(o[8 * e + 2], o[8 * e + 3]),
+                                            pack2<T>(o[8 * e + 4], o[8 * e + 5]), pack2<T>(o[8 * e + 6], o[8 * e + 7]));
+                };
+                if (!I.cut) {
+                    const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+#pragma unroll 1
+                    for (int i = 0; i < D / 32; i++) {
+                        uint32_t o[32];
+                        tc_ld32(o_at + 32 * i, o);
+                        tc_wait_ld(o);
+                        if (live) put(i, o, inv);
+                    }
+                    continue;
+                }
+                // [slot][warp 0..7][d / 4][lane] and [slot][warp][lane]
+                auto slot = [&](int c) { return parts + ((int64_t) c * 2 + (c == I.c0)) * B_PART; };
+                auto slot_o = [&](int c) { return reinterpret_cast<float4 *>(slot(c)) + warp * (D / 4) * 32 + lane; };
+                auto slot_m = [&](int c) { return reinterpret_cast<float2 *>(slot(c) + B_TILE * 128) + warp * 32 + lane; };
+#pragma unroll 1
+                for (int i = 0; i < D / 32; i++) {
+                    uint32_t o[32];
+                    tc_ld32(o_at + 32 * i, o);
+                    tc_wait_ld(o);
+#pragma unroll
+                    for (int e = 0; e < 8; e++)
+                        __stcg(slot_o(blockIdx.x) + (8 * i + e) * 32,
+                               make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]), __uint_as_float(o[4 * e + 2]),
+                                           __uint_as_float(o[4 * e + 3])));
+                }
+                __stcg(slot_m(blockIdx.x), make_float2(m, l));
+                __threadfence();
+                __syncwarp();
+                int last = 0;
+                if (lane == 0) last = atomicAdd(&counters[I.c0 * 8 + warp], 1) == I.others;
+                if (!__shfl_sync(0xFFFFFFFFu, last, 0)) continue;
+                __threadfence();
+                m = k_none;
+                l = 0.0f;
+                for (int c = I.c0; c <= I.c0 + I.others; c++) {
+                    const float2 ml = __ldcg(slot_m(c));
+                    const float mn = fmaxf(m, ml.x);
+                    l = l * ex2(m - mn) + ml.y * ex2(ml.x - mn);
+                    m = mn;
+                }
+                const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+#pragma unroll 1
+                for (int i = 0; i < D / 32; i++) {
+                    float a[32] = {};
+                    for (int c = I.c0; c <= I.c0 + I.others; c++) {
+                        const float f = ex2(__ldcg(slot_m(c)).x - m);
+#pragma unroll
+                        for (int e = 0; e < 8; e++) {
+                            const float4 v = __ldcg(slot_o(c) + (8 * i + e) * 32);
+                            a[4 * e] += v.x * f;
+                            a[4 * e + 1] += v.y * f;
+                            a[4 * e + 2] += v.z * f;
+                            a[4 * e + 3] += v.w * f;
+                        }
+                    }
+                    uint32_t o[32];
+#pragma unroll
+                    for (int e = 0; e < 32; e++) o[e] = __float_as_uint(a[e]);
+                    if (live) put(i, o, inv);
+                }
+                if (lane == 0) counters[I.c0 * 8 + warp] = 0;
+            }
+            tc_wait_st();
+        }
+        __syncwarp();
+    }
+    tc_before();
+    __syncthreads();
+    if (work && warp == 8) {
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;\n" :: "r"(C.tmem));
+        if (lane == 0 && C.stop) atomicAdd(&g_paged_errors[1], 1ull);
+    }
+    // whoever waits for this grid waits for the rows kernel too
+    if (after_rows) asm volatile("griddepcontrol.wait;\n" ::: "memory");
 }
 
 // ============================ sampling =====================================
@@ -697,7 +1357,7 @@ bool paged_ok(const lnsb_paged_kv & a, int * st) {
         (a.k_cache == nullptr || a.v_cache == nullptr || a.page_table == nullptr || a.q_start == nullptr || a.kv_len == nullptr))
         return false;
     *st = LNSB_E_TOO_LARGE;
-    if (a.max_kv > 0x7FFFFFFF || a.n_pages > 0x7FFFFFFF || a.n_tokens > 0x7FFFFFFF || a.n_seqs > 65536 || a.n_head_kv > 65535)
+    if (a.max_kv > 0x7FFFFF00 || a.n_pages > 0x7FFFFFFF || a.n_tokens > 0x7FFFFFFF || a.n_seqs > 65536 || a.n_head_kv > 65535)
         return false;
     *st = 0;
     return true;
@@ -734,34 +1394,96 @@ void launch_append(const lnsb_paged_append_args & a, cudaStream_t s) {
 
 constexpr int k_max_devices = 64;
 
-template <class T, int D>
-int launch_rows(const lnsb_paged_attn_args & a, cudaStream_t s) {
-    auto kern = k_paged_attn_rows<T, D>;
-    static bool attr[k_max_devices] = {};
+constexpr float k_log2e = 1.44269504088896340736f;
+
+// dynamic shared memory of a kernel, once per device
+template <class K>
+int allow_smem(K kern, bool (&done)[k_max_devices], int bytes) {
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return (int) e;
     if (dev < 0 || dev >= k_max_devices) return LNSB_E_NO_DEVICE;
-    if (!attr[dev]) {
-        e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, a_smem<D>());
-        if (e != cudaSuccess) return (int) e;
-        attr[dev] = true;
-    }
+    if (done[dev]) return 0;
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != cudaSuccess) return (int) e;
+    done[dev] = true;
+    return 0;
+}
+
+template <class T, int D>
+int launch_rows(const lnsb_paged_attn_args & a, int64_t rows_most, cudaStream_t s) {
+    auto kern = k_paged_attn_rows<T, D>;
+    static bool attr[k_max_devices] = {};
+    const int st = allow_smem(kern, attr, a_smem<D>());
+    if (st != 0) return st;
     unsigned char * w = static_cast<unsigned char *>(a.work);
     launch_k(kern, dim3(A_CTAS), dim3(128), (size_t) a_smem<D>(), s, view_of(a.kv), static_cast<const T *>(a.q),
              static_cast<T *>(a.dst), static_cast<const T *>(a.kv.k_cache), static_cast<const T *>(a.kv.v_cache), a.q_ld,
-             a.dst_ld, a.n_head / a.kv.n_head_kv, a.scale * 1.44269504088896340736f, a.window, reinterpret_cast<int *>(w),
+             a.dst_ld, a.n_head / a.kv.n_head_kv, a.scale * k_log2e, a.window, rows_most, reinterpret_cast<int *>(w),
              reinterpret_cast<float *>(w + A_COUNT_BYTES));
     return launch_status();
+}
+
+using encode_fn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
+                               const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
+                               CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+encode_fn tensor_map_encoder() {
+    static const encode_fn fn = [] {
+        void * f = nullptr;
+        cudaDriverEntryPointQueryResult r;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &r) != cudaSuccess) f = nullptr;
+        return reinterpret_cast<encode_fn>(f);
+    }();
+    return fn;
+}
+// a cache as (64 of dim, row of the page, kv head, page); false: not to be described
+bool map_cache(CUtensorMap * m, const lnsb_paged_kv & c, void * cache) {
+    const encode_fn encode = tensor_map_encoder();
+    if (encode == nullptr) return false;
+    const cuuint64_t dims[4] = { (cuuint64_t) c.head_dim, (cuuint64_t) c.page_size, (cuuint64_t) c.n_head_kv, (cuuint64_t) c.n_pages };
+    const cuuint64_t strides[3] = { (cuuint64_t) c.row_stride * 2, (cuuint64_t) c.head_stride * 2, (cuuint64_t) c.page_stride * 2 };
+    const cuuint32_t box[4] = { 64, (cuuint32_t) std::min(c.page_size, B_KEYS), 1, 1 }, one[4] = { 1, 1, 1, 1 };
+    return encode(m, c.type == LNSB_TYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, cache, dims,
+                  strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <class T, int D>
+int launch_attn_dim(const lnsb_paged_attn_args & a, cudaStream_t s) {
+    if constexpr (D == 64 || D == 128) {
+        const int G = a.n_head / a.kv.n_head_kv;
+        CUtensorMap km, vm;
+        // scale > 0: the tiles take the maximum before the scale
+        if (a.max_q * G > ROWS && a.kv.n_pages > 0 && a.scale > 0.0f && std::isfinite(a.scale) && map_cache(&km, a.kv, a.kv.k_cache) &&
+            map_cache(&vm, a.kv, a.kv.v_cache)) {
+            auto kern = k_paged_attn_tiles<T, D>;
+            static bool attr[k_max_devices] = {};
+            int st = allow_smem(kern, attr, b_smem<D>());
+            // sequences of few rows go to the rows kernel; one sequence alone does not split
+            const bool both = a.kv.n_seqs > 1;
+            if (st == 0 && both) st = launch_rows<T, D>(a, ROWS, s);
+            if (st != 0) return st;
+            tile_plan L;
+            L.rows_above = both ? ROWS : 0;
+            L.window = a.window;
+            L.G = G;
+            unsigned char * w = static_cast<unsigned char *>(a.work) + A_WORK;
+            launch_k(kern, dim3(B_CTAS), dim3(B_THREADS), (size_t) b_smem<D>(), s, km, vm, view_of(a.kv), L,
+                     static_cast<const T *>(a.q), static_cast<T *>(a.dst), a.q_ld, a.dst_ld, a.scale * k_log2e,
+                     reinterpret_cast<int *>(w), reinterpret_cast<float *>(w + B_COUNT_BYTES), both ? 1 : 0);
+            return launch_status();
+        }
+    }
+    return launch_rows<T, D>(a, INT64_MAX, s);
 }
 template <class T>
 int launch_attn(const lnsb_paged_attn_args & a, cudaStream_t s) {
     switch (a.kv.head_dim) {
-        case 16:  return launch_rows<T, 16>(a, s);
-        case 32:  return launch_rows<T, 32>(a, s);
-        case 64:  return launch_rows<T, 64>(a, s);
-        case 128: return launch_rows<T, 128>(a, s);
-        default:  return launch_rows<T, 256>(a, s);
+        case 16:  return launch_attn_dim<T, 16>(a, s);
+        case 32:  return launch_attn_dim<T, 32>(a, s);
+        case 64:  return launch_attn_dim<T, 64>(a, s);
+        case 128: return launch_attn_dim<T, 128>(a, s);
+        default:  return launch_attn_dim<T, 256>(a, s);
     }
 }
 
@@ -803,7 +1525,7 @@ int lnsb_paged_append(const lnsb_paged_append_args * a, lnsb_stream_t stream) {
     return launch_status();
 }
 
-int64_t lnsb_paged_attn_work_bytes(void) { return A_WORK; }
+int64_t lnsb_paged_attn_work_bytes(void) { return A_WORK + B_WORK; }
 
 int lnsb_paged_attn(const lnsb_paged_attn_args * a, lnsb_stream_t stream) {
     if (a == nullptr) return LNSB_E_INVALID;
@@ -811,6 +1533,7 @@ int lnsb_paged_attn(const lnsb_paged_attn_args * a, lnsb_stream_t stream) {
     if (!paged_ok(a->kv, &st)) return st;
     const lnsb_paged_kv & c = a->kv;
     if (a->n_head <= 0 || a->n_head % c.n_head_kv != 0 || a->max_q < 0 || a->window < 0) return LNSB_E_INVALID;
+    if (c.n_tokens * a->n_head > 0x7FFFFFFF) return LNSB_E_TOO_LARGE;
     const int64_t w = (int64_t) a->n_head * c.head_dim;
     if (a->q_ld < w || a->dst_ld < w || a->q_ld % 8 || a->dst_ld % 8) return LNSB_E_INVALID;
     if ((reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->dst) | reinterpret_cast<uintptr_t>(a->work)) % 16)
