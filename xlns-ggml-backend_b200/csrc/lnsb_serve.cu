@@ -5,6 +5,7 @@
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+#include <cooperative_groups.h>
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -14,6 +15,8 @@
 
 #include "lnsb200.h"
 #include "lnsb_launch.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace lnsb {
 namespace {
@@ -1122,37 +1125,539 @@ k_paged_attn_tiles(const __grid_constant__ CUtensorMap kmap, const __grid_consta
 
 // ============================ sampling =====================================
 //
-// One CTA a row.  The cut of the sorted order -- a key, and how many of the
-// tokens that share it -- is found without sorting: by radix selection over
-// the 32-bit order-preserving keys, by count for top-k, by mass for top-p.
+// One cluster of CTAs a row; every logit is read once and stays in shared memory:
+// warp w of CTA c holds a contiguous part of the row, in order of index
+// (CTA, warp, vector, lane, element).  What bounds it is reading the logits
+// where there are many, and the cluster's barriers where there are few.
+//
+// The cut of the sorted order -- a key, and how many of the tokens that share
+// it stay -- is found without sorting the row.  A histogram over z = (x - max)
+// / t (1024 buckets of 28 / 1024, by count for top-k, by mass for top-p) gives
+// the bucket where the cut falls.  If few tokens lie above and in it, they go
+// to CTA 0, which sorts them and does the rest.  Otherwise the bucket's range
+// of 32-bit order-preserving keys is split again, 1024-fold a step, until one
+// key is left; then the token is found from the warps' masses.
+//
+// Masses are integers of 2^-40 of the largest weight: sums are exact in any
+// order, in histograms too, so the result hangs on no order of atomics.
 
-constexpr int S_THREADS = 512, S_WARPS = S_THREADS / 32;
+constexpr int S_THREADS = 512, S_WARPS = S_THREADS / 32, S_VECS = 16, S_BUCKETS = 1024, S_LIST = 2048;
+constexpr float S_RANGE = 28.0f;               // exp(-28) < 2^-40: weightless
 
-__device__ __forceinline__ uint32_t order_key(float x) {          // x is no NaN, -0 is +0
+using ull = unsigned long long;
+
+__device__ __forceinline__ uint32_t order_key(float x) {          // x is no NaN, and no -0
     const uint32_t b = __float_as_uint(x);
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
-// w in units of 2^-40; w in [0, 1]
-__device__ __forceinline__ unsigned long long mass_of(float w) {
+__device__ __forceinline__ float key_value(uint32_t k) {
+    return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k);
+}
+// w in [0, 1] in units of 2^-40, rounded down
+__device__ __forceinline__ ull mass_of(float w) {
     const uint32_t b = __float_as_uint(w);
     const int e = (int) (b >> 23) - 110;                          // w = mant * 2^(e - 40)
-    const unsigned long long mant = (b & 0x7FFFFFu) | 0x800000u;
-    if (e >= 0) return mant << e;
-    return e > -24 ? mant >> -e : 0ull;
+    const uint32_t mant = (b & 0x7FFFFFu) | 0x800000u;
+    return (ull) (mant >> min(max(-e, 0), 31)) << max(e, 0);
 }
 
-struct sample_par {
-    float    inv_t, top_p, min_p, u;
-    int      k;
-    bool     greedy;
+struct sample_row {
+    float top, inv_t, top_p, min_p, u;
+    int   k;
+    bool  greedy;
+    __device__ void read(int64_t row, int V, const float * temperature, const int32_t * top_k, const float * p, const float * m,
+                         const float * uniform) {
+        const float t = temperature ? temperature[row] : 1.0f;
+        greedy = !(t > 0.0f);
+        inv_t = 1.0f / t;
+        k = top_k ? top_k[row] : 0;
+        if (k <= 0 || k > V) k = V;
+        top_p = p ? p[row] : 1.0f;
+        min_p = m ? fminf(m[row], 1.0f) : 0.0f;                   // the largest always stays
+        if (min_p != min_p) min_p = 0.0f;
+        u = uniform[row];
+    }
+    __device__ float z(float v) const { return v == top ? 0.0f : (v - top) * inv_t; }
+    __device__ float weight(float v) const { return v == top ? 1.0f : expf((v - top) * inv_t); }
+    __device__ ull   mass(float v) const {
+        const float w = weight(v);
+        return w >= 0x1p-40f ? mass_of(w) : 0ull;
+    }
+    __device__ int bucket(float v) const { return min((int) (z(v) * (-S_BUCKETS / S_RANGE)), S_BUCKETS - 1); }
+    // the masses' limit: what lies before a kept token stays at or below it
+    __device__ ull mass_limit(ull whole) const {
+        const double want = ceil((double) top_p * (double) whole);
+        return want >= 1.0 ? (ull) want - 1 : 0ull;
+    }
+    __device__ ull goal(ull total) const {
+        const ull g = (ull) ((double) fminf(fmaxf(u, 0.0f), 1.0f) * (double) total);
+        return g < total ? g : total - 1;
+    }
+    __device__ float prob(float w, ull total) const { return (float) ((double) w / ((double) total * 0x1p-40)); }
+};
+
+struct alignas(16) sample_smem {                // the row's vectors follow it
+    // a mass below 2^41 in three 14-bit parts: 2^16 of them fit 32 bits each
+    uint32_t hist[3][S_BUCKETS];
+    ull      list[S_LIST];
+    ull      sorted[S_LIST];       // CTA 0: the candidates of the cluster
+    ull      scan[S_WARPS + 1];
+    ull      warp_mass[S_WARPS];
+    uint32_t warp_ties[S_WARPS];
+    float    top[S_WARPS];
+    uint32_t key_lo, key_hi;
+    int      best, n, first;
+    // CTA 0's answers
+    ull      above, inside;
+    int      bucket;
+    ull      goal, ties, total;
+    int      cta, warp;
+};
+
+// inclusive scan over the block, total in *total
+__device__ __forceinline__ ull block_scan(ull v, ull * sums, ull * total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const ull o = __shfl_up_sync(0xFFFFFFFFu, v, d);
+        if (lane >= d) v += o;
+    }
+    __syncthreads();
+    if (lane == 31) sums[warp] = v;
+    __syncthreads();
+    ull t = 0;
+    for (int w = 0; w < S_WARPS; w++) {
+        if (w < warp) v += sums[w];
+        t += sums[w];
+    }
+    *total = t;
+    return v;
+}
+// falling order, n a power of two
+__device__ __forceinline__ void block_sort(ull * a, int n) {
+    for (int size = 2; size <= n; size <<= 1)
+        for (int d = size >> 1; d; d >>= 1) {
+            __syncthreads();
+            for (int i = threadIdx.x; i < n / 2; i += S_THREADS) {
+                const int x = 2 * i - (i & (d - 1)), y = x + d;
+                const bool down = (x & size) == 0;
+                const ull u = a[x], v = a[y];
+                if ((u < v) == down) {
+                    a[x] = v;
+                    a[y] = u;
+                }
+            }
+        }
+    __syncthreads();
+}
+
+static_assert(sizeof(sample_smem) % 16 == 0, "vectors behind it");
+
+template <class T> struct vec16;
+template <> struct vec16<float> {
+    static constexpr int N = 4;
+    static __device__ __forceinline__ float at(const uint4 & v, int e) {
+        return __uint_as_float(e == 0 ? v.x : e == 1 ? v.y : e == 2 ? v.z : v.w);
+    }
+};
+template <class T> struct vec16 {
+    static constexpr int N = 8;
+    static __device__ __forceinline__ float at(const uint4 & v, int e) {
+        const uint32_t w = e < 2 ? v.x : e < 4 ? v.y : e < 6 ? v.z : v.w;
+        const uint16_t h = (uint16_t) (e & 1 ? w >> 16 : w & 0xFFFF);
+        return num<T>::to(*reinterpret_cast<const T *>(&h));
+    }
 };
 
 template <class T>
-__global__ void __launch_bounds__(S_THREADS)
-k_sample(const T * __restrict__ logits, int64_t ld, int V, const float * __restrict__ temperature,
+__global__ void __launch_bounds__(S_THREADS, 2)
+k_sample(const T * __restrict__ logits, int64_t ld, int V, int vecs, const float * __restrict__ temperature,
          const int32_t * __restrict__ top_k, const float * __restrict__ top_p, const float * __restrict__ min_p,
          const float * __restrict__ u, int32_t * __restrict__ token, float * __restrict__ prob) {
-    using ull = unsigned long long;
+    constexpr int E = vec16<T>::N;
+    extern __shared__ __align__(16) unsigned char sample_sm[];
+    sample_smem & M = *reinterpret_cast<sample_smem *>(sample_sm);
+    cg::cluster_group cluster = cg::this_cluster();
+    const int C = (int) cluster.num_blocks(), cta = (int) cluster.block_rank();
+    const int64_t row = blockIdx.x / C;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    sample_smem & M0 = *cluster.map_shared_rank(&M, 0);
+    pdl_entry();
+
+    // ---- the logits: NaN and what lies beyond the row are -inf, -0 is 0
+    const T * x = logits + row * ld;
+    const int lead = (int) (reinterpret_cast<uintptr_t>(x) % 16 / sizeof(T));    // vectors start at 16-byte boundaries
+    const int base = (cta * S_WARPS + warp) * vecs * 32 * E + lane * E - lead;   // index of element e of vector i: + i * 32 * E + e
+    uint4 * const mine = reinterpret_cast<uint4 *>(sample_sm + sizeof(sample_smem)) + tid;   // vector i at i * S_THREADS
+    for (int i = 0; i < vecs; i++) {
+        const int at = base + i * 32 * E;
+        if (at >= 0 && at + E <= V) {
+            cp16(smem_addr(mine + i * S_THREADS), x + at, true);
+        } else {
+            alignas(16) T t[E];
+#pragma unroll
+            for (int e = 0; e < E; e++) t[e] = at + e >= 0 && at + e < V ? x[at + e] : num<T>::from(-INFINITY);
+            mine[i * S_THREADS] = *reinterpret_cast<const uint4 *>(t);
+        }
+    }
+    cp_commit();
+    auto value = [&](const uint4 & r, int e) {
+        const float v = vec16<T>::at(r, e);
+        return v == v ? v + 0.0f : -INFINITY;
+    };
+    sample_row R;
+    R.read(row, V, temperature, top_k, top_p, min_p, u);
+    // ---- the maximum
+    float top = -INFINITY;
+    cp_wait<0>();                              // a thread reads only what it has fetched
+    for (int i = 0; i < vecs; i++) {
+        const uint4 r = mine[i * S_THREADS];
+#pragma unroll
+        for (int e = 0; e < E; e++) top = fmaxf(top, vec16<T>::at(r, e));
+    }
+#pragma unroll
+    for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
+    if (lane == 0) M.top[warp] = top;
+    if (tid == 0) {
+        M.n = 0;
+        M.first = 0x7FFFFFFF;
+    }
+    cluster.sync();
+    for (int i = lane; i < C * S_WARPS; i += 32) top = fmaxf(top, cluster.map_shared_rank(&M, i / S_WARPS)->top[i % S_WARPS]);
+#pragma unroll
+    for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
+    R.top = top + 0.0f;
+    if (R.top == -INFINITY || R.greedy) {
+        if (R.top != -INFINITY) {
+            int first = 0x7FFFFFFF;
+            for (int i = vecs - 1; i >= 0; i--) {
+                const uint4 r = mine[i * S_THREADS];
+#pragma unroll
+                for (int e = E - 1; e >= 0; e--)
+                    if (value(r, e) == R.top) first = base + i * 32 * E + e;
+            }
+            first = __reduce_min_sync(0xFFFFFFFFu, first);
+            if (lane == 0 && first != 0x7FFFFFFF) atomicMin(&M0.first, first);
+        }
+        cluster.sync();
+        if (cta == 0 && tid == 0) {
+            token[row] = R.top == -INFINITY ? -1 : M.first;
+            if (prob) prob[row] = R.top == -INFINITY ? 0.0f : 1.0f;
+        }
+        return;
+    }
+
+    uint32_t cut = 0;                          // kept: key > cut, and the first `ties` of key == cut
+    ull ties = (ull) V;
+    for (int by_mass = 0; by_mass < 2; by_mass++) {
+        if (by_mass ? !(R.top_p < 1.0f) : R.k >= V) continue;
+        ull limit = (ull) (R.k - 1), above = 0, whole = 0;
+        uint32_t key_lo = 0, key_hi = 0;
+        int shift = 32;                        // 32: the buckets of z
+        while (true) {
+            __syncthreads();
+            for (int i = tid; i < (by_mass ? 3 : 1) * S_BUCKETS; i += S_THREADS) (&M.hist[0][0])[i] = 0;
+            if (tid == 0) {
+                M.best = 0;
+                M.key_lo = 0xFFFFFFFFu;
+                M.key_hi = 0;
+            }
+            __syncthreads();
+            for (int i = 0; i < vecs; i++) {
+                const uint4 r = mine[i * S_THREADS];
+#pragma unroll
+                for (int e = 0; e < E; e++) {
+                    const float v = value(r, e);
+                    const uint32_t key = order_key(v);
+                    if (key < cut || (shift < 32 && (key < key_lo || key > key_hi)) || v == -INFINITY) continue;
+                    const int b = shift == 32 ? R.bucket(v) : (int) ((key_hi - key) >> shift);
+                    if (!by_mass) {
+                        atomicAdd(&M.hist[0][b], 1u);
+                    } else {
+                        const ull m = R.mass(v);
+                        if (m) {
+                            atomicAdd(&M.hist[0][b], (uint32_t) m & 0x3FFFu);
+                            atomicAdd(&M.hist[1][b], (uint32_t) (m >> 14) & 0x3FFFu);
+                            atomicAdd(&M.hist[2][b], (uint32_t) (m >> 28));
+                        }
+                    }
+                }
+            }
+            cluster.sync();
+            if (cta == 0) {
+                ull v[2] = { 0, 0 }, total;
+#pragma unroll
+                for (int j = 0; j < 2; j++)
+                    for (int c = 0; c < C; c++) {
+                        const sample_smem & Mc = *cluster.map_shared_rank(&M, c);
+                        v[j] += Mc.hist[0][2 * tid + j];
+                        if (by_mass) v[j] += ((ull) Mc.hist[1][2 * tid + j] << 14) + ((ull) Mc.hist[2][2 * tid + j] << 28);
+                    }
+                const ull upto = block_scan(v[0] + v[1], M.scan, &total);
+                if (by_mass && shift == 32) {
+                    // what top-k left: of the tokens at its cut only some count
+                    whole = total;
+                    if (R.k < V) whole -= (M.inside - ties) * R.mass(key_value(cut));
+                    limit = R.mass_limit(whole);
+                }
+                const ull x0 = above + upto - v[0] - v[1], x1 = x0 + v[0];
+                if (v[0] && x0 <= limit) atomicMax(&M.best, 2 * tid);
+                if (v[1] && x1 <= limit) atomicMax(&M.best, 2 * tid + 1);
+                __syncthreads();
+                if (M.best >> 1 == tid) {
+                    M.bucket = M.best;
+                    M.above = M.best & 1 ? x1 : x0;
+                    M.inside = M.best & 1 ? v[1] : v[0];
+                    M.total = whole;
+                }
+            }
+            cluster.sync();
+            const int b = M0.bucket;
+            above = M0.above;
+            const ull inside = M0.inside;
+            whole = M0.total;
+            if (by_mass) limit = R.mass_limit(whole);
+            if (shift == 0) {
+                key_hi -= (uint32_t) b;
+                ull n = limit - above + 1;
+                if (by_mass) n = (limit - above) / R.mass(key_value(key_hi)) + 1;
+                if (key_hi > cut) {
+                    cut = key_hi;
+                    ties = n;
+                } else {
+                    ties = min(ties, n);
+                }
+                cluster.sync();                // CTA 0's answers are read
+                if (cta == 0 && tid == 0) M.inside = inside;      // tokens at top-k's cut
+                break;
+            }
+            if (shift < 32) {
+                key_hi -= (uint32_t) b << shift;
+                key_lo = max(key_lo, key_hi - ((1u << shift) - 1));
+            } else {
+                // few tokens down to the bucket, and none cut away before: they go to CTA 0
+                const bool some = cut == 0 && (by_mass || above + inside <= S_LIST);
+                uint32_t lo = 0xFFFFFFFFu, hi = 0;
+                for (int i = 0; i < vecs; i++) {
+                    const uint4 r = mine[i * S_THREADS];
+#pragma unroll
+                    for (int e = 0; e < E; e++) {
+                        const float v = value(r, e);
+                        const uint32_t key = order_key(v);
+                        if (key < cut || v == -INFINITY) continue;
+                        const int vb = R.bucket(v);
+                        if (vb > b) continue;
+                        if (vb == b) {
+                            lo = min(lo, key);
+                            hi = max(hi, key);
+                        }
+                        if (some && *(volatile int *) &M.n <= S_LIST) {
+                            const int at = atomicAdd(&M.n, 1);
+                            if (at < S_LIST) M.list[at] = (ull) key << 32 | (uint32_t) ~(base + i * 32 * E + e);
+                        }
+                    }
+                }
+                lo = __reduce_min_sync(0xFFFFFFFFu, lo);
+                hi = __reduce_max_sync(0xFFFFFFFFu, hi);
+                if (lane == 0) {
+                    atomicMin(&M.key_lo, lo);
+                    atomicMax(&M.key_hi, hi);
+                }
+                cluster.sync();
+                int n = 0;
+                key_lo = 0xFFFFFFFFu;
+                for (int c = 0; c < C; c++) {
+                    const sample_smem & Mc = *cluster.map_shared_rank(&M, c);
+                    n += Mc.n;
+                    key_lo = min(key_lo, Mc.key_lo);
+                    key_hi = max(key_hi, Mc.key_hi);
+                }
+                if (some && n <= S_LIST) {
+                    // ---- the list: sorted, cut, sorted again by index
+                    if (cta != 0) {
+                        cluster.sync();
+                        return;
+                    }
+                    int at = 0, size = 2;
+                    while (size < n) size <<= 1;
+                    for (int c = 0; c < C; c++) {
+                        const sample_smem & Mc = *cluster.map_shared_rank(&M, c);
+                        for (int i = tid; i < Mc.n; i += S_THREADS) M.sorted[at + i] = Mc.list[i];
+                        at += Mc.n;
+                    }
+                    for (int i = n + tid; i < size; i += S_THREADS) M.sorted[i] = 0;
+                    cluster.sync();            // the others may go
+                    block_sort(M.sorted, size);
+                    // four consecutive tokens a thread
+                    float w[4];
+                    ull m[4], sum = 0, total;
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const int i = 4 * tid + j;
+                        w[j] = i < n ? R.weight(key_value((uint32_t) (M.sorted[i] >> 32))) : 0.0f;
+                        m[j] = i < n && i < R.k && w[j] >= 0x1p-40f ? mass_of(w[j]) : 0ull;
+                        sum += m[j];
+                    }
+                    ull run = block_scan(sum, M.scan, &total) - sum;
+                    if (R.k < V) whole = total;
+                    limit = R.top_p < 1.0f ? R.mass_limit(whole) : ~0ull;
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const int i = 4 * tid + j;
+                        const bool keep = i < n && i < R.k && run <= limit && w[j] >= R.min_p;
+                        run += m[j];
+                        if (i < size) M.list[i] = keep ? (ull) (uint32_t) M.sorted[i] << 32 | (uint32_t) (M.sorted[i] >> 32) : 0ull;
+                    }
+                    block_sort(M.list, size);  // falling ~index
+                    sum = 0;
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const int i = 4 * tid + j;
+                        const ull a = i < size ? M.list[i] : 0ull;
+                        w[j] = a ? R.weight(key_value((uint32_t) a)) : 0.0f;
+                        m[j] = a && w[j] >= 0x1p-40f ? mass_of(w[j]) : 0ull;
+                        sum += m[j];
+                    }
+                    run = block_scan(sum, M.scan, &total) - sum;
+                    const ull goal = R.goal(total);
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        if (m[j] && run <= goal && goal < run + m[j]) {
+                            token[row] = (int32_t) ~(uint32_t) (M.list[4 * tid + j] >> 32);
+                            if (prob) prob[row] = R.prob(w[j], total);
+                        }
+                        run += m[j];
+                    }
+                    return;
+                }
+                if (tid == 0) M.n = S_LIST + 1;                    // no second try
+            }
+            const uint32_t span = key_hi - key_lo;
+            shift = span < S_BUCKETS ? 0 : 22 - __clz(span);
+            cluster.sync();                    // everyone has read
+        }
+    }
+
+    // ---- the warps' masses, in order of index
+    {
+        ull m = 0;
+        uint32_t eq = 0;
+        for (int i = 0; i < vecs; i++) {
+            const uint4 r = mine[i * S_THREADS];
+#pragma unroll
+            for (int e = 0; e < E; e++) {
+                const float v = value(r, e);
+                const uint32_t key = order_key(v);
+                eq += key == cut;
+                if (key > cut) {
+                    const float w = R.weight(v);
+                    if (w >= R.min_p && w >= 0x1p-40f) m += mass_of(w);
+                }
+            }
+        }
+#pragma unroll
+        for (int d = 16; d; d >>= 1) m += __shfl_xor_sync(0xFFFFFFFFu, m, d);
+        eq = __reduce_add_sync(0xFFFFFFFFu, eq);
+        if (lane == 0) {
+            M.warp_mass[warp] = m;
+            M.warp_ties[warp] = eq;
+        }
+    }
+    const float w_cut = cut ? R.weight(key_value(cut)) : 0.0f;
+    const ull m_cut = cut && w_cut >= R.min_p && w_cut >= 0x1p-40f ? mass_of(w_cut) : 0ull;
+    cluster.sync();
+    if (cta == 0) {
+        ull eq = 0, m = 0, total;
+        if (tid < C * S_WARPS) {
+            const sample_smem & Mc = *cluster.map_shared_rank(&M, tid / S_WARPS);
+            m = Mc.warp_mass[tid % S_WARPS];
+            eq = Mc.warp_ties[tid % S_WARPS];
+        }
+        const ull eq_before = block_scan(eq, M.scan, &total) - eq;
+        const ull left = eq_before < ties ? ties - eq_before : 0;
+        const ull mine = m + min(left, eq) * m_cut;
+        const ull before = block_scan(mine, M.scan, &total) - mine;
+        const ull goal = R.goal(total);
+        if (goal >= before && goal < before + mine) {
+            M.cta = tid / S_WARPS;
+            M.warp = tid % S_WARPS;
+            M.goal = goal - before;
+            M.ties = left;
+            M.total = total;
+        }
+    }
+    cluster.sync();
+    if (M0.cta == cta && M0.warp == warp) {
+        // 32 lanes' elements of a vector at a time
+        ull goal = M0.goal, left = M0.ties;
+        const ull total = M0.total;
+        bool found = false;
+        for (int i = 0; i < vecs && !found; i++) {
+            const uint4 r = mine[i * S_THREADS];
+            uint32_t eq = 0;
+#pragma unroll
+            for (int e = 0; e < E; e++) eq += order_key(value(r, e)) == cut;
+            uint32_t eq_upto = eq;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const uint32_t o = __shfl_up_sync(0xFFFFFFFFu, eq_upto, d);
+                if (lane >= d) eq_upto += o;
+            }
+            const ull lane_left = left > eq_upto - eq ? left - (eq_upto - eq) : 0;
+            auto part = [&](int e, ull & room) {
+                const float v = value(r, e);
+                const uint32_t key = order_key(v);
+                if (key > cut) {
+                    const float w = R.weight(v);
+                    return w >= R.min_p && w >= 0x1p-40f ? mass_of(w) : 0ull;
+                }
+                if (key == cut && room) {
+                    room--;
+                    return m_cut;
+                }
+                return 0ull;
+            };
+            ull sum = 0, room = lane_left;
+#pragma unroll
+            for (int e = 0; e < E; e++) sum += part(e, room);
+            ull upto = sum;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const ull o = __shfl_up_sync(0xFFFFFFFFu, upto, d);
+                if (lane >= d) upto += o;
+            }
+            const ull all = __shfl_sync(0xFFFFFFFFu, upto, 31);
+            if (goal < all) {
+                found = true;
+                ull run = upto - sum;
+                room = lane_left;
+                if (goal >= run && goal < upto) {
+#pragma unroll
+                    for (int e = 0; e < E; e++) {
+                        const ull m = part(e, room);
+                        if (m && goal >= run && goal < run + m) {
+                            token[row] = base + i * 32 * E + e;
+                            if (prob) prob[row] = R.prob(R.weight(value(r, e)), total);
+                        }
+                        run += m;
+                    }
+                }
+            }
+            goal -= min(goal, all);
+            const uint32_t eqs = __shfl_sync(0xFFFFFFFFu, eq_upto, 31);
+            left = left > eqs ? left - eqs : 0;
+        }
+    }
+    cluster.sync();                            // CTA 0's answers are read
+}
+
+// Rows that the shared memory of a cluster does not hold: one CTA a row reads the
+// logits again for each step, radix selection eight bits of the key at a time.
+template <class T>
+__global__ void __launch_bounds__(S_THREADS)
+k_sample_long(const T * __restrict__ logits, int64_t ld, int V, const float * __restrict__ temperature,
+         const int32_t * __restrict__ top_k, const float * __restrict__ top_p, const float * __restrict__ min_p,
+         const float * __restrict__ u, int32_t * __restrict__ token, float * __restrict__ prob) {
     __shared__ ull s_mass[256];
     __shared__ float s_f[S_WARPS];
     __shared__ ull s_w[S_WARPS];
@@ -1163,16 +1668,8 @@ k_sample(const T * __restrict__ logits, int64_t ld, int V, const float * __restr
     const int64_t row = blockIdx.x;
     const T * x = logits + row * ld;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    sample_par p;
-    const float t = temperature ? temperature[row] : 1.0f;
-    p.greedy = !(t > 0.0f);
-    p.inv_t = 1.0f / t;
-    p.k = top_k ? top_k[row] : 0;
-    if (p.k <= 0 || p.k > V) p.k = V;
-    p.top_p = top_p ? top_p[row] : 1.0f;
-    p.min_p = min_p ? fminf(min_p[row], 1.0f) : 0.0f;             // the largest always stays
-    if (p.min_p != p.min_p) p.min_p = 0.0f;
-    p.u = u[row];
+    sample_row p;
+    p.read(row, V, temperature, top_k, top_p, min_p, u);
     auto value = [&](int i) {
         const float v = num<T>::to(x[i]);
         return v != v ? -INFINITY : v + 0.0f;
@@ -1192,7 +1689,8 @@ k_sample(const T * __restrict__ logits, int64_t ld, int V, const float * __restr
         }
         return;
     }
-    auto weight = [&](float v) { return v == top ? 1.0f : expf((v - top) * p.inv_t); };
+    p.top = top;
+    auto weight = [&](float v) { return p.weight(v); };
     uint32_t cut = 0;                         // kept: key > cut, and the first `ties` of key == cut
     ull ties = (ull) V;
     if (p.greedy) {
@@ -1207,7 +1705,7 @@ k_sample(const T * __restrict__ logits, int64_t ld, int V, const float * __restr
                 ull m = 0;
                 for (int i = tid; i < V; i += S_THREADS) {
                     const float v = value(i);
-                    if (order_key(v) > cut) m += mass_of(weight(v));
+                    if (order_key(v) > cut) m += p.mass(v);
                 }
 #pragma unroll
                 for (int d = 16; d; d >>= 1) m += __shfl_xor_sync(0xFFFFFFFFu, m, d);
@@ -1217,16 +1715,15 @@ k_sample(const T * __restrict__ logits, int64_t ld, int V, const float * __restr
                 whole = 0;
                 for (int w = 0; w < S_WARPS; w++) whole += s_w[w];
                 if (p.k < V) {
-                    const float vc = __uint_as_float(cut & 0x80000000u ? cut & 0x7FFFFFFFu : ~cut);
-                    whole += ties * mass_of(weight(vc));
+                    const float vc = key_value(cut);
+                    whole += ties * p.mass(vc);
                 }
             }
             uint32_t prefix = 0, mask = 0;
             // what lies above must be <= limit (count: k - 1; mass: below top_p * whole)
             ull limit = (ull) (p.k - 1);
             if (by_mass) {
-                const double want = (double) p.top_p * (double) whole;
-                limit = want > 0 ? (ull) ceil(want) - (ceil(want) > 0 ? 1 : 0) : 0;
+                limit = p.mass_limit(whole);
             }
             ull above = 0;
             for (int shift = 24; shift >= 0; shift -= 8) {
@@ -1237,7 +1734,7 @@ k_sample(const T * __restrict__ logits, int64_t ld, int V, const float * __restr
                     const float v = value(i);
                     const uint32_t k = order_key(v);
                     if ((k & mask) == prefix && k >= cut) {
-                        const ull a = by_mass ? mass_of(weight(v)) : 1ull;
+                        const ull a = by_mass ? p.mass(v) : 1ull;
                         if (a) atomicAdd(&s_mass[(k >> shift) & 255], a);
                     }
                 }
@@ -1265,8 +1762,8 @@ k_sample(const T * __restrict__ logits, int64_t ld, int V, const float * __restr
             }
             ull n = limit - above + 1;                            // by count
             if (by_mass) {
-                const float vc = __uint_as_float(prefix & 0x80000000u ? prefix & 0x7FFFFFFFu : ~prefix);
-                const ull w = mass_of(weight(vc));
+                const float vc = key_value(prefix);
+                const ull w = p.mass(vc);
                 n = (limit - above) / w + 1;
             }
             if (prefix > cut) {
@@ -1299,7 +1796,7 @@ k_sample(const T * __restrict__ logits, int64_t ld, int V, const float * __restr
         const bool keep = in && (k > cut || (k == cut && rank + __popc(tie & ((1u << lane) - 1)) < ties));
         rank += __popc(tie);
         w = keep ? weight(v) : 0.0f;
-        return keep && (p.greedy || w >= p.min_p) ? (p.greedy ? 1ull : mass_of(w)) : 0ull;
+        return keep && (p.greedy || w >= p.min_p) ? (p.greedy ? 1ull : w >= 0x1p-40f ? mass_of(w) : 0ull) : 0ull;
     };
     ull sum = 0, rank = before;
     for (int i = i0; i < i1; i += 32) {
@@ -1316,9 +1813,7 @@ k_sample(const T * __restrict__ logits, int64_t ld, int V, const float * __restr
         if (w < warp) base += s_w[w];
         total += s_w[w];
     }
-    const float uu = fminf(fmaxf(p.u, 0.0f), 1.0f);
-    ull goal = (ull) ((double) uu * (double) total);
-    if (goal >= total) goal = total - 1;
+    const ull goal = p.goal(total);
     if (goal < base || goal >= base + sum) return;
     // the warp that holds the token
     rank = before;
@@ -1333,7 +1828,7 @@ k_sample(const T * __restrict__ logits, int64_t ld, int V, const float * __restr
         const bool hit = a && goal >= base + run - a && goal < base + run;
         if (hit) {
             token[row] = i + lane;
-            if (prob) prob[row] = p.greedy ? 1.0f : (float) ((double) w / ((double) total * 0x1p-40));
+            if (prob) prob[row] = p.greedy ? 1.0f : p.prob(w, total);
         }
         if (__any_sync(0xFFFFFFFFu, hit)) return;
         base += __shfl_sync(0xFFFFFFFFu, run, 31);
@@ -1394,8 +1889,6 @@ void launch_append(const lnsb_paged_append_args & a, cudaStream_t s) {
 
 constexpr int k_max_devices = 64;
 
-constexpr float k_log2e = 1.44269504088896340736f;
-
 // dynamic shared memory of a kernel, once per device
 template <class K>
 int allow_smem(K kern, bool (&done)[k_max_devices], int bytes) {
@@ -1409,6 +1902,44 @@ int allow_smem(K kern, bool (&done)[k_max_devices], int bytes) {
     done[dev] = true;
     return 0;
 }
+
+template <class T>
+int launch_sample(const lnsb_sample_args & a, cudaStream_t s) {
+    const T * x = static_cast<const T *>(a.logits);
+    const int V = (int) a.n_vocab, E = vec16<T>::N, need = V + E - 1;      // a row may start inside a vector
+    const int line = S_THREADS * E;                                       // one vector of each thread
+    int C = 1;
+    while (C < 8 && need > C * line * S_VECS / 2) C *= 2;                 // two CTAs to an SM where the row allows it
+    if (need > C * line * S_VECS) {
+        launch_k(k_sample_long<T>, dim3((unsigned) a.n_rows), dim3(S_THREADS), 0, s, x, a.ld, V, a.temperature, a.top_k, a.top_p,
+                 a.min_p, a.u, a.token, a.prob);
+        return launch_status();
+    }
+    // few rows: more CTAs to each, while they have an SM of their own and a vector to read
+    while (C < 8 && a.n_rows * C * 2 <= k_sms && need > C * line) C *= 2;
+    auto kern = k_sample<T>;
+    static bool attr[k_max_devices] = {};
+    const int st = allow_smem(kern, attr, (int) sizeof(sample_smem) + S_VECS * S_THREADS * 16);
+    if (st != 0) return st;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned) (a.n_rows * C));
+    cfg.blockDim = dim3(S_THREADS);
+    const int vecs = (need + C * line - 1) / (C * line);
+    cfg.dynamicSmemBytes = sizeof(sample_smem) + (size_t) vecs * S_THREADS * 16;
+    cfg.stream = s;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = LNSB_PDL;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim = { (unsigned) C, 1, 1 };
+    cfg.attrs = at;
+    cfg.numAttrs = 2;
+    (void) cudaLaunchKernelEx(&cfg, kern, x, a.ld, V, vecs, a.temperature, a.top_k, a.top_p, a.min_p, a.u, a.token,
+                              a.prob);   // an error stays in cudaGetLastError
+    return launch_status();
+}
+
+constexpr float k_log2e = 1.44269504088896340736f;
 
 template <class T, int D>
 int launch_rows(const lnsb_paged_attn_args & a, int64_t rows_most, cudaStream_t s) {
@@ -1561,20 +2092,10 @@ int lnsb_sample(const lnsb_sample_args * a, lnsb_stream_t stream) {
     if (a->type != LNSB_TYPE_F32 && a->type != LNSB_TYPE_F16 && a->type != LNSB_TYPE_BF16) return LNSB_E_INVALID;
     if (a->n_rows == 0) return 0;
     if (a->logits == nullptr || a->u == nullptr || a->token == nullptr) return LNSB_E_INVALID;
-    if (a->n_vocab > (1 << 20) || a->n_rows > 0x7FFFFFFF) return LNSB_E_TOO_LARGE;
+    if (a->n_vocab > (1 << 20) || a->n_rows > (1 << 27)) return LNSB_E_TOO_LARGE;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const dim3 grid((unsigned) a->n_rows);
-    const int V = (int) a->n_vocab;
-    if (a->type == LNSB_TYPE_F32)
-        launch_k(k_sample<float>, grid, dim3(S_THREADS), 0, s, static_cast<const float *>(a->logits), a->ld, V, a->temperature,
-                 a->top_k, a->top_p, a->min_p, a->u, a->token, a->prob);
-    else if (a->type == LNSB_TYPE_F16)
-        launch_k(k_sample<__half>, grid, dim3(S_THREADS), 0, s, static_cast<const __half *>(a->logits), a->ld, V,
-                 a->temperature, a->top_k, a->top_p, a->min_p, a->u, a->token, a->prob);
-    else
-        launch_k(k_sample<__nv_bfloat16>, grid, dim3(S_THREADS), 0, s, static_cast<const __nv_bfloat16 *>(a->logits), a->ld, V,
-                 a->temperature, a->top_k, a->top_p, a->min_p, a->u, a->token, a->prob);
-    return launch_status();
+    if (a->type == LNSB_TYPE_F32) return launch_sample<float>(*a, s);
+    return a->type == LNSB_TYPE_F16 ? launch_sample<__half>(*a, s) : launch_sample<__nv_bfloat16>(*a, s);
 }
 
 }  // extern "C"
