@@ -80,7 +80,8 @@ __device__ __forceinline__ int64_t page_of(const paged & P, int s, int64_t row) 
 
 // ============================ append =======================================
 
-// One thread per rotated pair, copied element or v element.
+// Any alignment and any n_dims: one thread a rotated pair, copied element or v
+// element.
 template <class TI, class TC>
 __global__ void k_paged_append(paged P, const TI * __restrict__ k, const TI * __restrict__ v, const TI * __restrict__ q,
                                TC * __restrict__ q_out, const float * __restrict__ cos_sin, int64_t k_ld, int64_t v_ld,
@@ -130,6 +131,121 @@ __global__ void k_paged_append(paged P, const TI * __restrict__ k, const TI * __
         const float x0 = num<TI>::to(src[d0]), x1 = num<TI>::to(src[d1]);
         dst[d0] = num<TC>::from(x0 * c - x1 * s);
         dst[d1] = num<TC>::from(x0 * s + x1 * c);
+    }
+}
+
+// 8 elements at a 16-byte boundary
+template <class T>
+__device__ __forceinline__ void load8(const T * p, float (&x)[8]) {
+    if constexpr (sizeof(T) == 4) {
+        const float4 a = __ldg(reinterpret_cast<const float4 *>(p)), b = __ldg(reinterpret_cast<const float4 *>(p) + 1);
+        x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+    } else {
+        const uint4 v = __ldg(reinterpret_cast<const uint4 *>(p));
+        const uint32_t w[4] = { v.x, v.y, v.z, v.w };
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const uint16_t h = (uint16_t) (w[i / 2] >> (16 * (i & 1)));
+            x[i] = num<T>::to(*reinterpret_cast<const T *>(&h));
+        }
+    }
+}
+template <class T>
+__device__ __forceinline__ void store8(T * p, const float (&x)[8]) {
+    *reinterpret_cast<uint4 *>(p) = make_uint4(num<T>::pack(x[0], x[1]), num<T>::pack(x[2], x[3]), num<T>::pack(x[4], x[5]),
+                                               num<T>::pack(x[6], x[7]));
+}
+
+// Where rows lie at 16-byte boundaries and n_dims is a multiple of 16: a thread
+// takes 8 elements (NEOX: 8 of each half of the pairs), a block `tokens`
+// tokens.  Its inputs are on their way while the first threads look up where
+// the block's tokens go.
+template <class TI, class TC, bool NEOX>
+__global__ void __launch_bounds__(256)
+k_paged_append_vec(paged P, const TI * __restrict__ k, const TI * __restrict__ v, const TI * __restrict__ q,
+                   TC * __restrict__ q_out, const float * __restrict__ cos_sin, int64_t k_ld, int64_t v_ld, int64_t q_ld,
+                   int64_t q_out_ld, int n_head, int D, int n_dims, int tokens, TC * __restrict__ kc, TC * __restrict__ vc) {
+    __shared__ int64_t s_at[256];                       // the token's place in a head of the caches, -1: none
+    __shared__ int     s_row[256];                      // its row, negative: none
+    pdl_entry();
+    const int tid = threadIdx.x, half = n_dims / 2;
+    const int turned = NEOX ? half / 8 : n_dims / 8;    // units of a q or k head: turned ones, then copied ones
+    const int per = turned + (D - n_dims) / 8, qk = (n_head + P.n_head_kv) * per, units = qk + P.n_head_kv * (D / 8);
+    const int64_t t0 = (int64_t) blockIdx.x * tokens;
+    bool planned = false;
+    for (int i = tid; i - tid < tokens * units; i += 256) {
+        const bool in = i < tokens * units;
+        const int tb = tokens == 1 ? 0 : i / units, r = i - tb * units;
+        const int64_t t = t0 + tb;
+        const bool live = in && t < P.n_tokens, is_v = r >= qk;
+        const int h = is_v ? (r - qk) / (D / 8) : r / per, j = is_v ? (r - qk) % (D / 8) : r % per;
+        const bool is_q = !is_v && h < n_head, turn = !is_v && j < turned;
+        const int kvh = is_v ? h : h - n_head;
+        // NEOX: dims 8 j and half + 8 j of the pairs, copied units after both halves
+        const int d = turn || is_v ? 8 * j : n_dims + 8 * (j - turned);
+        float x[8], y[8];
+        if (live) {
+            const TI * src = (is_q ? q + t * q_ld + (int64_t) h * D : is_v ? v + t * v_ld + (int64_t) kvh * D
+                                                                           : k + t * k_ld + (int64_t) kvh * D) + d;
+            load8(src, x);
+            if (NEOX && turn) load8(src + half, y);
+        }
+        if (!planned) {
+            planned = true;
+            if (tid < tokens) {
+                const int64_t tt = t0 + tid;
+                int row = -1;
+                int64_t at = -1;
+                if (tt < P.n_tokens) {
+                    int lo = 0, hi = P.n_seqs;          // the last sequence that starts at or before the token
+                    while (hi - lo > 1) {
+                        const int mid = (lo + hi) / 2;
+                        if (P.q_start[mid] <= tt) lo = mid; else hi = mid;
+                    }
+                    const seq_span S = span_of(P, lo);
+                    const int64_t rw = S.kv - S.n + (tt - S.first);
+                    if (tt >= S.first && tt < S.first + S.n && rw >= 0) {
+                        row = (int) rw;
+                        const int64_t id = page_of(P, lo, rw);
+                        if (id >= 0) at = id * P.page_stride + (rw & ((1 << P.page_shift) - 1)) * P.row_stride;
+                    }
+                }
+                s_row[tid] = row;
+                s_at[tid] = at;
+            }
+            __syncthreads();
+        }
+        if (!live) continue;
+        const int row = s_row[tb];
+        const int64_t at = s_at[tb];
+        if (row < 0 || (!is_q && at < 0)) continue;
+        TC * dst = (is_q ? q_out + t * q_out_ld + (int64_t) h * D : (is_v ? vc : kc) + at + kvh * P.head_stride) + d;
+        if (turn) {
+            float c[8], s[8];
+            const float4 * cs = reinterpret_cast<const float4 *>(cos_sin + ((int64_t) row * half + (NEOX ? 8 : 4) * j) * 2);
+#pragma unroll
+            for (int e = 0; e < (NEOX ? 4 : 2); e++) {
+                const float4 w = __ldg(cs + e);
+                c[2 * e] = w.x, s[2 * e] = w.y, c[2 * e + 1] = w.z, s[2 * e + 1] = w.w;
+            }
+            if (NEOX) {
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const float a = x[e], b = y[e];
+                    x[e] = a * c[e] - b * s[e];
+                    y[e] = a * s[e] + b * c[e];
+                }
+                store8(dst + half, y);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const float a = x[2 * e], b = x[2 * e + 1];
+                    x[2 * e] = a * c[e] - b * s[e];
+                    x[2 * e + 1] = a * s[e] + b * c[e];
+                }
+            }
+        }
+        store8(dst, x);
     }
 }
 
@@ -1876,15 +1992,31 @@ paged view_of(const lnsb_paged_kv & a) {
 }
 
 template <class TI, class TC>
-void launch_append(const lnsb_paged_append_args & a, cudaStream_t s) {
+int launch_append(const lnsb_paged_append_args & a, cudaStream_t s) {
     const lnsb_paged_kv & c = a.kv;
+    const TI * k = static_cast<const TI *>(a.k), * v = static_cast<const TI *>(a.v), * q = static_cast<const TI *>(a.q);
+    TC * qo = static_cast<TC *>(a.q_out), * kc = static_cast<TC *>(c.k_cache), * vc = static_cast<TC *>(c.v_cache);
+    const uintptr_t at = reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(q) |
+                         reinterpret_cast<uintptr_t>(qo) | reinterpret_cast<uintptr_t>(a.cos_sin);
+    const int64_t ld = ((a.k_ld | a.v_ld | a.q_ld) * (int64_t) sizeof(TI)) | (a.q_out_ld * (int64_t) sizeof(TC));
+    const bool neox = a.neox != 0;
+    if (at % 16 == 0 && ld % 16 == 0 && a.n_dims % 16 == 0) {
+        const int64_t per = (neox ? a.n_dims / 16 : a.n_dims / 8) + (c.head_dim - a.n_dims) / 8;
+        const int64_t units = (a.n_head + c.n_head_kv) * per + (int64_t) c.n_head_kv * (c.head_dim / 8);
+        // one thread a unit while that keeps a block within one token; short tokens share a block
+        const int64_t tokens = std::max<int64_t>(1, std::min<int64_t>(256 / units, c.n_tokens));
+        if (units > 0x7FFFFFFF / 2) return LNSB_E_TOO_LARGE;
+        auto kern = neox ? k_paged_append_vec<TI, TC, true> : k_paged_append_vec<TI, TC, false>;
+        launch_k(kern, dim3((unsigned) ((c.n_tokens + tokens - 1) / tokens)), dim3(256), 0, s, view_of(c), k, v, q, qo, a.cos_sin,
+                 a.k_ld, a.v_ld, a.q_ld, a.q_out_ld, a.n_head, c.head_dim, a.n_dims, (int) tokens, kc, vc);
+        return launch_status();
+    }
     const int64_t per = a.n_dims / 2 + (c.head_dim - a.n_dims);
     const int64_t n = c.n_tokens * ((int64_t) (a.n_head + c.n_head_kv) * per + (int64_t) c.n_head_kv * c.head_dim);
     const int64_t blocks = std::min<int64_t>((n + 255) / 256, k_sms * 64);
-    launch_k(k_paged_append<TI, TC>, dim3((unsigned) blocks), dim3(256), 0, s, view_of(c), static_cast<const TI *>(a.k),
-             static_cast<const TI *>(a.v), static_cast<const TI *>(a.q), static_cast<TC *>(a.q_out), a.cos_sin, a.k_ld, a.v_ld,
-             a.q_ld, a.q_out_ld, a.n_head, c.head_dim, a.n_dims, a.neox, static_cast<TC *>(c.k_cache),
-             static_cast<TC *>(c.v_cache));
+    launch_k(k_paged_append<TI, TC>, dim3((unsigned) blocks), dim3(256), 0, s, view_of(c), k, v, q, qo, a.cos_sin, a.k_ld, a.v_ld,
+             a.q_ld, a.q_out_ld, a.n_head, c.head_dim, a.n_dims, a.neox, kc, vc);
+    return launch_status();
 }
 
 constexpr int k_max_devices = 64;
@@ -2044,16 +2176,10 @@ int lnsb_paged_append(const lnsb_paged_append_args * a, lnsb_stream_t stream) {
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool f16 = c.type == LNSB_TYPE_F16;
     switch (a->in_type) {
-        case LNSB_TYPE_F32:
-            if (f16) launch_append<float, __half>(b, s); else launch_append<float, __nv_bfloat16>(b, s);
-            break;
-        case LNSB_TYPE_F16:
-            if (f16) launch_append<__half, __half>(b, s); else launch_append<__half, __nv_bfloat16>(b, s);
-            break;
-        default:
-            if (f16) launch_append<__nv_bfloat16, __half>(b, s); else launch_append<__nv_bfloat16, __nv_bfloat16>(b, s);
+        case LNSB_TYPE_F32: return f16 ? launch_append<float, __half>(b, s) : launch_append<float, __nv_bfloat16>(b, s);
+        case LNSB_TYPE_F16: return f16 ? launch_append<__half, __half>(b, s) : launch_append<__half, __nv_bfloat16>(b, s);
+        default:            return f16 ? launch_append<__nv_bfloat16, __half>(b, s) : launch_append<__nv_bfloat16, __nv_bfloat16>(b, s);
     }
-    return launch_status();
 }
 
 int64_t lnsb_paged_attn_work_bytes(void) { return A_WORK + B_WORK; }

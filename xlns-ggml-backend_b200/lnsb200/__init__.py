@@ -252,48 +252,39 @@ class KernelSet:
         _lib.check(self.lib, "lnsb_f16_to_f32", self.lib.lnsb_f16_to_f32(_ptr(src), _ptr(dst), n, _stream(stream)))
 
 
-    # ---- serving many sequences from a paged KV cache (no LNS: any format, any mode) ----
-    def _paged(self, k_cache, v_cache, page_table, q_start, kv_len, max_kv, n_tokens):
-        """lnsb_paged_kv of caches [n_pages][page_size][n_head_kv][head_dim] (any strides, dims contiguous), F16 or
-        BF16, with the plan arrays page_table [n_seqs][pages], q_start [n_seqs + 1], kv_len [n_seqs] (int32)"""
-        ty = _type_id(k_cache)
-        n_pages, page_size, n_head_kv, head_dim = k_cache.shape
-        st = k_cache.stride()
-        _want(v_cache.dtype == k_cache.dtype and v_cache.shape == k_cache.shape and v_cache.stride() == st and st[3] == 1,
-              "k_cache and v_cache must have the same type, shape and strides, with contiguous heads")
-        n_seqs, table_ld = page_table.shape
-        _want(page_table.dtype == q_start.dtype == kv_len.dtype == _int32() and page_table.is_contiguous()
-              and q_start.is_contiguous() and kv_len.is_contiguous() and q_start.numel() == n_seqs + 1
-              and kv_len.numel() == n_seqs, "page_table [n_seqs][pages], q_start [n_seqs + 1] and kv_len [n_seqs] must be "
-              "contiguous int32")
-        return (k_cache.data_ptr(), v_cache.data_ptr(), st[0], st[1], st[2], page_table.data_ptr(), q_start.data_ptr(),
-                kv_len.data_ptr(), table_ld, n_pages, n_tokens, max_kv, n_seqs, ty, page_size, n_head_kv, head_dim, 0)
-
+    # ---- serving many sequences from a paged KV cache (no LNS: any format, any mode).  A token's
+    # latency is a few microseconds of GPU time, so these bindings keep to few Python steps ----
     def paged_append(self, k, v, k_cache, v_cache, page_table, q_start, kv_len, max_kv, q=None, q_out=None, cos_sin=None,
                      neox=False, stream=None):
         """lnsb_paged_append: k, v [n_tokens][n_head_kv][head_dim] (F32, F16 or BF16; token rows any distance apart) into
-        the caches, k turned by cos_sin [rows][n_dims / 2][2] (F32; None: not turned); q [n_tokens][n_head][head_dim]
-        turned into q_out (of the caches' type)"""
-        T = k.shape[0]
-        _want(v.shape == k.shape and v.dtype == k.dtype and k.shape[1:] == k_cache.shape[2:] and _heads(k) and _heads(v),
-              "k and v must be [n_tokens][n_head_kv][head_dim] of one type, heads contiguous")
-        n_dims = 0
+        the caches [n_pages][page_size][n_head_kv][head_dim] (F16 or BF16; any strides, heads contiguous), k turned by
+        cos_sin [rows][n_dims / 2][2] (F32; None: not turned); q [n_tokens][n_head][head_dim] turned into q_out (of the
+        caches' type).  The plan: page_table [n_seqs][pages], q_start [n_seqs + 1], kv_len [n_seqs], int32 on the device"""
+        T, n_head_kv, D = k.shape
+        kv = _paged_kv(k_cache, v_cache, page_table, q_start, kv_len, max_kv, T)
+        ks, vs, ty = k.stride(), v.stride(), k.dtype
+        if not (v.shape == k.shape and v.dtype is ty and ty in _type_ids and kv[15] == n_head_kv and kv[16] == D
+                and _rows_ok(ks, n_head_kv, D) and _rows_ok(vs, n_head_kv, D)):
+            raise ValueError("k and v must be [n_tokens][n_head_kv][head_dim] of one type (F32, F16, BF16), heads contiguous")
+        cs = qp = op = None
+        n_dims = n_head = q_ld = o_ld = 0
         if cos_sin is not None:
-            n_dims = 2 * cos_sin.shape[1]
-            _want(cos_sin.dtype == _f32() and cos_sin.is_contiguous() and cos_sin.shape[0] >= max_kv
-                  and cos_sin.shape[2] == 2, "cos_sin must be contiguous F32 [rows >= max_kv][n_dims / 2][2]")
-        n_head = q_ld = qo_ld = 0
+            rows, half, two = cos_sin.shape
+            if not (cos_sin.dtype is _f32 and two == 2 and rows >= max_kv and cos_sin.is_contiguous()):
+                raise ValueError("cos_sin must be contiguous F32 [rows >= max_kv][n_dims / 2][2]")
+            n_dims, cs = 2 * half, cos_sin.data_ptr() if half else None
         if q is not None:
-            n_head, q_ld = q.shape[1], q.stride(0)
-            _want(q_out is not None and q_out.shape == q.shape and q.dtype == k.dtype and q_out.dtype == k_cache.dtype
-                  and q.shape[0] == T and q.shape[2] == k.shape[2] and _heads(q) and _heads(q_out),
-                  "q must be [n_tokens][n_head][head_dim] of k's type, q_out the same of the caches' type")
-            qo_ld = q_out.stride(0)
-        a = _lib.PagedAppendArgs(*self._paged(k_cache, v_cache, page_table, q_start, kv_len, max_kv, T), k.data_ptr(),
-                                 v.data_ptr(), q.data_ptr() if n_head else None, q_out.data_ptr() if n_head else None,
-                                 cos_sin.data_ptr() if n_dims else None, k.stride(0), v.stride(0), q_ld, qo_ld,
-                                 _type_id(k), n_head, n_dims, 1 if neox else 0)
-        _lib.check(self.lib, "lnsb_paged_append", self.lib.lnsb_paged_append(ctypes.byref(a), _stream(stream)))
+            n, n_head, d = q.shape
+            qs, qos = q.stride(), q_out.stride() if q_out is not None else ()
+            if not (q_out is not None and q_out.shape == q.shape and q.dtype is ty and q_out.dtype is k_cache.dtype and n == T
+                    and d == D and _rows_ok(qs, n_head, D) and _rows_ok(qos, n_head, D)):
+                raise ValueError("q must be [n_tokens][n_head][head_dim] of k's type, q_out the same of the caches' type")
+            q_ld, o_ld, qp, op = _ld(qs, T, n_head, D), _ld(qos, T, n_head, D), q.data_ptr(), q_out.data_ptr()
+        a = _lib.PagedAppendArgs(*kv, k.data_ptr(), v.data_ptr(), qp, op, cs, _ld(ks, T, n_head_kv, D), _ld(vs, T, n_head_kv, D),
+                                 q_ld, o_ld, _type_ids[ty], n_head, n_dims, 1 if neox else 0)
+        st = self.lib.lnsb_paged_append(ctypes.byref(a), _raw_stream(stream))
+        if st:
+            _lib.check(self.lib, "lnsb_paged_append", st)
 
     def paged_attn_work(self, device=None):
         """a workspace for paged_attn on one stream (zeroed, as its first use wants it)"""
@@ -302,16 +293,19 @@ class KernelSet:
 
     def paged_attn(self, q, k_cache, v_cache, page_table, q_start, kv_len, max_q, max_kv, dst, work, scale=None, window=0,
                    stream=None):
-        """lnsb_paged_attn: q, dst [n_tokens][n_head][head_dim] of the caches' type; scale None: 1 / sqrt(head_dim);
-        window 0: every earlier row is visible"""
-        _want(q.dtype == dst.dtype == k_cache.dtype and q.shape == dst.shape and q.shape[2] == k_cache.shape[3]
-              and _heads(q) and _heads(dst), "q and dst must be [n_tokens][n_head][head_dim] of the caches' type, heads "
-              "contiguous")
+        """lnsb_paged_attn: q, dst [n_tokens][n_head][head_dim] of the caches' type; the plan as in paged_append; scale
+        None: 1 / sqrt(head_dim); window 0: every earlier row is visible"""
         T, n_head, D = q.shape
-        a = _lib.PagedAttnArgs(*self._paged(k_cache, v_cache, page_table, q_start, kv_len, max_kv, T), q.data_ptr(),
-                               dst.data_ptr(), work.data_ptr(), work.numel() * work.element_size(), q.stride(0),
-                               dst.stride(0), max_q, window, n_head, D ** -0.5 if scale is None else scale)
-        _lib.check(self.lib, "lnsb_paged_attn", self.lib.lnsb_paged_attn(ctypes.byref(a), _stream(stream)))
+        kv = _paged_kv(k_cache, v_cache, page_table, q_start, kv_len, max_kv, T)
+        qs, ds, ty = q.stride(), dst.stride(), k_cache.dtype
+        if not (q.dtype is ty and dst.dtype is ty and dst.shape == q.shape and kv[16] == D and _rows_ok(qs, n_head, D)
+                and _rows_ok(ds, n_head, D)):
+            raise ValueError("q and dst must be [n_tokens][n_head][head_dim] of the caches' type, heads contiguous")
+        a = _lib.PagedAttnArgs(*kv, q.data_ptr(), dst.data_ptr(), work.data_ptr(), work.nbytes, _ld(qs, T, n_head, D),
+                               _ld(ds, T, n_head, D), max_q, window, n_head, D ** -0.5 if scale is None else scale)
+        st = self.lib.lnsb_paged_attn(ctypes.byref(a), _raw_stream(stream))
+        if st:
+            _lib.check(self.lib, "lnsb_paged_attn", st)
 
     def paged_errors(self):
         """(page ids outside the cache, waits that ran out) since the last call, on the current device"""
@@ -324,48 +318,70 @@ class KernelSet:
         apart) from one number u [n_rows] in [0, 1); token int32 [n_rows], prob F32 [n_rows] or None; temperature,
         top_p, min_p F32 [n_rows] and top_k int32 [n_rows], each or None"""
         R, V = logits.shape
-        _want(logits.stride(1) == 1 or V == 1, "logits must have contiguous rows")
-        for t, d in ((u, _f32()), (token, _int32()), (prob, _f32()), (temperature, _f32()), (top_k, _int32()),
-                     (top_p, _f32()), (min_p, _f32())):
-            _want(t is None or (t.dtype == d and t.numel() == R and t.is_contiguous()),
-                  "u, prob, temperature, top_p, min_p must be F32 [n_rows], token and top_k int32 [n_rows]")
-        a = _lib.SampleArgs(logits.data_ptr(), *(t.data_ptr() if t is not None else None
-                                                 for t in (temperature, top_k, top_p, min_p, u, token, prob)),
-                            logits.stride(0) if R > 1 else V, R, V, _type_id(logits))
-        _lib.check(self.lib, "lnsb_sample", self.lib.lnsb_sample(ctypes.byref(a), _stream(stream)))
+        if not _type_ids:
+            _load_types()
+        ld, step = logits.stride()
+        if not ((step == 1 or V == 1) and logits.dtype in _type_ids):
+            raise ValueError("logits must be F32, F16 or BF16 with contiguous rows")
+        a = _lib.SampleArgs(logits.data_ptr(), _row_ptr(temperature, _f32, R), _row_ptr(top_k, _i32, R), _row_ptr(top_p, _f32, R),
+                            _row_ptr(min_p, _f32, R), _row_ptr(u, _f32, R), _row_ptr(token, _i32, R), _row_ptr(prob, _f32, R),
+                            ld if R > 1 else V, R, V, _type_ids[logits.dtype])
+        st = self.lib.lnsb_sample(ctypes.byref(a), _raw_stream(stream))
+        if st:
+            _lib.check(self.lib, "lnsb_sample", st)
 
 
-def _want(ok, what):
-    if not ok:
-        raise ValueError(what)
+# torch's types, looked up at the first use (the module itself does not import torch)
+_type_ids = {}
+_f32 = _i32 = _current_stream = None
 
 
-def _int32():
+def _load_types():
+    global _f32, _i32, _current_stream
     import torch
-    return torch.int32
+    _current_stream = torch.cuda.current_stream
+    _f32, _i32 = torch.float32, torch.int32
+    _type_ids.update({_f32: _lib.TYPES["f32"], torch.float16: _lib.TYPES["f16"], torch.bfloat16: _lib.TYPES["bf16"]})
 
 
-def _f32():
-    import torch
-    return torch.float32
+def _raw_stream(stream):
+    """the given or the current stream's cudaStream_t"""
+    return (stream if stream is not None else _current_stream()).cuda_stream
 
 
-def _heads(t):
-    """[tokens][heads][dim] with a token's heads contiguous"""
-    return t.dim() == 3 and (t.stride(2) == 1 or t.shape[2] == 1) and (t.stride(1) == t.shape[2] or t.shape[1] == 1)
+def _rows_ok(st, heads, D):
+    """strides of [tokens][heads][D] whose rows are contiguous"""
+    return st[2] == 1 and (st[1] == D or heads == 1)
 
 
-_TYPE_IDS = {}
+def _ld(st, tokens, heads, D):
+    """elements between token rows; the stride of a single one may be anything"""
+    return st[0] if tokens > 1 else heads * D
 
 
-def _type_id(t):
-    if not _TYPE_IDS:
-        import torch
-        _TYPE_IDS.update({torch.float32: _lib.TYPES["f32"], torch.float16: _lib.TYPES["f16"],
-                          torch.bfloat16: _lib.TYPES["bf16"]})
-    if t.dtype not in _TYPE_IDS:
-        raise ValueError("%s is none of F32, F16 and BF16" % t.dtype)
-    return _TYPE_IDS[t.dtype]
+def _row_ptr(t, dtype, rows):
+    if t is None:
+        return None
+    if not (t.dtype is dtype and t.numel() == rows and t.is_contiguous()):
+        raise ValueError("u, prob, temperature, top_p, min_p must be F32 [n_rows], token and top_k int32 [n_rows]")
+    return t.data_ptr()
+
+
+def _paged_kv(k_cache, v_cache, page_table, q_start, kv_len, max_kv, n_tokens):
+    """the fields of lnsb_paged_kv"""
+    if not _type_ids:
+        _load_types()
+    n_pages, page_size, n_head_kv, head_dim = shape = k_cache.shape
+    st, ty = k_cache.stride(), k_cache.dtype
+    if not (v_cache.dtype is ty and ty in _type_ids and v_cache.shape == shape and v_cache.stride() == st and st[3] == 1):
+        raise ValueError("k_cache and v_cache must be [n_pages][page_size][n_head_kv][head_dim] of one type, with the same "
+                         "strides and contiguous heads")
+    n_seqs, table_ld = page_table.shape
+    if not (page_table.dtype is _i32 and q_start.dtype is _i32 and kv_len.dtype is _i32 and q_start.numel() == n_seqs + 1
+            and kv_len.numel() == n_seqs and page_table.is_contiguous() and q_start.is_contiguous() and kv_len.is_contiguous()):
+        raise ValueError("page_table [n_seqs][pages], q_start [n_seqs + 1] and kv_len [n_seqs] must be contiguous int32")
+    return (k_cache.data_ptr(), v_cache.data_ptr(), st[0], st[1], st[2], page_table.data_ptr(), q_start.data_ptr(),
+            kv_len.data_ptr(), table_ld, n_pages, n_tokens, max_kv, n_seqs, _type_ids[ty], page_size, n_head_kv, head_dim, 0)
 
 
 def kernels(fmt=XLNS16, mode="base"):
