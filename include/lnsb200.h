@@ -499,8 +499,8 @@ int lnsb_paged_errors(int64_t * bad_pages, int64_t * timeouts);
  * running sum of w passes u[r] times the kept ones' sum; prob is its w over
  * that sum.  t <= 0 takes the largest logit, the first of equal ones, with
  * prob 1.  A row without a logit above -inf gives token -1 and prob 0.
- * w is a 32-bit float, its sums are exact integers of 2^-40 (the remainder of
- * each w below that is dropped), so nothing hangs on an order of additions.
+ * w is a 32-bit float, its sums are integers of 2^-38 (each w rounded to the
+ * nearest), so nothing hangs on an order of additions.
  * temperature, top_k, top_p, min_p: per row, in device memory; NULL, or
  * top_k <= 0, top_p >= 1, min_p <= 0 in a row, leaves that filter out (NULL
  * temperature: 1).  u in [0, 1). */

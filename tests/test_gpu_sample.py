@@ -71,6 +71,27 @@ def test_sample(ks, type, vocab, spread):
 
 
 @pytest.mark.parametrize("type", sorted(TYPES))
+@pytest.mark.parametrize("vocab,rows", ((300001, 2), (1 << 20, 1), (20000, 160)))
+def test_long_rows_and_many(ks, type, vocab, rows):
+    """the largest vocabularies, more rows than SMs, and cuts deep in the row"""
+    g = torch.Generator().manual_seed(vocab)
+    pars = [(1.0, vocab // 3, 1.0, 0.0), (0.9, vocab // 2, 0.9, 0.0), (1.0, 0, 0.97, 0.0), (1.5, 0, 0.5, 1e-4),
+            (0.3, 0, 0.9, 0.0), (1.0, 4000, 0.99, 0.0), (1.0, 3000, 1.0, 0.01), (4.0, 0, 1.0, 0.6)]
+    x = (torch.randn((len(pars), vocab), generator=g) * 2.0).to(TYPES[type])
+    want = []
+    for r, (t, k, p, m) in enumerate(pars):
+        p = _safe_p(x[r], _f32(t), k, p) if 0 < p < 1 else p
+        want.append((t, k, p, m) + _case(x[r], t, k, p, m, g))
+    x = x.cuda()
+    for r0 in range(0, len(pars), rows):
+        part = [r % len(pars) for r in range(r0, r0 + rows)]
+        t, k, p, m, u, token, prob = zip(*(want[r] for r in part))
+        got, gp = _run(ks, x[part], u, t, k, p, m)
+        assert got == list(token)
+        assert all(abs(a - b) <= (2.0 ** -21 + vocab * 2.0 ** -40) * b + 1e-12 for a, b in zip(gp, prob))
+
+
+@pytest.mark.parametrize("type", sorted(TYPES))
 @pytest.mark.parametrize("rows", (1, 3, 200))
 def test_equal_logits_go_by_index(ks, type, rows):
     """every cut falls inside a run of equal logits: the lowest indices stay"""

@@ -1241,40 +1241,78 @@ k_paged_attn_tiles(const __grid_constant__ CUtensorMap kmap, const __grid_consta
 
 // ============================ sampling =====================================
 //
-// One cluster of CTAs a row; every logit is read once and stays in shared memory:
-// warp w of CTA c holds a contiguous part of the row, in order of index
-// (CTA, warp, vector, lane, element).  What bounds it is reading the logits
-// where there are many, and the cluster's barriers where there are few.
+// Where rows are fewer than SMs a cluster of CTAs takes a row and holds it in
+// shared memory, each logit read once; where they are more, one CTA does and
+// reads the row again in each step, from L2.  A warp has a contiguous part of
+// the row, in order of index (CTA, warp, vector, lane, element).  What bounds it
+// is instructions a logit where there are many rows, and the latencies of the
+// steps and of the cluster's barriers where there are few.
 //
-// The cut of the sorted order -- a key, and how many of the tokens that share
-// it stay -- is found without sorting the row.  A histogram over z = (x - max)
-// / t (1024 buckets of 28 / 1024, by count for top-k, by mass for top-p) gives
-// the bucket where the cut falls.  If few tokens lie above and in it, they go
-// to CTA 0, which sorts them and does the rest.  Otherwise the bucket's range
-// of 32-bit order-preserving keys is split again, 1024-fold a step, until one
-// key is left; then the token is found from the warps' masses.
+// The sorted order is cut without sorting the row:
+//   top-k    the k-th largest of the groups' maxima (a group: one place in one
+//            thread's vectors) is a bound that the k largest logits pass; the
+//            few that do go to a list, which is cut and finished;
+//   min-p    the logits near enough to the maximum go to the list;
+//   top-p    a histogram of the distance to the maximum bounds each bucket's
+//            mass from its count, and so the cut's place to a few buckets; one
+//            pass then takes the exact masses of all, of what lies above those
+//            buckets, and the list of what lies in them;
+//   a list that would be too long falls back to radix selection over the
+//            32-bit order-preserving keys.
 //
-// Masses are integers of 2^-40 of the largest weight: sums are exact in any
-// order, in histograms too, so the result hangs on no order of atomics.
+// Masses are integers of 2^-38 of the largest weight, rounded to nearest: sums
+// are exact in any order, so the result hangs on no order of atomics.
 
-constexpr int S_THREADS = 512, S_WARPS = S_THREADS / 32, S_VECS = 16, S_BUCKETS = 1024, S_LIST = 2048;
+constexpr int S_BUCKETS = 8192, S_COARSE = 1024, S_RADIX = 1024, S_LIST = 4096;
+constexpr int k_row_ctas = 4;                   // of a cluster at most: a peer's memory is slow to read
 constexpr float S_RANGE = 28.0f;               // exp(-28) < 2^-40: weightless
+constexpr float S_UNIT = 0x1p-38f;
 
 using ull = unsigned long long;
 
-__device__ __forceinline__ uint32_t order_key(float x) {          // x is no NaN, and no -0
-    const uint32_t b = __float_as_uint(x);
+__device__ __forceinline__ uint32_t order_key(float x) {          // x is no NaN
+    const uint32_t b = __float_as_uint(x + 0.0f);                 // -0 is 0
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ float key_value(uint32_t k) {
     return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k);
 }
-// w in [0, 1] in units of 2^-40, rounded down
+// w in [0, 1] as hi 2^-15 + lo 2^-38: adding 1.5 2^8 leaves the multiple of
+// 2^-15 in the low bits, adding 1.5 2^-15 to the remainder that of 2^-38
+constexpr float S_HI = 384.0f, S_LO = 0x1.8p-15f;
+__device__ __forceinline__ void mass_parts(float w, uint32_t & hi, uint32_t & lo) {
+    const float h = w + S_HI, r = w - (h - S_HI);
+    hi = __float_as_uint(h);
+    lo = __float_as_uint(r + S_LO);
+}
+__device__ __forceinline__ ull mass_sum(uint32_t hi, uint32_t lo, int n) {  // of n parts added up
+    const int h = (int) (hi - (uint32_t) n * 0x43C00000u), l = (int) (lo - (uint32_t) n * 0x38400000u);
+    return (ull) (((long long) h << 23) + l);
+}
 __device__ __forceinline__ ull mass_of(float w) {
-    const uint32_t b = __float_as_uint(w);
-    const int e = (int) (b >> 23) - 110;                          // w = mant * 2^(e - 40)
-    const uint32_t mant = (b & 0x7FFFFFu) | 0x800000u;
-    return (ull) (mant >> min(max(-e, 0), 31)) << max(e, 0);
+    uint32_t hi, lo;
+    mass_parts(w, hi, lo);
+    return mass_sum(hi, lo, 1);
+}
+
+// two floats in one instruction
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 c;
+    asm("{\n.reg .b64 x, y, z;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\nadd.rn.f32x2 z, x, y;\nmov.b64 {%0, %1}, z;\n}\n"
+        : "=f"(c.x), "=f"(c.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return c;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 c;
+    asm("{\n.reg .b64 x, y, z;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\nmul.rn.f32x2 z, x, y;\nmov.b64 {%0, %1}, z;\n}\n"
+        : "=f"(c.x), "=f"(c.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return c;
+}
+__device__ __forceinline__ void mass_parts2(float2 w, uint32_t (&hi)[2], uint32_t (&lo)[2]) {
+    const float2 h = add2(w, make_float2(S_HI, S_HI)), g = add2(h, make_float2(-S_HI, -S_HI));
+    const float2 l = add2(add2(w, make_float2(-g.x, -g.y)), make_float2(S_LO, S_LO));
+    hi[0] = __float_as_uint(h.x), hi[1] = __float_as_uint(h.y);
+    lo[0] = __float_as_uint(l.x), lo[1] = __float_as_uint(l.y);
 }
 
 struct sample_row {
@@ -1285,7 +1323,7 @@ struct sample_row {
                          const float * uniform) {
         const float t = temperature ? temperature[row] : 1.0f;
         greedy = !(t > 0.0f);
-        inv_t = 1.0f / t;
+        inv_t = fminf(1.0f / t, 3.4e38f);
         k = top_k ? top_k[row] : 0;
         if (k <= 0 || k > V) k = V;
         top_p = p ? p[row] : 1.0f;
@@ -1293,13 +1331,16 @@ struct sample_row {
         if (min_p != min_p) min_p = 0.0f;
         u = uniform[row];
     }
-    __device__ float z(float v) const { return v == top ? 0.0f : (v - top) * inv_t; }
-    __device__ float weight(float v) const { return v == top ? 1.0f : expf((v - top) * inv_t); }
-    __device__ ull   mass(float v) const {
-        const float w = weight(v);
-        return w >= 0x1p-40f ? mass_of(w) : 0ull;
+    // NaN and what is too far below: no weight
+    __device__ __forceinline__ float weight(float v) const { return expf(fmaxf((v - top) * inv_t, -100.0f)); }
+    __device__ __forceinline__ float2 distance2(float a, float b) const {
+        return add2(make_float2(a, b), make_float2(-top, -top));
     }
-    __device__ int bucket(float v) const { return min((int) (z(v) * (-S_BUCKETS / S_RANGE)), S_BUCKETS - 1); }
+    __device__ __forceinline__ float2 weight2(float2 d) const {
+        const float2 z = mul2(d, make_float2(inv_t, inv_t));
+        return make_float2(expf(fmaxf(z.x, -100.0f)), expf(fmaxf(z.y, -100.0f)));
+    }
+    __device__ __forceinline__ ull mass(float v) const { return mass_of(weight(v)); }
     // the masses' limit: what lies before a kept token stays at or below it
     __device__ ull mass_limit(ull whole) const {
         const double want = ceil((double) top_p * (double) whole);
@@ -1309,65 +1350,164 @@ struct sample_row {
         const ull g = (ull) ((double) fminf(fmaxf(u, 0.0f), 1.0f) * (double) total);
         return g < total ? g : total - 1;
     }
-    __device__ float prob(float w, ull total) const { return (float) ((double) w / ((double) total * 0x1p-40)); }
+    __device__ float prob(float w, ull total) const { return (float) ((double) w / ((double) total * (double) S_UNIT)); }
 };
 
-struct alignas(16) sample_smem {                // the row's vectors follow it
-    // a mass below 2^41 in three 14-bit parts: 2^16 of them fit 32 bits each
-    uint32_t hist[3][S_BUCKETS];
-    ull      list[S_LIST];
-    ull      sorted[S_LIST];       // CTA 0: the candidates of the cluster
-    ull      scan[S_WARPS + 1];
-    ull      warp_mass[S_WARPS];
-    uint32_t warp_ties[S_WARPS];
-    float    top[S_WARPS];
+struct alignas(16) sample_smem {   // the row's vectors follow it
+    ull      list[S_LIST];           // key << 32 | ~index: the sorted order
+    uint32_t hist[S_BUCKETS];      // counts, or four 11-bit parts of the masses of S_RADIX buckets
+    ull      scan[33], ends[32], part_mass[32];
+    uint32_t part_ties[32];
+    uint32_t list_mass[3][k_row_ctas * 32], list_ties[k_row_ctas * 32];   // CTA 0: what the list adds to the parts
+    ull      shared[2][2];         // sums that the cluster adds up, two uses in turn
+    float    hi[32], lo[32], top, low;
     uint32_t key_lo, key_hi;
-    int      best, n, first;
-    // CTA 0's answers
-    ull      above, inside;
-    int      bucket;
-    ull      goal, ties, total;
-    int      cta, warp;
+    int      n, best, first, b1, b2, at;
+    ull      above, goal, ties, total, v_lo, v_hi;
+    float    cut;
 };
 
-// inclusive scan over the block, total in *total
-__device__ __forceinline__ ull block_scan(ull v, ull * sums, ull * total) {
+// inclusive scan over the block, total in total
+template <int WARPS, class V>
+__device__ __forceinline__ V block_scan(V v, V * sums, V & total) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-        const ull o = __shfl_up_sync(0xFFFFFFFFu, v, d);
+        const V o = __shfl_up_sync(0xFFFFFFFFu, v, d);
         if (lane >= d) v += o;
     }
     __syncthreads();
     if (lane == 31) sums[warp] = v;
     __syncthreads();
-    ull t = 0;
-    for (int w = 0; w < S_WARPS; w++) {
-        if (w < warp) v += sums[w];
-        t += sums[w];
+    V s = lane < WARPS ? sums[lane] : V(0), run = s;
+#pragma unroll
+    for (int d = 1; d < WARPS; d <<= 1) {
+        const V o = __shfl_up_sync(0xFFFFFFFFu, run, d);
+        if (lane >= d) run += o;
     }
-    *total = t;
-    return v;
+    total = __shfl_sync(0xFFFFFFFFu, run, WARPS - 1);
+    return v + __shfl_sync(0xFFFFFFFFu, run - s, warp);
 }
-// falling order, n a power of two
-__device__ __forceinline__ void block_sort(ull * a, int n) {
-    for (int size = 2; size <= n; size <<= 1)
-        for (int d = size >> 1; d; d >>= 1) {
-            __syncthreads();
-            for (int i = threadIdx.x; i < n / 2; i += S_THREADS) {
-                const int x = 2 * i - (i & (d - 1)), y = x + d;
-                const bool down = (x & size) == 0;
-                const ull u = a[x], v = a[y];
-                if ((u < v) == down) {
-                    a[x] = v;
-                    a[y] = u;
-                }
-            }
-        }
+template <int WARPS, class V>
+__device__ __forceinline__ V block_sum(V v, V * sums) {
+#pragma unroll
+    for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, d);
     __syncthreads();
+    if ((threadIdx.x & 31) == 0) sums[threadIdx.x >> 5] = v;
+    __syncthreads();
+    V t = 0;
+#pragma unroll
+    for (int w = 0; w < WARPS; w++) t += sums[w];
+    return t;
+}
+// Of the block's items (those with m > 0, all v different) in falling order of
+// v: the last one that has at most `limit` of m before it.  A histogram over
+// the items' range, 1024-fold finer each time, until one item is left.
+template <int THREADS, int PER, class S>
+__device__ __forceinline__ ull block_select(const ull (&v)[PER], const ull (&m)[PER], ull limit, S & M) {
+    constexpr int PR = S_RADIX / THREADS;
+    const int tid = threadIdx.x, lane = tid & 31;
+    ull lo = ~0ull, hi = 0, above = 0;
+#pragma unroll
+    for (int j = 0; j < PER; j++)
+        if (m[j]) {
+            lo = min(lo, v[j]);
+            hi = max(hi, v[j]);
+        }
+#pragma unroll
+    for (int d = 16; d; d >>= 1) {
+        lo = min(lo, __shfl_xor_sync(0xFFFFFFFFu, lo, d));
+        hi = max(hi, __shfl_xor_sync(0xFFFFFFFFu, hi, d));
+    }
+    __syncthreads();
+    if (lane == 0) {
+        M.scan[tid >> 5] = lo;
+        M.ends[tid >> 5] = hi;
+    }
+    __syncthreads();
+    lo = lane < THREADS / 32 ? M.scan[lane] : ~0ull;
+    hi = lane < THREADS / 32 ? M.ends[lane] : 0ull;
+#pragma unroll
+    for (int d = 16; d; d >>= 1) {
+        lo = min(lo, __shfl_xor_sync(0xFFFFFFFFu, lo, d));
+        hi = max(hi, __shfl_xor_sync(0xFFFFFFFFu, hi, d));
+    }
+    while (lo < hi) {
+        const ull span = hi - lo;
+        const int shift = span < S_RADIX ? 0 : 54 - __clzll(span);
+        for (int i = tid; i < 2 * S_RADIX; i += THREADS) M.hist[i] = 0;
+        if (tid == 0) {
+            M.best = -1;
+            M.v_lo = ~0ull;
+            M.v_hi = 0;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < PER; j++)
+            if (m[j] && v[j] >= lo && v[j] <= hi) {               // 4096 items of 2^38: two sums of 19 bits each
+                const int b = (int) ((hi - v[j]) >> shift);
+                atomicAdd(&M.hist[b], (uint32_t) m[j] & 0x7FFFFu);
+                if (m[j] >> 19) atomicAdd(&M.hist[S_RADIX + b], (uint32_t) (m[j] >> 19));
+            }
+        __syncthreads();
+        ull c[PR], sum = 0, t;
+#pragma unroll
+        for (int j = 0; j < PR; j++) {
+            c[j] = M.hist[PR * tid + j] + ((ull) M.hist[S_RADIX + PR * tid + j] << 19);
+            sum += c[j];
+        }
+        ull run = above + block_scan<THREADS / 32>(sum, M.scan, t) - sum, at[PR];
+        int best = -1;
+#pragma unroll
+        for (int j = 0; j < PR; j++) {
+            at[j] = run;
+            if (c[j] && run <= limit) best = PR * tid + j;
+            run += c[j];
+        }
+        best = __reduce_max_sync(0xFFFFFFFFu, best);
+        if (lane == 0 && best >= 0) atomicMax(&M.best, best);
+        __syncthreads();
+        best = M.best;
+#pragma unroll
+        for (int j = 0; j < PR; j++)
+            if (PR * tid + j == best) M.above = at[j];
+#pragma unroll
+        for (int j = 0; j < PER; j++)
+            if (m[j] && v[j] >= lo && v[j] <= hi && (int) ((hi - v[j]) >> shift) == best) {
+                atomicMin(&M.v_lo, v[j]);
+                atomicMax(&M.v_hi, v[j]);
+            }
+        __syncthreads();
+        lo = M.v_lo;
+        hi = M.v_hi;
+        above = M.above;
+        __syncthreads();
+    }
+    return hi;
 }
 
-static_assert(sizeof(sample_smem) % 16 == 0, "vectors behind it");
+// falling order over the threads below `size` (a power of two from 32 on); the
+// other warps take no part
+__device__ __forceinline__ ull block_sort(ull v, int size, ull * a) {
+    const int tid = threadIdx.x;
+    if (tid >= size) return v;
+    auto sync = [&] { asm volatile("bar.sync 1, %0;\n" :: "r"(size) : "memory"); };
+    for (int run = 2; run <= size; run <<= 1)
+        for (int d = run >> 1; d; d >>= 1) {
+            ull o;
+            if (d < 32) {
+                o = __shfl_xor_sync(0xFFFFFFFFu, v, d);
+            } else {
+                sync();
+                a[tid] = v;
+                sync();
+                o = a[tid ^ d];
+            }
+            const bool larger = ((tid & run) == 0) == ((tid & d) == 0);
+            v = larger ? max(v, o) : min(v, o);
+        }
+    return v;
+}
 
 template <class T> struct vec16;
 template <> struct vec16<float> {
@@ -1375,579 +1515,763 @@ template <> struct vec16<float> {
     static __device__ __forceinline__ float at(const uint4 & v, int e) {
         return __uint_as_float(e == 0 ? v.x : e == 1 ? v.y : e == 2 ? v.z : v.w);
     }
+    static __device__ __forceinline__ float top(const uint4 & r) { return fmaxf(fmaxf(at(r, 0), at(r, 1)), fmaxf(at(r, 2), at(r, 3))); }
+    // the maximum of each place in the vectors; NaN counts for nothing
+    template <class Each> static __device__ __forceinline__ void maxima(Each each, float (&top)[N]) {
+#pragma unroll
+        for (int e = 0; e < N; e++) top[e] = -INFINITY;
+        each([&](const uint4 & r, int) {
+#pragma unroll
+            for (int e = 0; e < N; e++) top[e] = fmaxf(top[e], at(r, e));
+        });
+    }
 };
 template <class T> struct vec16 {
     static constexpr int N = 8;
     static __device__ __forceinline__ float at(const uint4 & v, int e) {
         const uint32_t w = e < 2 ? v.x : e < 4 ? v.y : e < 6 ? v.z : v.w;
+        if constexpr (std::is_same<T, __nv_bfloat16>::value) return __uint_as_float(e & 1 ? w & 0xFFFF0000u : w << 16);
         const uint16_t h = (uint16_t) (e & 1 ? w >> 16 : w & 0xFFFF);
         return num<T>::to(*reinterpret_cast<const T *>(&h));
     }
-};
-
-template <class T>
-__global__ void __launch_bounds__(S_THREADS, 2)
-k_sample(const T * __restrict__ logits, int64_t ld, int V, int vecs, const float * __restrict__ temperature,
-         const int32_t * __restrict__ top_k, const float * __restrict__ top_p, const float * __restrict__ min_p,
-         const float * __restrict__ u, int32_t * __restrict__ token, float * __restrict__ prob) {
-    constexpr int E = vec16<T>::N;
-    extern __shared__ __align__(16) unsigned char sample_sm[];
-    sample_smem & M = *reinterpret_cast<sample_smem *>(sample_sm);
-    cg::cluster_group cluster = cg::this_cluster();
-    const int C = (int) cluster.num_blocks(), cta = (int) cluster.block_rank();
-    const int64_t row = blockIdx.x / C;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    sample_smem & M0 = *cluster.map_shared_rank(&M, 0);
-    pdl_entry();
-
-    // ---- the logits: NaN and what lies beyond the row are -inf, -0 is 0
-    const T * x = logits + row * ld;
-    const int lead = (int) (reinterpret_cast<uintptr_t>(x) % 16 / sizeof(T));    // vectors start at 16-byte boundaries
-    const int base = (cta * S_WARPS + warp) * vecs * 32 * E + lane * E - lead;   // index of element e of vector i: + i * 32 * E + e
-    uint4 * const mine = reinterpret_cast<uint4 *>(sample_sm + sizeof(sample_smem)) + tid;   // vector i at i * S_THREADS
-    for (int i = 0; i < vecs; i++) {
-        const int at = base + i * 32 * E;
-        if (at >= 0 && at + E <= V) {
-            cp16(smem_addr(mine + i * S_THREADS), x + at, true);
-        } else {
-            alignas(16) T t[E];
+    using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+    static __device__ __forceinline__ float top(const uint4 & r) {
+        const T2 a = __hmax2(__hmax2(*reinterpret_cast<const T2 *>(&r.x), *reinterpret_cast<const T2 *>(&r.y)),
+                             __hmax2(*reinterpret_cast<const T2 *>(&r.z), *reinterpret_cast<const T2 *>(&r.w)));
+        return num<T>::to(__hmax(a.x, a.y));
+    }
+    template <class Each> static __device__ __forceinline__ void maxima(Each each, float (&top)[N]) {
+        const T none = num<T>::from(-INFINITY);
+        T2 m[4];
 #pragma unroll
-            for (int e = 0; e < E; e++) t[e] = at + e >= 0 && at + e < V ? x[at + e] : num<T>::from(-INFINITY);
-            mine[i * S_THREADS] = *reinterpret_cast<const uint4 *>(t);
+        for (int e = 0; e < 4; e++) m[e] = T2(none, none);
+        each([&](const uint4 & r, int) {
+            const uint32_t w[4] = { r.x, r.y, r.z, r.w };
+#pragma unroll
+            for (int e = 0; e < 4; e++) m[e] = __hmax2(m[e], *reinterpret_cast<const T2 *>(&w[e]));
+        });
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            top[2 * e] = num<T>::to(m[e].x);
+            top[2 * e + 1] = num<T>::to(m[e].y);
         }
     }
-    cp_commit();
-    auto value = [&](const uint4 & r, int e) {
-        const float v = vec16<T>::at(r, e);
-        return v == v ? v + 0.0f : -INFINITY;
+};
+
+template <class T, int THREADS, bool HELD>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS)
+k_sample(const T * __restrict__ logits, int64_t ld, int V, int vecs, int C, const float * __restrict__ temperature,
+         const int32_t * __restrict__ top_k, const float * __restrict__ top_p, const float * __restrict__ min_p,
+         const float * __restrict__ u, int32_t * __restrict__ token, float * __restrict__ prob) {
+    constexpr int E = vec16<T>::N, WARPS = THREADS / 32, PER = S_LIST / THREADS;
+    extern __shared__ __align__(16) unsigned char sample_sm[];
+    using smem = sample_smem;
+    smem & M = *reinterpret_cast<smem *>(sample_sm);
+    const int64_t row = blockIdx.x / C;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int cta = HELD ? (int) (blockIdx.x % C) : 0;            // the cluster is the row's C CTAs in order
+    auto peer = [&](int c) -> smem & {
+        if constexpr (HELD) return *cg::this_cluster().map_shared_rank(&M, c);
+        return M;
     };
+    auto csync = [&] {
+        if (HELD && C > 1) cg::this_cluster().sync();
+        else __syncthreads();
+    };
+    const T * x = logits + row * ld;
+    const int lead = (int) (reinterpret_cast<uintptr_t>(x) % 16 / sizeof(T));    // vectors start at 16-byte boundaries
+    // vector i of the row, 32 lanes of E elements: warp w of CTA c has vecs of them from (c * WARPS + w) * vecs on
+    const int origin = lane * E - lead, w_first = (cta * WARPS + warp) * vecs;
+    uint4 * const held = reinterpret_cast<uint4 *>(sample_sm + sizeof(smem)) + lane;
+    auto ends = [&](int at) {                  // a vector at the row's ends: -inf beyond them
+        alignas(16) T t[E];
+#pragma unroll
+        for (int e = 0; e < E; e++) t[e] = at + e >= 0 && at + e < V ? x[at + e] : num<T>::from(-INFINITY);
+        return *reinterpret_cast<const uint4 *>(t);
+    };
+    auto fetch = [&](int i) {
+        if constexpr (HELD) return held[(i - cta * WARPS * vecs) * 32];
+        const int at = origin + i * 32 * E;
+        if (at >= 0 && at + E <= V) return __ldg(reinterpret_cast<const uint4 *>(x + at));
+        return ends(at);
+    };
+    // f(vector, index of its first element) for the row's vectors from .. to - 1; eight on their way at a time
+    auto each_vec = [&](int from, int to, auto f) {
+        constexpr int N = HELD ? 1 : 8;
+        for (int i = from; i < to; i += N) {
+            uint4 r[N];
+#pragma unroll
+            for (int j = 0; j < N; j++)
+                if (i + j < to) r[j] = fetch(i + j);
+#pragma unroll
+            for (int j = 0; j < N; j++)
+                if (i + j < to) f(r[j], origin + (i + j) * 32 * E);
+        }
+    };
+    // f(value, index, its place in the vector) for this warp's part
+    auto each = [&](auto f) {
+        each_vec(w_first, w_first + vecs, [&](const uint4 & r, int at) {
+#pragma unroll
+            for (int e = 0; e < E; e++) f(vec16<T>::at(r, e), at + e, e);
+        });
+    };
+    // sums over the cluster's threads
+    int turn = 0;
+    auto cluster_sum = [&](ull a, ull b, ull & all_a, ull & all_b) {
+        a = block_sum<WARPS>(a, M.scan);
+        b = block_sum<WARPS>(b, M.scan);
+        if (tid == 0) {
+            M.shared[turn][0] = a;
+            M.shared[turn][1] = b;
+        }
+        csync();
+        all_a = lane < C ? peer(lane).shared[turn][0] : 0ull;     // side by side: a peer's memory is far
+        all_b = lane < C ? peer(lane).shared[turn][1] : 0ull;
+#pragma unroll
+        for (int d = 1; d < k_row_ctas; d <<= 1) {
+            all_a += __shfl_xor_sync(0xFFFFFFFFu, all_a, d);
+            all_b += __shfl_xor_sync(0xFFFFFFFFu, all_b, d);
+        }
+        all_a = __shfl_sync(0xFFFFFFFFu, all_a, 0);
+        all_b = __shfl_sync(0xFFFFFFFFu, all_b, 0);
+        turn ^= 1;
+    };
+    pdl_entry();
+    if constexpr (HELD) {
+        for (int i = 0; i < vecs; i++) {
+            const int at = origin + (w_first + i) * 32 * E;
+            uint4 * to = held + (warp * vecs + i) * 32;
+            if (at >= 0 && at + E <= V) cp16(smem_addr(to), x + at, true);
+            else *to = ends(at);
+        }
+        cp_commit();
+    }
     sample_row R;
     R.read(row, V, temperature, top_k, top_p, min_p, u);
-    // ---- the maximum
-    float top = -INFINITY;
-    cp_wait<0>();                              // a thread reads only what it has fetched
-    for (int i = 0; i < vecs; i++) {
-        const uint4 r = mine[i * S_THREADS];
-#pragma unroll
-        for (int e = 0; e < E; e++) top = fmaxf(top, vec16<T>::at(r, e));
-    }
-#pragma unroll
-    for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
-    if (lane == 0) M.top[warp] = top;
+    for (int i = tid; i < S_BUCKETS; i += THREADS) M.hist[i] = 0;
+    for (int i = tid; i < 3 * k_row_ctas * 32; i += THREADS) (&M.list_mass[0][0])[i] = 0;
+    for (int i = tid; i < k_row_ctas * 32; i += THREADS) M.list_ties[i] = 0;
     if (tid == 0) {
         M.n = 0;
         M.first = 0x7FFFFFFF;
+        M.b1 = M.b2 = S_BUCKETS;
+        M.key_lo = 0xFFFFFFFFu;
+        M.key_hi = 0;
     }
-    cluster.sync();
-    for (int i = lane; i < C * S_WARPS; i += 32) top = fmaxf(top, cluster.map_shared_rank(&M, i / S_WARPS)->top[i % S_WARPS]);
+    if constexpr (HELD) cp_wait<0>();          // a lane reads only what it has fetched, until the barrier
+
+    // ---- the largest and the smallest finite logit, and the groups' maxima
+    float group[E], low = INFINITY, top = -INFINITY;
+    vec16<T>::maxima([&](auto f) { each_vec(w_first, w_first + vecs, f); }, group);
 #pragma unroll
-    for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
-    R.top = top + 0.0f;
-    if (R.top == -INFINITY || R.greedy) {
-        if (R.top != -INFINITY) {
-            int first = 0x7FFFFFFF;
-            for (int i = vecs - 1; i >= 0; i--) {
-                const uint4 r = mine[i * S_THREADS];
+    for (int g = 0; g < E; g++) top = fmaxf(top, group[g]);
+    if (R.top_p < 1.0f && !R.greedy) each([&](float v, int, int) { low = fminf(low, v == -INFINITY ? INFINITY : v); });
+    auto warp_ends = [&] {
 #pragma unroll
-                for (int e = E - 1; e >= 0; e--)
-                    if (value(r, e) == R.top) first = base + i * 32 * E + e;
-            }
-            first = __reduce_min_sync(0xFFFFFFFFu, first);
-            if (lane == 0 && first != 0x7FFFFFFF) atomicMin(&M0.first, first);
+        for (int d = 16; d; d >>= 1) {
+            top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
+            low = fminf(low, __shfl_xor_sync(0xFFFFFFFFu, low, d));
         }
-        cluster.sync();
+    };
+    warp_ends();
+    if (lane == 0) {
+        M.hi[warp] = top;
+        M.lo[warp] = low;
+    }
+    __syncthreads();
+    top = lane < WARPS ? M.hi[lane] : -INFINITY;
+    low = lane < WARPS ? M.lo[lane] : INFINITY;
+    warp_ends();
+    if (HELD && C > 1) {
+        if (tid == 0) {
+            M.top = top;
+            M.low = low;
+        }
+        csync();
+        if (lane < C) {
+            top = peer(lane).top;
+            low = peer(lane).low;
+        }
+        warp_ends();
+    }
+    R.top = top + 0.0f;
+    if (top == -INFINITY || R.greedy) {
+        int at = 0x7FFFFFFF;
+        if (top != -INFINITY) each([&](float v, int i, int) {
+            if (v == top) at = min(at, i);
+        });
+        at = __reduce_min_sync(0xFFFFFFFFu, at);
+        if (lane == 0 && at != 0x7FFFFFFF) atomicMin(&peer(0).first, at);
+        csync();
         if (cta == 0 && tid == 0) {
-            token[row] = R.top == -INFINITY ? -1 : M.first;
-            if (prob) prob[row] = R.top == -INFINITY ? 0.0f : 1.0f;
+            token[row] = top == -INFINITY ? -1 : M.first;
+            if (prob) prob[row] = top == -INFINITY ? 0.0f : 1.0f;
         }
         return;
     }
 
-    uint32_t cut = 0;                          // kept: key > cut, and the first `ties` of key == cut
-    ull ties = (ull) V;
-    for (int by_mass = 0; by_mass < 2; by_mass++) {
-        if (by_mass ? !(R.top_p < 1.0f) : R.k >= V) continue;
-        ull limit = (ull) (R.k - 1), above = 0, whole = 0;
-        uint32_t key_lo = 0, key_hi = 0;
-        int shift = 32;                        // 32: the buckets of z
-        while (true) {
+    // kept: above `cut`, and the first `ties` equal to it
+    float cut = -INFINITY;
+    ull ties = 0, whole = 0;
+    const bool by_k = R.k < V, by_p = R.top_p < 1.0f;
+
+    // ---- CTA 0: the list, cut and finished.  `above`: the mass before it, whose tokens stay; with `open` the tokens
+    // above the list are not in it: the cut is found, and what is kept is left to the steps below
+    auto set_cut = [&](uint32_t key, int kept_equal) {
+        cut = key_value(key);
+        for (int i = tid; i < k_row_ctas * 32; i += THREADS) M.list_mass[0][i] = M.list_mass[1][i] = M.list_mass[2][i] = M.list_ties[i] = 0;
+        ties = block_sum<WARPS>(kept_equal, reinterpret_cast<int *>(M.scan));
+    };
+    // a kept token of the list counts for its warp; 4096 masses in three 14-bit parts fit 32 bits
+    auto add_to_part = [&](ull token_key, float w) {
+        const int part = (int) (~(uint32_t) token_key + lead) / (vecs * 32 * E);
+        if (key_value((uint32_t) (token_key >> 32)) == cut) {
+            atomicAdd(&M.list_ties[part], 1u);
+        } else {
+            const ull m = mass_of(w);
+            atomicAdd(&M.list_mass[0][part], (uint32_t) m & 0x3FFFu);
+            if (m >> 14) atomicAdd(&M.list_mass[1][part], (uint32_t) (m >> 14) & 0x3FFFu);
+            if (m >> 28) atomicAdd(&M.list_mass[2][part], (uint32_t) (m >> 28));
+        }
+    };
+    auto finish_sorted = [&](int n, ull above, bool open) {       // n <= THREADS: one token a thread
+        int size = 32;
+        while (size < n) size <<= 1;
+        const ull mine = tid < n ? M.list[tid] : 0ull;
+        __syncthreads();                       // the list's place is free
+        ull a = block_sort(mine, size, M.list), total;
+        float w = a ? R.weight(key_value((uint32_t) (a >> 32))) : 0.0f;
+        ull m = a && tid < R.k ? mass_of(w) : 0ull;
+        const ull run = above + block_scan<WARPS>(m, M.scan, total) - m;
+        if (by_k) whole = total;
+        const bool keep = a && tid < R.k && (!by_p || run <= R.mass_limit(whole)) && w >= R.min_p;
+        if (open) {
+            const int all = __syncthreads_count(keep);            // the list's first ones
+            if (all == 0) return;                                 // min_p: nothing of the list stays
+            if (tid == all - 1) M.key_lo = (uint32_t) (a >> 32);
             __syncthreads();
-            for (int i = tid; i < (by_mass ? 3 : 1) * S_BUCKETS; i += S_THREADS) (&M.hist[0][0])[i] = 0;
-            if (tid == 0) {
-                M.best = 0;
-                M.key_lo = 0xFFFFFFFFu;
-                M.key_hi = 0;
-            }
-            __syncthreads();
-            for (int i = 0; i < vecs; i++) {
-                const uint4 r = mine[i * S_THREADS];
+            const uint32_t key = M.key_lo;
+            set_cut(key, keep && (uint32_t) (a >> 32) == key);
+            if (keep) add_to_part(a, w);
+            return;
+        }
+        // ~index first: falling in order of index
+        a = block_sort(keep ? (ull) (uint32_t) a << 32 | (uint32_t) (a >> 32) : 0ull, size, M.list);
+        w = a ? R.weight(key_value((uint32_t) a)) : 0.0f;
+        m = a ? mass_of(w) : 0ull;
+        const ull upto = block_scan<WARPS>(m, M.scan, total), goal = R.goal(total);
+        if (m && goal < upto && goal >= upto - m) {
+            token[row] = (int32_t) ~(uint32_t) (a >> 32);
+            if (prob) prob[row] = R.prob(w, total);
+        }
+    };
+    auto finish_selected = [&](int n, ull above, bool open) {
+        ull a[PER], m[PER];
+        float w[PER];
 #pragma unroll
-                for (int e = 0; e < E; e++) {
-                    const float v = value(r, e);
-                    const uint32_t key = order_key(v);
-                    if (key < cut || (shift < 32 && (key < key_lo || key > key_hi)) || v == -INFINITY) continue;
-                    const int b = shift == 32 ? R.bucket(v) : (int) ((key_hi - key) >> shift);
-                    if (!by_mass) {
-                        atomicAdd(&M.hist[0][b], 1u);
-                    } else {
-                        const ull m = R.mass(v);
-                        if (m) {
-                            atomicAdd(&M.hist[0][b], (uint32_t) m & 0x3FFFu);
-                            atomicAdd(&M.hist[1][b], (uint32_t) (m >> 14) & 0x3FFFu);
-                            atomicAdd(&M.hist[2][b], (uint32_t) (m >> 28));
+        for (int j = 0; j < PER; j++) {
+            const int i = tid + j * THREADS;
+            a[j] = i < n ? M.list[i] : 0ull;
+            w[j] = i < n ? R.weight(key_value((uint32_t) (a[j] >> 32))) : 0.0f;
+            m[j] = i < n ? 1ull : 0ull;
+        }
+        auto cut_off = [&](ull limit) {
+            const ull last = block_select<THREADS>(a, m, limit, M);
+#pragma unroll
+            for (int j = 0; j < PER; j++)
+                if (a[j] < last) a[j] = 0;
+        };
+        if (by_k && n > R.k) cut_off((ull) R.k - 1);
+        ull sum = 0;
+#pragma unroll
+        for (int j = 0; j < PER; j++) sum += m[j] = a[j] ? mass_of(w[j]) : 0ull;
+        if (by_k) whole = block_sum<WARPS>(sum, M.scan);
+        if (by_p) cut_off(max(R.mass_limit(whole), above) - above);
+#pragma unroll
+        for (int j = 0; j < PER; j++)
+            if (!(w[j] >= R.min_p)) a[j] = 0;
+        if (open) {
+            uint32_t key = 0xFFFFFFFFu;
+#pragma unroll
+            for (int j = 0; j < PER; j++)
+                if (a[j]) key = min(key, (uint32_t) (a[j] >> 32));
+            key = __reduce_min_sync(0xFFFFFFFFu, key);
+            __syncthreads();
+            if (tid == 0) M.key_lo = 0xFFFFFFFFu;
+            __syncthreads();
+            if (lane == 0) atomicMin(&M.key_lo, key);
+            __syncthreads();
+            key = M.key_lo;
+            if (key == 0xFFFFFFFFu) return;
+            int eq = 0;
+#pragma unroll
+            for (int j = 0; j < PER; j++) eq += a[j] && (uint32_t) (a[j] >> 32) == key;
+            set_cut(key, eq);
+#pragma unroll
+            for (int j = 0; j < PER; j++)
+                if (a[j]) add_to_part(a[j], w[j]);
+            return;
+        }
+        sum = 0;
+#pragma unroll
+        for (int j = 0; j < PER; j++) {
+            sum += m[j] = a[j] ? mass_of(w[j]) : 0ull;
+            a[j] = (uint32_t) a[j];
+        }
+        const ull total = block_sum<WARPS>(sum, M.scan);
+        const ull pick = block_select<THREADS>(a, m, R.goal(total), M);
+#pragma unroll
+        for (int j = 0; j < PER; j++)
+            if (m[j] && a[j] == pick) {
+                token[row] = (int32_t) ~(uint32_t) pick;
+                if (prob) prob[row] = R.prob(w[j], total);
+            }
+    };
+    // the list (n tokens, with `apart` in the CTAs' own lists), finished by CTA 0; true: the row is done
+    auto finish = [&](int n, ull above, bool open, bool apart) {
+        if (apart && cta == 0 && C > 1) {
+            // warp w copies of CTA w % C
+            const int nc = lane < C ? peer(lane).n : 0, c = warp % C;
+            int at = 0;
+            for (int r = 0; r < c; r++) at += __shfl_sync(0xFFFFFFFFu, nc, r);
+            const int mine = __shfl_sync(0xFFFFFFFFu, nc, c);
+            if (c > 0)
+                for (int i = warp / C * 32 + lane; i < mine; i += WARPS / C * 32) M.list[at + i] = peer(c).list[i];
+        }
+        if (apart) csync();                    // CTA 0 has them all
+        if (cta == 0) {
+            if (n <= THREADS) finish_sorted(n, above, open);
+            else finish_selected(n, above, open);
+            if (open && tid == 0) {
+                M.cut = cut;
+                M.ties = ties;
+            }
+        }
+        if (!open) {
+            if (HELD && C > 1 && cta == 0) cg::this_cluster().sync();    // the others have read its memory, and are gone
+            return true;
+        }
+        csync();
+        cut = peer(0).cut;
+        ties = peer(0).ties;
+        return false;
+    };
+    auto push = [&](float v, int i) {
+        const int at = atomicAdd(&M.n, 1);
+        if (at < S_LIST) M.list[at] = (ull) order_key(v) << 32 | (uint32_t) ~i;
+    };
+    auto listed = [&] {                        // after a barrier
+        return (int) __reduce_add_sync(0xFFFFFFFFu, lane < C ? (uint32_t) min(peer(lane).n, S_LIST + 1) : 0u);
+    };
+
+    bool found = false;                        // cut and ties are known
+    bool parts_known = false;                  // and the warps' masses: above the list in part_mass, the list's in list_mass
+    if (top == INFINITY || (by_p && low >= top)) {
+        // nothing but the maximum has a weight, or every logit is the maximum
+        ull eq = 0, none;
+        each([&](float v, int, int) { eq += v == top; });
+        cluster_sum(eq, 0, eq, none);
+        ties = min(eq, (ull) R.k);
+        if (by_p) ties = max(1ull, min(ties, (ull) ceil((double) R.top_p * (double) ties)));
+        cut = top;
+        found = true;
+    } else if (by_k || by_p || R.min_p > 0.0f) {
+        // distance to the maximum in buckets: up to the smallest logit, or to where nothing weighs
+        const float reach = fminf(low < top ? top - low : INFINITY, S_RANGE / R.inv_t);
+        const float q = -(S_BUCKETS - 1) / reach;
+        auto place = [&](float v) { return (v - top) * q; };      // NaN, or S_BUCKETS and more: none
+        float below = 0.0f;                                       // the list: place < below
+        bool list = false;
+        if (by_k) {
+            // every group's maximum is a logit: where k of them are, k logits are
+#pragma unroll
+            for (int g = 0; g < E; g++) {
+                const float b = place(group[g]);
+                if (b < S_BUCKETS) atomicAdd(&M.hist[(int) b / (S_BUCKETS / S_COARSE)], 1u);
+            }
+            csync();
+            // every CTA adds up the cluster's histograms for itself
+            constexpr int PB = (S_COARSE + THREADS - 1) / THREADS;
+            uint32_t c[PB] = {}, sum = 0, all, h[PB][k_row_ctas];
+#pragma unroll
+            for (int j = 0; j < PB; j++)
+#pragma unroll
+                for (int r = 0; r < k_row_ctas; r++)
+                    if (r < C) h[j][r] = peer(r).hist[PB * tid + j];
+#pragma unroll
+            for (int j = 0; j < PB; j++) {
+#pragma unroll
+                for (int r = 0; r < k_row_ctas; r++)
+                    if (r < C) c[j] += h[j][r];
+                sum += c[j];
+            }
+            uint32_t run = block_scan<WARPS>(sum, reinterpret_cast<uint32_t *>(M.scan), all) - sum;
+            int b1 = S_COARSE;
+#pragma unroll
+            for (int j = 0; j < PB; j++) {
+                run += c[j];
+                if (run >= (uint32_t) R.k) b1 = min(b1, PB * tid + j);
+            }
+            b1 = __reduce_min_sync(0xFFFFFFFFu, b1);
+            if (lane == 0) atomicMin(&M.b1, b1);
+            __syncthreads();
+            below = (float) min(S_BUCKETS, (M.b1 + 1) * (S_BUCKETS / S_COARSE));
+            list = true;
+        } else if (by_p) {
+            // a CTA that holds its part has less than 2^16 logits: two counts to a word, for the cluster's sake
+            each([&](float v, int, int) {
+                const float b = place(v);
+                if (b < S_BUCKETS) {
+                    if (HELD) atomicAdd(&M.hist[(int) b >> 1], (int) b & 1 ? 0x10000u : 1u);
+                    else atomicAdd(&M.hist[(int) b], 1u);
+                }
+            });
+        } else {
+            // exp(-d) >= min_p, with room for exp's and the logarithm's rounding
+            below = fminf((float) S_BUCKETS, (1e-3f - logf(R.min_p)) / R.inv_t * -q + 1.0f);
+            list = true;
+        }
+        if (!list) {
+            csync();
+            constexpr int PB = S_BUCKETS / THREADS;
+            uint32_t c[PB] = {};
+            if constexpr (HELD) {
+                uint4 h[PB / 8][k_row_ctas];
+#pragma unroll
+                for (int j = 0; j < PB / 8; j++)
+#pragma unroll
+                    for (int r = 0; r < k_row_ctas; r++)
+                        if (r < C) h[j][r] = reinterpret_cast<const uint4 *>(peer(r).hist + PB / 2 * tid)[j];
+#pragma unroll
+                for (int j = 0; j < PB / 8; j++)
+#pragma unroll
+                    for (int r = 0; r < k_row_ctas; r++)
+                        if (r < C) {
+                            const uint32_t w[4] = { h[j][r].x, h[j][r].y, h[j][r].z, h[j][r].w };
+#pragma unroll
+                            for (int e = 0; e < 4; e++) {
+                                c[8 * j + 2 * e] += w[e] & 0xFFFFu;
+                                c[8 * j + 2 * e + 1] += w[e] >> 16;
+                            }
+                        }
+            } else {
+#pragma unroll
+                for (int j = 0; j < PB; j++) c[j] = M.hist[PB * tid + j];
+            }
+                // each bucket's mass lies between count x its ends' weights; 1e-4 for the rounding of places and sums
+                const float step = R.inv_t / -q, ratio = expf(-step), w_first_bucket = expf(-step * (PB * tid));
+                float least = 0, most = 0, all_least, all_most, wb = w_first_bucket;
+#pragma unroll
+                for (int j = 0; j < PB; j++) {
+                    most += c[j] * wb;
+                    wb *= ratio;
+                    least += c[j] * wb;
+                }
+                float * fs = reinterpret_cast<float *>(M.scan);
+                const float least_upto = block_scan<WARPS>(least, fs, all_least);
+                float lower = least_upto - least, upper = block_scan<WARPS>(most, fs, all_most) - most;
+                int b1 = S_BUCKETS, b2 = S_BUCKETS;
+                wb = w_first_bucket;
+#pragma unroll
+                for (int j = 0; j < PB; j++) {
+                    upper += c[j] * wb;
+                    wb *= ratio;
+                    lower += c[j] * wb;
+                    if (upper * 1.0001f >= R.top_p * all_least * 0.9999f) b1 = min(b1, PB * tid + j);
+                    if (lower * 0.9999f >= R.top_p * all_most * 1.0001f) b2 = min(b2, PB * tid + j);
+                }
+                b1 = __reduce_min_sync(0xFFFFFFFFu, b1);
+                b2 = __reduce_min_sync(0xFFFFFFFFu, b2);
+                if (lane == 0) {
+                    atomicMin(&M.b1, b1);
+                    atomicMin(&M.b2, b2);
+                }
+                __syncthreads();
+                b1 = M.b1 == S_BUCKETS ? 0 : M.b1;
+                b2 = min(M.b2, S_BUCKETS - 1);
+                // all down to the cut's buckets, if they are few, else the cut's buckets
+                uint32_t upto = 0;
+#pragma unroll
+                for (int j = 0; j < PB; j++) upto += PB * tid + j <= b2 ? c[j] : 0u;
+                upto = block_sum<WARPS>(upto, reinterpret_cast<uint32_t *>(M.scan));
+                const float from = upto <= S_LIST ? 0.0f : (float) b1, to = (float) b2 + 1.0f;
+                ull all_m = 0, above_m = 0, above;
+                uint32_t klo = 0xFFFFFFFFu, khi = 0;
+                each_vec(w_first, w_first + vecs, [&](const uint4 & r, int at) {
+                    uint32_t hi = 0, lo = 0, ahi = 0, alo = 0;
+                    int an = 0;
+                    bool some = false;
+#pragma unroll
+                    for (int e = 0; e < E; e += 2) {
+                        const float2 d = R.distance2(vec16<T>::at(r, e), vec16<T>::at(r, e + 1)), b2 = mul2(d, make_float2(q, q));
+                        uint32_t h[2], l[2];
+                        mass_parts2(R.weight2(d), h, l);
+#pragma unroll
+                        for (int j = 0; j < 2; j++) {
+                            const float b = j ? b2.y : b2.x;
+                            const bool over = b < from;
+                            hi += h[j];
+                            lo += l[j];
+                            ahi += over ? h[j] : 0u;
+                            alo += over ? l[j] : 0u;
+                            an += over;
+                            some |= !over && b < to;
                         }
                     }
-                }
-            }
-            cluster.sync();
-            if (cta == 0) {
-                ull v[2] = { 0, 0 }, total;
+                    all_m += mass_sum(hi, lo, E);
+                    above_m += mass_sum(ahi, alo, an);
+                    if (some) {
 #pragma unroll
-                for (int j = 0; j < 2; j++)
-                    for (int c = 0; c < C; c++) {
-                        const sample_smem & Mc = *cluster.map_shared_rank(&M, c);
-                        v[j] += Mc.hist[0][2 * tid + j];
-                        if (by_mass) v[j] += ((ull) Mc.hist[1][2 * tid + j] << 14) + ((ull) Mc.hist[2][2 * tid + j] << 28);
+                        for (int e = 0; e < E; e++) {
+                            const float v = vec16<T>::at(r, e), b = place(v);
+                            if (b >= from && b < to) {
+                                klo = min(klo, order_key(v));
+                                khi = max(khi, order_key(v));
+                                if (*(volatile int *) &M.n <= S_LIST) push(v, at + e);
+                            }
+                        }
                     }
-                const ull upto = block_scan(v[0] + v[1], M.scan, &total);
-                if (by_mass && shift == 32) {
-                    // what top-k left: of the tokens at its cut only some count
-                    whole = total;
-                    if (R.k < V) whole -= (M.inside - ties) * R.mass(key_value(cut));
-                    limit = R.mass_limit(whole);
+                });
+                klo = __reduce_min_sync(0xFFFFFFFFu, klo);
+                khi = __reduce_max_sync(0xFFFFFFFFu, khi);
+                if (lane == 0) {
+                    atomicMin(&M.key_lo, klo);
+                    atomicMax(&M.key_hi, khi);
                 }
-                const ull x0 = above + upto - v[0] - v[1], x1 = x0 + v[0];
-                if (v[0] && x0 <= limit) atomicMax(&M.best, 2 * tid);
-                if (v[1] && x1 <= limit) atomicMax(&M.best, 2 * tid + 1);
-                __syncthreads();
-                if (M.best >> 1 == tid) {
-                    M.bucket = M.best;
-                    M.above = M.best & 1 ? x1 : x0;
-                    M.inside = M.best & 1 ? v[1] : v[0];
-                    M.total = whole;
+                {
+                    ull m = above_m;
+#pragma unroll
+                    for (int d = 16; d; d >>= 1) m += __shfl_xor_sync(0xFFFFFFFFu, m, d);
+                    if (lane == 0) M.part_mass[warp] = m;
                 }
-            }
-            cluster.sync();
-            const int b = M0.bucket;
-            above = M0.above;
-            const ull inside = M0.inside;
-            whole = M0.total;
-            if (by_mass) limit = R.mass_limit(whole);
-            if (shift == 0) {
-                key_hi -= (uint32_t) b;
-                ull n = limit - above + 1;
-                if (by_mass) n = (limit - above) / R.mass(key_value(key_hi)) + 1;
-                if (key_hi > cut) {
-                    cut = key_hi;
-                    ties = n;
-                } else {
-                    ties = min(ties, n);
+                cluster_sum(all_m, above_m, whole, above);
+                const int n = listed();
+                if (n <= S_LIST) {
+                    if (finish(n, above, from > 0.0f, true)) return;
+                    found = true;
+                    parts_known = R.min_p <= 0.0f;
                 }
-                cluster.sync();                // CTA 0's answers are read
-                if (cta == 0 && tid == 0) M.inside = inside;      // tokens at top-k's cut
-                break;
-            }
-            if (shift < 32) {
-                key_hi -= (uint32_t) b << shift;
-                key_lo = max(key_lo, key_hi - ((1u << shift) - 1));
-            } else {
-                // few tokens down to the bucket, and none cut away before: they go to CTA 0
-                const bool some = cut == 0 && (by_mass || above + inside <= S_LIST);
-                uint32_t lo = 0xFFFFFFFFu, hi = 0;
-                for (int i = 0; i < vecs; i++) {
-                    const uint4 r = mine[i * S_THREADS];
+                if (tid == 0) M.above = above;
+        }
+        if (list) {
+            smem & M0 = peer(0);               // into CTA 0's list
+            bool room = true;
+            each_vec(w_first, w_first + vecs, [&](const uint4 & r, int at) {
+                if (place(vec16<T>::top(r)) < below && room) {    // rarely
 #pragma unroll
                     for (int e = 0; e < E; e++) {
-                        const float v = value(r, e);
-                        const uint32_t key = order_key(v);
-                        if (key < cut || v == -INFINITY) continue;
-                        const int vb = R.bucket(v);
-                        if (vb > b) continue;
-                        if (vb == b) {
-                            lo = min(lo, key);
-                            hi = max(hi, key);
-                        }
-                        if (some && *(volatile int *) &M.n <= S_LIST) {
-                            const int at = atomicAdd(&M.n, 1);
-                            if (at < S_LIST) M.list[at] = (ull) key << 32 | (uint32_t) ~(base + i * 32 * E + e);
+                        const float v = vec16<T>::at(r, e);
+                        if (place(v) < below && room) {
+                            const int i = atomicAdd(&M0.n, 1);
+                            if (i < S_LIST) M0.list[i] = (ull) order_key(v) << 32 | (uint32_t) ~(at + e);
+                            else room = false;
                         }
                     }
                 }
-                lo = __reduce_min_sync(0xFFFFFFFFu, lo);
-                hi = __reduce_max_sync(0xFFFFFFFFu, hi);
-                if (lane == 0) {
-                    atomicMin(&M.key_lo, lo);
-                    atomicMax(&M.key_hi, hi);
-                }
-                cluster.sync();
-                int n = 0;
-                key_lo = 0xFFFFFFFFu;
-                for (int c = 0; c < C; c++) {
-                    const sample_smem & Mc = *cluster.map_shared_rank(&M, c);
-                    n += Mc.n;
-                    key_lo = min(key_lo, Mc.key_lo);
-                    key_hi = max(key_hi, Mc.key_hi);
-                }
-                if (some && n <= S_LIST) {
-                    // ---- the list: sorted, cut, sorted again by index
-                    if (cta != 0) {
-                        cluster.sync();
-                        return;
-                    }
-                    int at = 0, size = 2;
-                    while (size < n) size <<= 1;
-                    for (int c = 0; c < C; c++) {
-                        const sample_smem & Mc = *cluster.map_shared_rank(&M, c);
-                        for (int i = tid; i < Mc.n; i += S_THREADS) M.sorted[at + i] = Mc.list[i];
-                        at += Mc.n;
-                    }
-                    for (int i = n + tid; i < size; i += S_THREADS) M.sorted[i] = 0;
-                    cluster.sync();            // the others may go
-                    block_sort(M.sorted, size);
-                    // four consecutive tokens a thread
-                    float w[4];
-                    ull m[4], sum = 0, total;
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        const int i = 4 * tid + j;
-                        w[j] = i < n ? R.weight(key_value((uint32_t) (M.sorted[i] >> 32))) : 0.0f;
-                        m[j] = i < n && i < R.k && w[j] >= 0x1p-40f ? mass_of(w[j]) : 0ull;
-                        sum += m[j];
-                    }
-                    ull run = block_scan(sum, M.scan, &total) - sum;
-                    if (R.k < V) whole = total;
-                    limit = R.top_p < 1.0f ? R.mass_limit(whole) : ~0ull;
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        const int i = 4 * tid + j;
-                        const bool keep = i < n && i < R.k && run <= limit && w[j] >= R.min_p;
-                        run += m[j];
-                        if (i < size) M.list[i] = keep ? (ull) (uint32_t) M.sorted[i] << 32 | (uint32_t) (M.sorted[i] >> 32) : 0ull;
-                    }
-                    block_sort(M.list, size);  // falling ~index
-                    sum = 0;
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        const int i = 4 * tid + j;
-                        const ull a = i < size ? M.list[i] : 0ull;
-                        w[j] = a ? R.weight(key_value((uint32_t) a)) : 0.0f;
-                        m[j] = a && w[j] >= 0x1p-40f ? mass_of(w[j]) : 0ull;
-                        sum += m[j];
-                    }
-                    run = block_scan(sum, M.scan, &total) - sum;
-                    const ull goal = R.goal(total);
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        if (m[j] && run <= goal && goal < run + m[j]) {
-                            token[row] = (int32_t) ~(uint32_t) (M.list[4 * tid + j] >> 32);
-                            if (prob) prob[row] = R.prob(w[j], total);
-                        }
-                        run += m[j];
-                    }
-                    return;
-                }
-                if (tid == 0) M.n = S_LIST + 1;                    // no second try
+            });
+            csync();
+            const int n = M0.n;
+            if (n <= S_LIST) {
+                finish(n, 0, false, false);
+                return;
             }
-            const uint32_t span = key_hi - key_lo;
-            shift = span < S_BUCKETS ? 0 : 22 - __clz(span);
-            cluster.sync();                    // everyone has read
+        }
+        // ---- radix selection, by count for top-k, by mass for top-p
+        for (int by_mass = 0; by_mass < 2 && !found; by_mass++) {
+            if (by_mass ? !by_p : !by_k) continue;
+            const bool after_k = by_mass && by_k;
+            uint32_t key_lo = 0x00800000u, key_hi = order_key(top);   // above -inf
+            ull above = 0, limit = (ull) (R.k - 1);
+            csync();
+            if (by_mass && !by_k) {
+                for (int c = 0; c < C; c++) {
+                    key_lo = c ? min(key_lo, peer(c).key_lo) : peer(c).key_lo;
+                    key_hi = c ? max(key_hi, peer(c).key_hi) : peer(c).key_hi;
+                }
+                above = M.above;
+            } else if (by_mass) {
+                key_lo = order_key(cut);
+                ull m = 0, none;
+                each([&](float v, int, int) { m += v > cut ? R.mass(v) : 0ull; });
+                cluster_sum(m, 0, whole, none);
+                whole += ties * R.mass(cut);
+            }
+            if (by_mass) limit = R.mass_limit(whole);
+            while (true) {
+                const uint32_t span = key_hi - key_lo;
+                const int shift = span < S_RADIX ? 0 : 22 - __clz(span);
+                csync();                       // the cluster has read the last step's histograms
+                for (int i = tid; i < 4 * S_RADIX; i += THREADS) M.hist[i] = 0;
+                if (tid == 0) M.best = -1;
+                __syncthreads();
+                each([&](float v, int, int) {
+                    if (!(v > -INFINITY)) return;
+                    const uint32_t key = order_key(v);
+                    if (key < key_lo || key > key_hi) return;
+                    const int b = (int) ((key_hi - key) >> shift);
+                    const ull m = by_mass ? R.mass(v) : 1ull;
+                    if (m == 0) return;
+                    atomicAdd(&M.hist[b], (uint32_t) m & 0x7FFu);
+                    if (by_mass) {
+                        atomicAdd(&M.hist[S_RADIX + b], (uint32_t) (m >> 11) & 0x7FFu);
+                        atomicAdd(&M.hist[2 * S_RADIX + b], (uint32_t) (m >> 22) & 0x7FFu);
+                        atomicAdd(&M.hist[3 * S_RADIX + b], (uint32_t) (m >> 33));
+                    }
+                });
+                csync();
+                constexpr int PR = S_RADIX / THREADS;
+                ull v[PR] = {}, sum = 0, t;
+#pragma unroll
+                for (int j = 0; j < PR; j++) {
+                    for (int c = 0; c < C; c++) {
+                        const uint32_t * h = peer(c).hist + PR * tid + j;
+                        v[j] += (ull) h[0] + ((ull) h[S_RADIX] << 11) + ((ull) h[2 * S_RADIX] << 22) + ((ull) h[3 * S_RADIX] << 33);
+                    }
+                    sum += v[j];
+                }
+                ull run = above + block_scan<WARPS>(sum, M.scan, t) - sum, at[PR];
+#pragma unroll
+                for (int j = 0; j < PR; j++) {
+                    at[j] = run;
+                    if (v[j] && run <= limit) atomicMax(&M.best, PR * tid + j);
+                    run += v[j];
+                }
+                __syncthreads();
+                const int best = M.best;
+#pragma unroll
+                for (int j = 0; j < PR; j++)
+                    if (PR * tid + j == best) M.above = at[j];
+                __syncthreads();
+                above = M.above;
+                key_hi -= (uint32_t) best << shift;
+                if (shift == 0) break;
+                key_lo = max(key_lo, key_hi - ((1u << shift) - 1));
+            }
+            const float at = key_value(key_hi);
+            const ull n = by_mass ? (limit - above) / R.mass(at) + 1 : limit - above + 1;
+            ties = after_k && at == cut ? min(ties, n) : n;
+            cut = at;
         }
     }
 
-    // ---- the warps' masses, in order of index
-    {
-        ull m = 0;
-        uint32_t eq = 0;
-        for (int i = 0; i < vecs; i++) {
-            const uint4 r = mine[i * S_THREADS];
+    // ---- the warps' masses, in order of index; then the token's warp is cut into WARPS parts, and the part's vectors
+    const float w_cut = cut > -INFINITY ? (cut == top ? 1.0f : R.weight(cut)) : 0.0f;
+    const ull m_cut = w_cut >= R.min_p ? mass_of(w_cut) : 0ull;
+    auto vec_mass = [&](const uint4 & r, int & eq) {
+        uint32_t hi = 0, lo = 0;
+        if (ties) {
 #pragma unroll
-            for (int e = 0; e < E; e++) {
-                const float v = value(r, e);
-                const uint32_t key = order_key(v);
-                eq += key == cut;
-                if (key > cut) {
-                    const float w = R.weight(v);
-                    if (w >= R.min_p && w >= 0x1p-40f) m += mass_of(w);
-                }
-            }
+            for (int e = 0; e < E; e++) eq += vec16<T>::at(r, e) == cut;
         }
+#pragma unroll
+        for (int e = 0; e < E; e += 2) {
+            const float v[2] = { vec16<T>::at(r, e), vec16<T>::at(r, e + 1) };
+            float2 w = R.weight2(R.distance2(v[0], v[1]));
+            w.x = v[0] > cut && w.x >= R.min_p ? w.x : 0.0f;
+            w.y = v[1] > cut && w.y >= R.min_p ? w.y : 0.0f;
+            uint32_t h[2], l[2];
+            mass_parts2(w, h, l);
+            hi += h[0] + h[1];
+            lo += l[0] + l[1];
+        }
+        return mass_sum(hi, lo, E);
+    };
+    int w0 = w_first, w1 = w0 + vecs;          // this warp's part of the row's vectors
+    ull goal = 0, left = ties, total = 0;
+    for (int level = 0; level < 2; level++) {
+        ull m = 0;
+        int eq = 0;
+        const bool known = level == 0 && parts_known;
+        if (!known) each_vec(w0, w1, [&](const uint4 & r, int) { m += vec_mass(r, eq); });
 #pragma unroll
         for (int d = 16; d; d >>= 1) m += __shfl_xor_sync(0xFFFFFFFFu, m, d);
         eq = __reduce_add_sync(0xFFFFFFFFu, eq);
-        if (lane == 0) {
-            M.warp_mass[warp] = m;
-            M.warp_ties[warp] = eq;
+        __syncthreads();
+        if (lane == 0 && !known) {
+            M.part_mass[warp] = m;
+            M.part_ties[warp] = eq;
         }
-    }
-    const float w_cut = cut ? R.weight(key_value(cut)) : 0.0f;
-    const ull m_cut = cut && w_cut >= R.min_p && w_cut >= 0x1p-40f ? mass_of(w_cut) : 0ull;
-    cluster.sync();
-    if (cta == 0) {
-        ull eq = 0, m = 0, total;
-        if (tid < C * S_WARPS) {
-            const sample_smem & Mc = *cluster.map_shared_rank(&M, tid / S_WARPS);
-            m = Mc.warp_mass[tid % S_WARPS];
-            eq = Mc.warp_ties[tid % S_WARPS];
-        }
-        const ull eq_before = block_scan(eq, M.scan, &total) - eq;
-        const ull left = eq_before < ties ? ties - eq_before : 0;
-        const ull mine = m + min(left, eq) * m_cut;
-        const ull before = block_scan(mine, M.scan, &total) - mine;
-        const ull goal = R.goal(total);
-        if (goal >= before && goal < before + mine) {
-            M.cta = tid / S_WARPS;
-            M.warp = tid % S_WARPS;
-            M.goal = goal - before;
-            M.ties = left;
-            M.total = total;
-        }
-    }
-    cluster.sync();
-    if (M0.cta == cta && M0.warp == warp) {
-        // 32 lanes' elements of a vector at a time
-        ull goal = M0.goal, left = M0.ties;
-        const ull total = M0.total;
-        bool found = false;
-        for (int i = 0; i < vecs && !found; i++) {
-            const uint4 r = mine[i * S_THREADS];
-            uint32_t eq = 0;
-#pragma unroll
-            for (int e = 0; e < E; e++) eq += order_key(value(r, e)) == cut;
-            uint32_t eq_upto = eq;
-#pragma unroll
-            for (int d = 1; d < 32; d <<= 1) {
-                const uint32_t o = __shfl_up_sync(0xFFFFFFFFu, eq_upto, d);
-                if (lane >= d) eq_upto += o;
-            }
-            const ull lane_left = left > eq_upto - eq ? left - (eq_upto - eq) : 0;
-            auto part = [&](int e, ull & room) {
-                const float v = value(r, e);
-                const uint32_t key = order_key(v);
-                if (key > cut) {
-                    const float w = R.weight(v);
-                    return w >= R.min_p && w >= 0x1p-40f ? mass_of(w) : 0ull;
-                }
-                if (key == cut && room) {
-                    room--;
-                    return m_cut;
-                }
-                return 0ull;
-            };
-            ull sum = 0, room = lane_left;
-#pragma unroll
-            for (int e = 0; e < E; e++) sum += part(e, room);
-            ull upto = sum;
-#pragma unroll
-            for (int d = 1; d < 32; d <<= 1) {
-                const ull o = __shfl_up_sync(0xFFFFFFFFu, upto, d);
-                if (lane >= d) upto += o;
-            }
-            const ull all = __shfl_sync(0xFFFFFFFFu, upto, 31);
-            if (goal < all) {
-                found = true;
-                ull run = upto - sum;
-                room = lane_left;
-                if (goal >= run && goal < upto) {
-#pragma unroll
-                    for (int e = 0; e < E; e++) {
-                        const ull m = part(e, room);
-                        if (m && goal >= run && goal < run + m) {
-                            token[row] = base + i * 32 * E + e;
-                            if (prob) prob[row] = R.prob(R.weight(value(r, e)), total);
-                        }
-                        run += m;
-                    }
-                }
-            }
-            goal -= min(goal, all);
-            const uint32_t eqs = __shfl_sync(0xFFFFFFFFu, eq_upto, 31);
-            left = left > eqs ? left - eqs : 0;
-        }
-    }
-    cluster.sync();                            // CTA 0's answers are read
-}
-
-// Rows that the shared memory of a cluster does not hold: one CTA a row reads the
-// logits again for each step, radix selection eight bits of the key at a time.
-template <class T>
-__global__ void __launch_bounds__(S_THREADS)
-k_sample_long(const T * __restrict__ logits, int64_t ld, int V, const float * __restrict__ temperature,
-         const int32_t * __restrict__ top_k, const float * __restrict__ top_p, const float * __restrict__ min_p,
-         const float * __restrict__ u, int32_t * __restrict__ token, float * __restrict__ prob) {
-    __shared__ ull s_mass[256];
-    __shared__ float s_f[S_WARPS];
-    __shared__ ull s_w[S_WARPS];
-    __shared__ int s_i[S_WARPS];
-    __shared__ uint32_t s_key;
-    __shared__ ull s_above;
-    pdl_entry();
-    const int64_t row = blockIdx.x;
-    const T * x = logits + row * ld;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    sample_row p;
-    p.read(row, V, temperature, top_k, top_p, min_p, u);
-    auto value = [&](int i) {
-        const float v = num<T>::to(x[i]);
-        return v != v ? -INFINITY : v + 0.0f;
-    };
-    // the maximum
-    float top = -INFINITY;
-    for (int i = tid; i < V; i += S_THREADS) top = fmaxf(top, value(i));
-#pragma unroll
-    for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
-    if (lane == 0) s_f[warp] = top;
-    __syncthreads();
-    for (int w = 0; w < S_WARPS; w++) top = fmaxf(top, s_f[w]);
-    if (top == -INFINITY) {
-        if (tid == 0) {
-            token[row] = -1;
-            if (prob) prob[row] = 0.0f;
-        }
-        return;
-    }
-    p.top = top;
-    auto weight = [&](float v) { return p.weight(v); };
-    uint32_t cut = 0;                         // kept: key > cut, and the first `ties` of key == cut
-    ull ties = (ull) V;
-    if (p.greedy) {
-        cut = order_key(top);
-        ties = 1;
-    } else {
-        // selection by count, then by mass: the largest key at which what lies above is < need
-        ull whole = 0;
-        for (int by_mass = 0; by_mass < 2; by_mass++) {
-            if (by_mass == 0 ? p.k >= V : !(p.top_p < 1.0f)) continue;
-            if (by_mass) {                                        // the mass of what top-k left
-                ull m = 0;
-                for (int i = tid; i < V; i += S_THREADS) {
-                    const float v = value(i);
-                    if (order_key(v) > cut) m += p.mass(v);
-                }
-#pragma unroll
-                for (int d = 16; d; d >>= 1) m += __shfl_xor_sync(0xFFFFFFFFu, m, d);
-                __syncthreads();
-                if (lane == 0) s_w[warp] = m;
-                __syncthreads();
-                whole = 0;
-                for (int w = 0; w < S_WARPS; w++) whole += s_w[w];
-                if (p.k < V) {
-                    const float vc = key_value(cut);
-                    whole += ties * p.mass(vc);
-                }
-            }
-            uint32_t prefix = 0, mask = 0;
-            // what lies above must be <= limit (count: k - 1; mass: below top_p * whole)
-            ull limit = (ull) (p.k - 1);
-            if (by_mass) {
-                limit = p.mass_limit(whole);
-            }
-            ull above = 0;
-            for (int shift = 24; shift >= 0; shift -= 8) {
-                __syncthreads();
-                for (int i = tid; i < 256; i += S_THREADS) s_mass[i] = 0;
-                __syncthreads();
-                for (int i = tid; i < V; i += S_THREADS) {
-                    const float v = value(i);
-                    const uint32_t k = order_key(v);
-                    if ((k & mask) == prefix && k >= cut) {
-                        const ull a = by_mass ? p.mass(v) : 1ull;
-                        if (a) atomicAdd(&s_mass[(k >> shift) & 255], a);
-                    }
-                }
-                __syncthreads();
-                if (tid == 0) {
-                    // the lowest bucket that what lies above it still allows
-                    int b = 255;
-                    ull run = above, at = above;
-                    int best = -1;
-                    for (; b >= 0; b--) {
-                        if (s_mass[b]) {
-                            if (run > limit) break;
-                            best = b;
-                            at = run;
-                        }
-                        run += s_mass[b];
-                    }
-                    s_key = prefix | ((uint32_t) best << shift);
-                    s_above = at;
-                }
-                __syncthreads();
-                prefix = s_key;
-                above = s_above;
-                mask |= 255u << shift;
-            }
-            ull n = limit - above + 1;                            // by count
-            if (by_mass) {
-                const float vc = key_value(prefix);
-                const ull w = p.mass(vc);
-                n = (limit - above) / w + 1;
-            }
-            if (prefix > cut) {
-                cut = prefix;
-                ties = n;
-            } else {
-                ties = min(ties, n);
+        if (level == 0) csync(); else __syncthreads();
+        // part i of the row: warp i % WARPS of CTA i / WARPS, and then of the token's CTA only
+        const int parts = level == 0 ? C * WARPS : WARPS;
+        ull pm = 0, pe = 0, t;
+        if (tid < parts) {
+            const smem & Mc = level == 0 ? peer(tid / WARPS) : M;
+            pm = Mc.part_mass[tid % WARPS];
+            pe = Mc.part_ties[tid % WARPS];
+            if (known) {
+                const smem & M0 = peer(0);
+                pm += M0.list_mass[0][tid] + ((ull) M0.list_mass[1][tid] << 14) + ((ull) M0.list_mass[2][tid] << 28);
+                pe = M0.list_ties[tid];
             }
         }
-    }
-    // in order of index: warp w takes a contiguous part of the row
-    const int part = (V + S_WARPS - 1) / S_WARPS;
-    const int i0 = min(warp * part, V), i1 = min(i0 + part, V);
-    int eq = 0;
-    for (int i = i0 + lane; i < i1; i += 32) eq += order_key(value(i)) == cut;
-#pragma unroll
-    for (int d = 16; d; d >>= 1) eq += __shfl_xor_sync(0xFFFFFFFFu, eq, d);
-    if (lane == 0) s_i[warp] = eq;
-    __syncthreads();
-    ull before = 0;
-    for (int w = 0; w < warp; w++) before += s_i[w];
-    auto kept = [&](int i, bool in, ull & rank, float & w) {       // all lanes; rank: ties before this step
-        float v = -INFINITY;
-        uint32_t k = 0;
-        if (in) {
-            v = value(i);
-            k = order_key(v);
+        const ull ties_before = block_scan<WARPS>(pe, M.scan, t) - pe;
+        const ull room = left > ties_before ? left - ties_before : 0;
+        const ull mine = pm + min(room, pe) * m_cut;
+        const ull run = block_scan<WARPS>(mine, M.scan, t);
+        if (level == 0) {
+            total = t;
+            goal = R.goal(total);
         }
-        const uint32_t tie = __ballot_sync(0xFFFFFFFFu, in && k == cut);
-        const bool keep = in && (k > cut || (k == cut && rank + __popc(tie & ((1u << lane) - 1)) < ties));
-        rank += __popc(tie);
-        w = keep ? weight(v) : 0.0f;
-        return keep && (p.greedy || w >= p.min_p) ? (p.greedy ? 1ull : w >= 0x1p-40f ? mass_of(w) : 0ull) : 0ull;
-    };
-    ull sum = 0, rank = before;
-    for (int i = i0; i < i1; i += 32) {
-        float w;
-        sum += kept(i + lane, i + lane < i1, rank, w);
+        if (goal >= run - mine && goal < run) {
+            M.at = tid;
+            M.goal = goal - (run - mine);
+            M.ties = room;
+        }
+        if (level == 0) csync(); else __syncthreads();
+        const int at = M.at;
+        goal = M.goal;
+        left = M.ties;
+        if (level == 0) {
+            if (at / WARPS != cta) return;     // the cluster has read what it needs
+            w0 = at * vecs + (int) ((int64_t) warp * vecs / WARPS);
+            w1 = at * vecs + (int) ((int64_t) (warp + 1) * vecs / WARPS);
+        }
     }
-#pragma unroll
-    for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
-    __syncthreads();
-    if (lane == 0) s_w[warp] = sum;
-    __syncthreads();
-    ull total = 0, base = 0;
-    for (int w = 0; w < S_WARPS; w++) {
-        if (w < warp) base += s_w[w];
-        total += s_w[w];
-    }
-    const ull goal = p.goal(total);
-    if (goal < base || goal >= base + sum) return;
-    // the warp that holds the token
-    rank = before;
-    for (int i = i0; i < i1; i += 32) {
-        float w;
-        ull a = kept(i + lane, i + lane < i1, rank, w), run = a;
+    if (warp != M.at) return;
+    for (int i = w0; i < w1; i++) {
+        const int at = origin + i * 32 * E;
+        const uint4 r = fetch(i);
+        int eq = 0;
+        const ull gt = vec_mass(r, eq);
+        int eq_upto = eq;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
-            const ull o = __shfl_up_sync(0xFFFFFFFFu, run, d);
-            if (lane >= d) run += o;
+            const int o = __shfl_up_sync(0xFFFFFFFFu, eq_upto, d);
+            if (lane >= d) eq_upto += o;
         }
-        const bool hit = a && goal >= base + run - a && goal < base + run;
-        if (hit) {
-            token[row] = i + lane;
-            if (prob) prob[row] = p.greedy ? 1.0f : p.prob(w, total);
+        ull room = left > (ull) (eq_upto - eq) ? left - (eq_upto - eq) : 0;
+        const ull sum = gt + min(room, (ull) eq) * m_cut;
+        ull upto = sum;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const ull o = __shfl_up_sync(0xFFFFFFFFu, upto, d);
+            if (lane >= d) upto += o;
         }
-        if (__any_sync(0xFFFFFFFFu, hit)) return;
-        base += __shfl_sync(0xFFFFFFFFu, run, 31);
+        if (goal >= upto - sum && goal < upto) {
+            ull run = upto - sum;
+#pragma unroll
+            for (int e = 0; e < E; e++) {
+                const float v = vec16<T>::at(r, e), w = v == cut ? w_cut : R.weight(v);
+                ull m = 0;
+                if (v > cut) {
+                    m = w >= R.min_p ? mass_of(w) : 0ull;
+                } else if (v == cut && room) {
+                    room--;
+                    m = m_cut;
+                }
+                if (m && goal >= run && goal < run + m) {
+                    token[row] = at + e;
+                    if (prob) prob[row] = R.prob(w, total);
+                }
+                run += m;
+            }
+        }
+        const ull all = __shfl_sync(0xFFFFFFFFu, upto, 31);
+        if (goal < all) return;
+        goal -= all;
+        const int eqs = __shfl_sync(0xFFFFFFFFu, eq_upto, 31);
+        left = left > (ull) eqs ? left - eqs : 0;
     }
 }
 
@@ -2019,7 +2343,7 @@ int launch_append(const lnsb_paged_append_args & a, cudaStream_t s) {
     return launch_status();
 }
 
-constexpr int k_max_devices = 64;
+constexpr int k_max_devices = 64, k_smem_most = 227 * 1024;
 
 // dynamic shared memory of a kernel, once per device
 template <class K>
@@ -2035,29 +2359,16 @@ int allow_smem(K kern, bool (&done)[k_max_devices], int bytes) {
     return 0;
 }
 
-template <class T>
-int launch_sample(const lnsb_sample_args & a, cudaStream_t s) {
-    const T * x = static_cast<const T *>(a.logits);
-    const int V = (int) a.n_vocab, E = vec16<T>::N, need = V + E - 1;      // a row may start inside a vector
-    const int line = S_THREADS * E;                                       // one vector of each thread
-    int C = 1;
-    while (C < 8 && need > C * line * S_VECS / 2) C *= 2;                 // two CTAs to an SM where the row allows it
-    if (need > C * line * S_VECS) {
-        launch_k(k_sample_long<T>, dim3((unsigned) a.n_rows), dim3(S_THREADS), 0, s, x, a.ld, V, a.temperature, a.top_k, a.top_p,
-                 a.min_p, a.u, a.token, a.prob);
-        return launch_status();
-    }
-    // few rows: more CTAs to each, while they have an SM of their own and a vector to read
-    while (C < 8 && a.n_rows * C * 2 <= k_sms && need > C * line) C *= 2;
-    auto kern = k_sample<T>;
+template <class T, int THREADS, bool HELD>
+int launch_sample(const lnsb_sample_args & a, int C, int vecs, cudaStream_t s) {
+    auto kern = k_sample<T, THREADS, HELD>;
     static bool attr[k_max_devices] = {};
-    const int st = allow_smem(kern, attr, (int) sizeof(sample_smem) + S_VECS * S_THREADS * 16);
+    const int st = allow_smem(kern, attr, HELD ? k_smem_most : (int) sizeof(sample_smem));
     if (st != 0) return st;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned) (a.n_rows * C));
-    cfg.blockDim = dim3(S_THREADS);
-    const int vecs = (need + C * line - 1) / (C * line);
-    cfg.dynamicSmemBytes = sizeof(sample_smem) + (size_t) vecs * S_THREADS * 16;
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = sizeof(sample_smem) + (HELD ? (size_t) vecs * THREADS * 16 : 0);
     cfg.stream = s;
     cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -2065,10 +2376,26 @@ int launch_sample(const lnsb_sample_args & a, cudaStream_t s) {
     at[1].id = cudaLaunchAttributeClusterDimension;
     at[1].val.clusterDim = { (unsigned) C, 1, 1 };
     cfg.attrs = at;
-    cfg.numAttrs = 2;
-    (void) cudaLaunchKernelEx(&cfg, kern, x, a.ld, V, vecs, a.temperature, a.top_k, a.top_p, a.min_p, a.u, a.token,
-                              a.prob);   // an error stays in cudaGetLastError
+    cfg.numAttrs = HELD ? 2 : 1;
+    (void) cudaLaunchKernelEx(&cfg, kern, static_cast<const T *>(a.logits), a.ld, (int) a.n_vocab, vecs, C, a.temperature, a.top_k,
+                              a.top_p, a.min_p, a.u, a.token, a.prob);    // an error stays in cudaGetLastError
     return launch_status();
+}
+template <class T>
+int launch_sample_rows(const lnsb_sample_args & a, cudaStream_t s) {
+    constexpr int E = vec16<T>::N;
+    const int need = (int) a.n_vocab + E - 1;                            // a row may start inside a vector
+    auto vecs = [&](int threads, int C) { return (need + C * threads * E - 1) / (C * threads * E); };
+    // few rows: as many CTAs to each as leave every one an SM of its own and its threads a vector each
+    constexpr int threads = 512;
+    int C = k_row_ctas;
+    while (C > 1 && (a.n_rows * C > k_sms || need <= C / 2 * threads * E)) C /= 2;
+    const int held = vecs(threads, C);
+    if (a.n_rows <= k_sms && held * threads * E < 65536 && (int) sizeof(sample_smem) + held * threads * 16 <= k_smem_most)
+        return launch_sample<T, threads, true>(a, C, held, s);
+    // the row stays in memory: one to an SM, else two
+    if (a.n_rows <= k_sms) return launch_sample<T, 1024, false>(a, 1, vecs(1024, 1), s);
+    return launch_sample<T, 512, false>(a, 1, vecs(512, 1), s);
 }
 
 constexpr float k_log2e = 1.44269504088896340736f;
@@ -2218,10 +2545,10 @@ int lnsb_sample(const lnsb_sample_args * a, lnsb_stream_t stream) {
     if (a->type != LNSB_TYPE_F32 && a->type != LNSB_TYPE_F16 && a->type != LNSB_TYPE_BF16) return LNSB_E_INVALID;
     if (a->n_rows == 0) return 0;
     if (a->logits == nullptr || a->u == nullptr || a->token == nullptr) return LNSB_E_INVALID;
-    if (a->n_vocab > (1 << 20) || a->n_rows > (1 << 27)) return LNSB_E_TOO_LARGE;
+    if (a->n_vocab > (1 << 20) || a->n_rows > 0x7FFFFFFF) return LNSB_E_TOO_LARGE;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (a->type == LNSB_TYPE_F32) return launch_sample<float>(*a, s);
-    return a->type == LNSB_TYPE_F16 ? launch_sample<__half>(*a, s) : launch_sample<__nv_bfloat16>(*a, s);
+    if (a->type == LNSB_TYPE_F32) return launch_sample_rows<float>(*a, s);
+    return a->type == LNSB_TYPE_F16 ? launch_sample_rows<__half>(*a, s) : launch_sample_rows<__nv_bfloat16>(*a, s);
 }
 
 }  // extern "C"

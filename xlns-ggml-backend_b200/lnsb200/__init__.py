@@ -339,14 +339,18 @@ _f32 = _i32 = _current_stream = None
 def _load_types():
     global _f32, _i32, _current_stream
     import torch
-    _current_stream = torch.cuda.current_stream
+    try:                                # the same handle without a Stream object: 0.2 us, not 3
+        raw, device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
+        _current_stream = lambda: raw(device())  # noqa: E731
+    except AttributeError:
+        _current_stream = lambda: torch.cuda.current_stream().cuda_stream  # noqa: E731
     _f32, _i32 = torch.float32, torch.int32
     _type_ids.update({_f32: _lib.TYPES["f32"], torch.float16: _lib.TYPES["f16"], torch.bfloat16: _lib.TYPES["bf16"]})
 
 
 def _raw_stream(stream):
     """the given or the current stream's cudaStream_t"""
-    return (stream if stream is not None else _current_stream()).cuda_stream
+    return stream.cuda_stream if stream is not None else _current_stream()
 
 
 def _rows_ok(st, heads, D):
