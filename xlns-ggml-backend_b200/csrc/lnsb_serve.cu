@@ -50,6 +50,32 @@ template <> struct num<__nv_bfloat16> {
     static constexpr uint32_t one2 = 0x3F803F80u;
 };
 
+// two floats in one instruction
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 c;
+    asm("{\n.reg .b64 x, y, z;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\nadd.rn.f32x2 z, x, y;\nmov.b64 {%0, %1}, z;\n}\n"
+        : "=f"(c.x), "=f"(c.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return c;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 c;
+    asm("{\n.reg .b64 x, y, z;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\nmul.rn.f32x2 z, x, y;\nmov.b64 {%0, %1}, z;\n}\n"
+        : "=f"(c.x), "=f"(c.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return c;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n.reg .b64 x, y, z, w;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\nmov.b64 z, {%6, %7};\n"
+        "fma.rn.f32x2 w, x, y, z;\nmov.b64 {%0, %1}, w;\n}\n"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
 // ============================ the plan =====================================
 
 // the device's view of lnsb_paged_kv
@@ -824,7 +850,7 @@ template <int D> __host__ __device__ constexpr int b_ring() { return D == 128 ? 
 struct tile_control {                // behind the tiles
     int64_t   sums[B_SUMS];
     tile_item item[B_ITEMS];
-    uint64_t  bar[2 * 10 + 2 * B_ITEMS + 9];
+    uint64_t  bar[2 * 10 + 2 * B_ITEMS + 11];
     uint32_t  tmem;
     int       stop;
 };
@@ -851,7 +877,7 @@ k_paged_attn_tiles(const __grid_constant__ CUtensorMap kmap, const __grid_consta
     const uint32_t q_sm = smem_addr(tile_sm), ring = q_sm + 2 * TB;
     const uint32_t bars = smem_addr(C.bar);
     const uint32_t kv_full = bars, kv_empty = bars + 8 * ST, q_full = kv_empty + 8 * ST, s_full = q_full + 16,
-                   p_ready = s_full + 16, o_full = p_ready + 16, it_full = o_full + 16, it_empty = it_full + 8 * B_ITEMS, drained = it_empty + 8 * B_ITEMS;
+                   p_ready = s_full + 16, o_full = p_ready + 32, it_full = o_full + 16, it_empty = it_full + 8 * B_ITEMS, drained = it_empty + 8 * B_ITEMS;
     volatile int * stop = &C.stop;
 
     if (tid == 0) {
@@ -862,7 +888,8 @@ k_paged_attn_tiles(const __grid_constant__ CUtensorMap kmap, const __grid_consta
         for (int g = 0; g < 2; g++) {
             bar_init(q_full + 8 * g, B_ROWS);
             bar_init(s_full + 8 * g, 1);
-            bar_init(p_ready + 8 * g, B_ROWS);
+            bar_init(p_ready + 16 * g, B_ROWS);
+            bar_init(p_ready + 16 * g + 8, B_ROWS);
             bar_init(o_full + 8 * g, 1);
         }
         for (int i = 0; i < B_ITEMS; i++) {
@@ -1017,12 +1044,17 @@ k_paged_attn_tiles(const __grid_constant__ CUtensorMap kmap, const __grid_consta
                         const uint32_t vb = ring + (v % ST) * TB;
                         ok = bar_wait(kv_full + 8 * (v % ST), (v / ST) & 1, stop);
                         for (int g = 0; ok && g < groups; g++) {
-                            if (!(ok = bar_wait(p_ready + 8 * g, np[g]++ & 1, stop))) break;
-                            tc_after();
 #pragma unroll
-                            for (int kk = 0; kk < B_KEYS / 16; kk++)
-                                mma_ts(tmem + O_COL + D * g, tmem + S_COL + 128 * g + 8 * kk,
-                                       smem_desc(vb + kk * 2048, HB, 1024), idesc_pv, j > 0 || kk > 0);
+                            for (int half = 0; half < 2; half++) {
+                                if (!(ok = ok && bar_wait(p_ready + 16 * g + 8 * half, np[g] & 1, stop))) break;
+                                tc_after();
+#pragma unroll
+                                for (int kk = 4 * half; kk < 4 * half + 4; kk++)
+                                    mma_ts(tmem + O_COL + D * g, tmem + S_COL + 128 * g + 8 * kk,
+                                           smem_desc(vb + kk * 2048, HB, 1024), idesc_pv, j > 0 || kk > 0);
+                            }
+                            if (!ok) break;
+                            np[g]++;
                             if (j + 1 < nt) {
                                 if (g == 0 && !(ok = bar_wait(kv_full + 8 * (k % ST), (k / ST) & 1, stop))) break;
                                 qk(g, k);
@@ -1054,18 +1086,31 @@ k_paged_attn_tiles(const __grid_constant__ CUtensorMap kmap, const __grid_consta
             const uint32_t s_at = tmem + lanes + S_COL + 128 * g, o_at = tmem + lanes + O_COL + D * g;
             uint32_t ns = 0, no = 0;                                 // phases of s_full and o_full
             uint32_t n = 0;
+            const int win = (int) min(L.window, (int64_t) 0x7FFFFFFF);
             bool ok = true;
-            while (ok && next_item()) {
-                const uint32_t nt = (uint32_t) I.n, ring0 = n;
+            for (; ok; items++) {
+                // the item stays in shared memory: the loop over the keys needs its registers for the scores
+                const uint32_t slot_i = items % B_ITEMS;
+                if (!(ok = bar_wait_warp(it_full + 8 * slot_i, (items / B_ITEMS) & 1, stop))) break;
+                const volatile tile_item & X = C.item[slot_i];
+                const uint32_t nt = (uint32_t) X.n, ring0 = n;
+                if (nt == 0) break;
                 n += 2 * nt;
-                const int r = I.r0 + B_ROWS * g + row;
-                if (I.r0 + B_ROWS * g >= I.rows) continue;           // no rows for this group
-                const bool live = r < I.rows;
-                const int64_t tok = I.first + r / L.G;
-                const int head = I.head * L.G + r % L.G;
+                auto release = [&] {
+                    __syncwarp();
+                    if (lane == 0) bar_arrive(it_empty + 8 * slot_i);
+                };
+                if (X.r0 + B_ROWS * g >= X.rows) {                   // no rows for this group
+                    release();
+                    continue;
+                }
+                auto my_row = [&] { return X.r0 + B_ROWS * g + row; };
                 {
-                    const uint4 * src = reinterpret_cast<const uint4 *>(q + tok * q_ld + (int64_t) head * D);
+                    const int r = my_row();
+                    const uint4 * src = reinterpret_cast<const uint4 *>(q + (int64_t) (X.first + r / L.G) * q_ld +
+                                                                        (int64_t) (X.head * L.G + r % L.G) * D);
                     const uint32_t qb = q_sm + g * TB + row * 128;
+                    const bool live = r < X.rows;
                     uint4 v[D / 8];
 #pragma unroll
                     for (int i = 0; i < D / 8; i++) v[i] = live ? __ldg(src + i) : make_uint4(0, 0, 0, 0);
@@ -1077,31 +1122,46 @@ k_paged_attn_tiles(const __grid_constant__ CUtensorMap kmap, const __grid_consta
                     asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
                     bar_arrive(q_full + 8 * g);
                 }
-                // the tile's first and last row, and this thread's
-                const int pos_a = I.pos0 + (I.r0 + B_ROWS * g) / L.G;
-                const int pos_z = I.pos0 + (min(I.r0 + B_ROWS * g + B_ROWS, I.rows) - 1) / L.G;
-                const int pos = I.pos0 + r / L.G;
-                const int seen = first_owned(I, L);
+                // a tile needs a look at its edges where its last key is past the first row's, or its first key before
+                // the last row's window; rows of V that the sequence does not own lie only in such tiles
+                const int first_pos = X.pos0 + (X.r0 + B_ROWS * g) / L.G - X.key0;
+                const int last_win = win ? X.pos0 + (min(X.r0 + B_ROWS * g + B_ROWS, X.rows) - 1) / L.G - win - X.key0 : -1;
                 float m = k_none, l = 0.0f;
                 for (uint32_t j = 0; j < nt; j++) {
-                    const int k0 = I.key0 + (int) j * B_KEYS;
                     if (!(ok = bar_wait_warp(s_full + 8 * g, ns++ & 1, stop))) break;
                     tc_after();
                     uint32_t sv[128];
 #pragma unroll
                     for (int i = 0; i < 4; i++) tc_ld32(s_at + 32 * i, sv + 32 * i);
                     tc_wait_ld(sv);
-                    if (k0 + B_KEYS - 1 > pos_a || (L.window > 0 && k0 <= pos_z - L.window)) {
-                        const int hi = pos - k0;                     // columns lo .. hi
-                        const int lo = L.window > 0 ? (int) max(pos - L.window + 1 - k0, (int64_t) 0) : 0;
+                    if ((int) j * B_KEYS + B_KEYS - 1 > first_pos || (int) j * B_KEYS <= last_win) {
+                        const int k0 = X.key0 + (int) j * B_KEYS, pos = X.pos0 + my_row() / L.G;
+                        const int seen = win ? max(0, X.pos0 - win + 1) : 0, kv = X.kv;
+                        const int hi = pos - k0, lo = win ? pos - win + 1 - k0 : 0;     // columns lo .. hi
 #pragma unroll
                         for (int i = 0; i < 128; i++)
                             if (i > hi || i < lo) sv[i] = 0xFF800000u;
-                    }
-                    float top = __uint_as_float(sv[0]);
+                        // those rows of V may hold anything: weight 0 must meet 0
+                        if (k0 + B_KEYS > kv || k0 < seen) {
+                            const uint32_t i = ring0 + 2 * j + 1;
+                            if (!(ok = bar_wait_warp(kv_full + 8 * (i % ST), (i / ST) & 1, stop))) break;
+                            if (k0 + row >= kv || k0 + row < seen) {
+                                const uint32_t vb = ring + (i % ST) * TB + row * 128;
 #pragma unroll
-                    for (int i = 1; i < 128; i++) top = fmaxf(top, __uint_as_float(sv[i]));
-                    top *= scale_log2;
+                                for (int c = 0; c < D / 8; c++)
+                                    asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};\n"
+                                                 :: "r"(vb + (c / 8) * HB + (c % 8) * 16), "r"(0) : "memory");
+                            }
+                            asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+                        }
+                    }
+                    float t4[4] = { -INFINITY, -INFINITY, -INFINITY, -INFINITY };
+#pragma unroll
+                    for (int i = 0; i < 128; i += 8)
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            t4[e] = max3(t4[e], __uint_as_float(sv[i + 2 * e]), __uint_as_float(sv[i + 2 * e + 1]));
+                    const float top = fmaxf(max3(t4[0], t4[1], t4[2]), t4[3]) * scale_log2;
                     if (__any_sync(0xFFFFFFFFu, top > m + k_lag)) {
                         const float mn = fmaxf(m, top), f = ex2(m - mn);
                         m = mn;
@@ -1118,40 +1178,33 @@ k_paged_attn_tiles(const __grid_constant__ CUtensorMap kmap, const __grid_consta
                             }
                         }
                     }
-                    float add[4] = { 0, 0, 0, 0 };
+                    // PV of the first 64 keys starts while the others' weights are computed
+                    float2 add[2] = { { 0, 0 }, { 0, 0 } };
+                    const float2 sc2 = make_float2(scale_log2, scale_log2), m2 = make_float2(-m, -m);
 #pragma unroll
                     for (int i = 0; i < 2; i++) {
                         uint32_t pv[32];
 #pragma unroll
                         for (int e = 0; e < 32; e++) {
-                            const float a = ex2(fmaf(__uint_as_float(sv[64 * i + 2 * e]), scale_log2, -m));
-                            const float b = ex2(fmaf(__uint_as_float(sv[64 * i + 2 * e + 1]), scale_log2, -m));
-                            add[2 * (e & 1)] += a;
-                            add[2 * (e & 1) + 1] += b;
-                            pv[e] = num<T>::pack(a, b);
+                            const float2 x = fma2(make_float2(__uint_as_float(sv[64 * i + 2 * e]), __uint_as_float(sv[64 * i + 2 * e + 1])),
+                                                  sc2, m2);
+                            const float2 w = make_float2(ex2(x.x), ex2(x.y));
+                            add[e & 1] = add2(add[e & 1], w);
+                            pv[e] = num<T>::pack(w.x, w.y);
                         }
                         tc_st32(s_at + 32 * i, pv);
+                        tc_wait_st();
+                        tc_before();
+                        bar_arrive(p_ready + 16 * g + 8 * i);
                     }
-                    l += (add[0] + add[1]) + (add[2] + add[3]);
-                    // rows of V that the sequence does not own may hold anything: weight 0 must meet 0
-                    if (k0 + B_KEYS > I.kv || k0 < seen) {
-                        const uint32_t i = ring0 + 2 * j + 1;
-                        if (!(ok = bar_wait_warp(kv_full + 8 * (i % ST), (i / ST) & 1, stop))) break;
-                        if (k0 + row >= I.kv || k0 + row < seen) {
-                            const uint32_t vb = ring + (i % ST) * TB + row * 128;
-#pragma unroll
-                            for (int c = 0; c < D / 8; c++)
-                                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};\n"
-                                             :: "r"(vb + (c / 8) * HB + (c % 8) * 16), "r"(0) : "memory");
-                        }
-                        asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
-                    }
-                    tc_wait_st();
-                    tc_before();
-                    bar_arrive(p_ready + 8 * g);
+                    l += (add[0].x + add[0].y) + (add[1].x + add[1].y);
                 }
                 if (!ok || !(ok = bar_wait_warp(o_full + 8 * g, no++ & 1, stop))) break;
                 tc_after();
+                const int r = my_row();
+                const bool live = r < X.rows;
+                const int64_t tok = X.first + r / L.G;
+                const int head = X.head * L.G + r % L.G;
                 // 32 dims at a time: o becomes the row's outputs
                 auto put = [&](int i, uint32_t (&o)[32], float inv) {
                     uint4 * out = reinterpret_cast<uint4 *>(dst + tok * dst_ld + (int64_t) head * D + 32 * i);
@@ -1162,7 +1215,10 @@ k_paged_attn_tiles(const __grid_constant__ CUtensorMap kmap, const __grid_consta
                         out[e] = make_uint4(pack2<T>(o[8 * e], o[8 * e + 1]), pack2<T>(o[8 * e + 2], o[8 * e + 3]),
                                             pack2<T>(o[8 * e + 4], o[8 * e + 5]), pack2<T>(o[8 * e + 6], o[8 * e + 7]));
                 };
-                if (!I.cut) {
+                const int c0 = X.c0, others = X.others;
+                const bool cut_up = X.cut != 0;
+                release();
+                if (!cut_up) {
                     const float inv = l != 0.0f ? 1.0f / l : 0.0f;
 #pragma unroll 1
                     for (int i = 0; i < D / 32; i++) {
@@ -1174,7 +1230,7 @@ k_paged_attn_tiles(const __grid_constant__ CUtensorMap kmap, const __grid_consta
                     continue;
                 }
                 // [slot][warp 0..7][d / 4][lane] and [slot][warp][lane]
-                auto slot = [&](int c) { return parts + ((int64_t) c * 2 + (c == I.c0)) * B_PART; };
+                auto slot = [&](int c) { return parts + ((int64_t) c * 2 + (c == c0)) * B_PART; };
                 auto slot_o = [&](int c) { return reinterpret_cast<float4 *>(slot(c)) + warp * (D / 4) * 32 + lane; };
                 auto slot_m = [&](int c) { return reinterpret_cast<float2 *>(slot(c) + B_TILE * 128) + warp * 32 + lane; };
 #pragma unroll 1
@@ -1192,12 +1248,12 @@ k_paged_attn_tiles(const __grid_constant__ CUtensorMap kmap, const __grid_consta
                 __threadfence();
                 __syncwarp();
                 int last = 0;
-                if (lane == 0) last = atomicAdd(&counters[I.c0 * 8 + warp], 1) == I.others;
+                if (lane == 0) last = atomicAdd(&counters[c0 * 8 + warp], 1) == others;
                 if (!__shfl_sync(0xFFFFFFFFu, last, 0)) continue;
                 __threadfence();
                 m = k_none;
                 l = 0.0f;
-                for (int c = I.c0; c <= I.c0 + I.others; c++) {
+                for (int c = c0; c <= c0 + others; c++) {
                     const float2 ml = __ldcg(slot_m(c));
                     const float mn = fmaxf(m, ml.x);
                     l = l * ex2(m - mn) + ml.y * ex2(ml.x - mn);
@@ -1207,7 +1263,7 @@ k_paged_attn_tiles(const __grid_constant__ CUtensorMap kmap, const __grid_consta
 #pragma unroll 1
                 for (int i = 0; i < D / 32; i++) {
                     float a[32] = {};
-                    for (int c = I.c0; c <= I.c0 + I.others; c++) {
+                    for (int c = c0; c <= c0 + others; c++) {
                         const float f = ex2(__ldcg(slot_m(c)).x - m);
 #pragma unroll
                         for (int e = 0; e < 8; e++) {
@@ -1223,7 +1279,7 @@ k_paged_attn_tiles(const __grid_constant__ CUtensorMap kmap, const __grid_consta
                     for (int e = 0; e < 32; e++) o[e] = __float_as_uint(a[e]);
                     if (live) put(i, o, inv);
                 }
-                if (lane == 0) counters[I.c0 * 8 + warp] = 0;
+                if (lane == 0) counters[c0 * 8 + warp] = 0;
             }
             tc_wait_st();
         }
@@ -1295,19 +1351,6 @@ __device__ __forceinline__ ull mass_of(float w) {
     return mass_sum(hi, lo, 1);
 }
 
-// two floats in one instruction
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-    float2 c;
-    asm("{\n.reg .b64 x, y, z;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\nadd.rn.f32x2 z, x, y;\nmov.b64 {%0, %1}, z;\n}\n"
-        : "=f"(c.x), "=f"(c.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-    return c;
-}
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-    float2 c;
-    asm("{\n.reg .b64 x, y, z;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\nmul.rn.f32x2 z, x, y;\nmov.b64 {%0, %1}, z;\n}\n"
-        : "=f"(c.x), "=f"(c.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-    return c;
-}
 __device__ __forceinline__ void mass_parts2(float2 w, uint32_t (&hi)[2], uint32_t (&lo)[2]) {
     const float2 h = add2(w, make_float2(S_HI, S_HI)), g = add2(h, make_float2(-S_HI, -S_HI));
     const float2 l = add2(add2(w, make_float2(-g.x, -g.y)), make_float2(S_LO, S_LO));
