@@ -616,23 +616,33 @@ k_paged_attn_rows(paged P, const T * __restrict__ q, T * __restrict__ dst, const
 // ===================== attention: chunks ===================================
 //
 // Sequences with more than 16 rows (token, head of the group) go to the
-// tensor cores in tiles of 256 rows, two groups of 128, over tiles of 128
-// keys.  S = Q K^T of a group lands in 128 columns of TMEM, one row a lane;
-// the group's 128 threads read one row each, so maximum and sum need no other
-// thread, and write the weights back into the same columns as the 16-bit A
-// operand of P V, whose sum O stays in TMEM.
+// tensor cores in tiles of 256 rows, two groups of 128, over tiles of keys.
+// S = Q K^T of a group lands in TMEM, one row a lane; the group's 128 threads
+// read one row each, so maximum and sum need no other thread, and write the
+// weights back into the same columns as the 16-bit A operand of P V, whose sum
+// O stays in TMEM.
+//
+// Head dim 64 leaves TMEM for two S of 64 keys to each group: while its softmax
+// works on one, the next is ready, so it waits for no product (45 us where one
+// S of 128 keys takes 57, on 16 sequences of up to 512 new tokens in a window
+// of 1,024).  At 128 the products are what counts, and QK over 64 keys reads
+// shared memory for Q as long as over 128: one S of 128 keys (765 us where two
+// of 64 take 998, on two chunks of 2,000 tokens over 16,384 keys), and PV of
+// its first 64 keys starts under the weights of the others.
 //
 //   warps 0-3, 4-7  group 0, group 1: Q into shared memory, softmax, output
 //   warp 8          one thread issues every MMA: PV of a group's tile j, then
-//                   its QK of tile j + 1, one group after the other, so one
-//                   group's softmax runs under the other's products
-//   warp 9          TMA of K and V pages through a ring of 128-key tiles
+//                   its QK of the next tile for that S, one group after the
+//                   other, so one group's softmax runs under the other's
+//                   products
+//   warp 9          TMA of K and V pages through a ring of tiles
 //   warp 10         walks the CTA's share of the line and hands out its items
 //   warp 11         nothing: it completes the warpgroup that gives registers to
-//                   the softmax (168 x 384 at launch = 208 x 256 + 88 x 128)
+//                   the softmax at head dim 128 (168 x 384 at launch = 208 x 256
+//                   + 88 x 128)
 //
-// TMEM operations of one thread run in the order of their issue: QK of tile
-// j + 1 may overwrite the weights that PV of tile j reads.  As with few rows,
+// TMEM operations of one thread run in the order of their issue: QK of the
+// next tile may overwrite the weights that PV of tile j reads.  As with few rows,
 // the (row tile, kv head, key tile) units of all sequences form a line that
 // the CTAs cut into equal shares; each warp joins its own 32 rows of a cut
 // item, so no warp waits for another outside the mbarriers.
@@ -640,7 +650,7 @@ k_paged_attn_rows(paged P, const T * __restrict__ q, T * __restrict__ dst, const
 // Every wait gives up after k_wait_cycles: the CTA then drains what it has in
 // flight, frees its TMEM and counts a timeout.
 
-constexpr int B_ROWS = 128, B_TILE = 256, B_KEYS = 128, B_THREADS = 384, B_SUMS = 256, B_ITEMS = 4, B_CTAS = k_sms;
+constexpr int B_ROWS = 128, B_TILE = 256, B_THREADS = 384, B_SUMS = 256, B_ITEMS = 4, B_CTAS = k_sms;
 constexpr long long k_wait_cycles = 1ll << 31;
 
 // partials: [slot][group][warp][d / 4][lane] float4, then [warp][lane] (m, l)
@@ -736,14 +746,15 @@ __device__ __forceinline__ void tc_st32(uint32_t a, const uint32_t * v) {
 // ---- the line ----
 struct tile_plan {
     int64_t rows_above, window;      // sequences of more rows than this
-    int     G;
+    int     G, key_shift;            // heads to a kv head; log2 of the keys of a tile
 };
 // key tiles [lo, hi) of row tile rt of a sequence; one at least
 __device__ __forceinline__ void tile_keys(const tile_plan & L, const seq_span & S, int64_t rt, int64_t & lo, int64_t & n) {
-    const int64_t R = S.n * L.G, pos0 = S.kv - S.n;
-    const int64_t last = (min((rt + 1) * B_TILE, R) - 1) / L.G, first = rt * B_TILE / L.G;
-    const int64_t hi = (max(min(S.kv, pos0 + last + 1), (int64_t) 0) + B_KEYS - 1) / B_KEYS;
-    lo = L.window > 0 ? max((int64_t) 0, pos0 + first - L.window + 1) / B_KEYS : 0;
+    const int64_t pos0 = S.kv - S.n;
+    const uint32_t R = (uint32_t) (S.n * L.G), r0 = (uint32_t) rt * B_TILE;      // below 2^31
+    const uint32_t last = (min(r0 + B_TILE, R) - 1) / (uint32_t) L.G, first = r0 / (uint32_t) L.G;
+    const int64_t hi = (max(min(S.kv, pos0 + last + 1), (int64_t) 0) + (1 << L.key_shift) - 1) >> L.key_shift;
+    lo = L.window > 0 ? max((int64_t) 0, pos0 + first - L.window + 1) >> L.key_shift : 0;
     n = max((int64_t) 1, hi - lo);
 }
 __device__ __forceinline__ int64_t row_tiles_of(const tile_plan & L, const seq_span & S) {
@@ -829,7 +840,7 @@ struct line_walk {
         I.pos0 = (int) (S.kv - S.n);
         I.r0 = (int) (rt * B_TILE);
         I.rows = (int) (S.n * L.G);
-        I.key0 = (int) ((lo0 + t0) * B_KEYS);
+        I.key0 = (int) ((lo0 + t0) << L.key_shift);
         I.n = (int) (t1 - t0);
         I.cut = t0 > 0 || t1 < len;
         // CTA b holds unit y where W b / N <= y
@@ -845,17 +856,19 @@ __device__ __forceinline__ int first_owned(const tile_item & I, const tile_plan 
 }
 
 // shared memory of one CTA
-template <int D> __host__ __device__ constexpr int b_tile_bytes() { return B_KEYS * D * 2; }
+template <int D> __host__ __device__ constexpr int b_keys() { return D == 128 ? 128 : 64; }
+template <int D> __host__ __device__ constexpr int b_tile_bytes() { return b_keys<D>() * D * 2; }
+template <int D> __host__ __device__ constexpr int b_q_bytes() { return B_ROWS * D * 2; }
 template <int D> __host__ __device__ constexpr int b_ring() { return D == 128 ? 5 : 10; }
 struct tile_control {                // behind the tiles
     int64_t   sums[B_SUMS];
     tile_item item[B_ITEMS];
-    uint64_t  bar[2 * 10 + 2 * B_ITEMS + 11];
+    uint64_t  bar[2 * 10 + 2 * B_ITEMS + 15];
     uint32_t  tmem;
     int       stop;
 };
 template <int D> __host__ __device__ constexpr int b_smem() {
-    return (2 + b_ring<D>()) * b_tile_bytes<D>() + (int) sizeof(tile_control);
+    return 2 * b_q_bytes<D>() + b_ring<D>() * b_tile_bytes<D>() + (int) sizeof(tile_control);
 }
 static_assert(b_smem<128>() <= 227 * 1024 && b_smem<64>() <= 227 * 1024, "shared memory of one CTA");
 
@@ -864,20 +877,22 @@ __global__ void __launch_bounds__(B_THREADS, 1)
 k_paged_attn_tiles(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, paged P, tile_plan L,
                    const T * __restrict__ q, T * __restrict__ dst, int64_t q_ld, int64_t dst_ld, float scale_log2,
                    int * __restrict__ counters, float * __restrict__ parts, int after_rows) {
-    constexpr int ST = b_ring<D>(), TB = b_tile_bytes<D>(), HB = B_KEYS * 128, HALVES = D / 64;
+    // bytes of a K or V tile, of its 64-dim halves, and of Q's
+    constexpr int B_KEYS = b_keys<D>(), BUFS = D == 128 ? 1 : 2, PARTS = B_KEYS / 64;
+    constexpr int ST = b_ring<D>(), TB = b_tile_bytes<D>(), HB = B_KEYS * 128, QB = b_q_bytes<D>(), QH = B_ROWS * 128, HALVES = D / 64;
     constexpr bool BF = std::is_same<T, __nv_bfloat16>::value;
     // f32 sums of 16-bit operands, 128 rows; B of PV is [key][dim], keys outside
     constexpr uint32_t fmt = (1u << 4) | ((BF ? 1u : 0u) << 7) | ((BF ? 1u : 0u) << 10) | (8u << 24);
     constexpr uint32_t idesc_qk = fmt | ((B_KEYS / 8) << 17), idesc_pv = fmt | (1u << 16) | ((D / 8) << 17);
-    constexpr uint32_t S_COL = 0, O_COL = 256;              // + 128 g, + D g
+    constexpr uint32_t S_COL = 0, O_COL = 256;              // + 128 g (+ 64 for every other tile of 64 keys), + D g
 
     extern __shared__ __align__(1024) unsigned char tile_sm[];     // swizzled tiles: 1024-byte boundaries
-    tile_control & C = *reinterpret_cast<tile_control *>(tile_sm + (2 + ST) * TB);
+    tile_control & C = *reinterpret_cast<tile_control *>(tile_sm + 2 * QB + ST * TB);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const uint32_t q_sm = smem_addr(tile_sm), ring = q_sm + 2 * TB;
+    const uint32_t q_sm = smem_addr(tile_sm), ring = q_sm + 2 * QB;
     const uint32_t bars = smem_addr(C.bar);
     const uint32_t kv_full = bars, kv_empty = bars + 8 * ST, q_full = kv_empty + 8 * ST, s_full = q_full + 16,
-                   p_ready = s_full + 16, o_full = p_ready + 32, it_full = o_full + 16, it_empty = it_full + 8 * B_ITEMS, drained = it_empty + 8 * B_ITEMS;
+                   p_ready = s_full + 32, o_full = p_ready + 32, pv_done = o_full + 16, it_full = pv_done + 16, it_empty = it_full + 8 * B_ITEMS, drained = it_empty + 8 * B_ITEMS;
     volatile int * stop = &C.stop;
 
     if (tid == 0) {
@@ -887,9 +902,11 @@ k_paged_attn_tiles(const __grid_constant__ CUtensorMap kmap, const __grid_consta
         }
         for (int g = 0; g < 2; g++) {
             bar_init(q_full + 8 * g, B_ROWS);
-            bar_init(s_full + 8 * g, 1);
-            bar_init(p_ready + 16 * g, B_ROWS);
-            bar_init(p_ready + 16 * g + 8, B_ROWS);
+            for (int b = 0; b < 2; b++) {
+                bar_init(s_full + 16 * g + 8 * b, 1);
+                bar_init(p_ready + 16 * g + 8 * b, B_ROWS);
+            }
+            bar_init(pv_done + 8 * g, 1);
             bar_init(o_full + 8 * g, 1);
         }
         for (int i = 0; i < B_ITEMS; i++) {
@@ -959,7 +976,7 @@ k_paged_attn_tiles(const __grid_constant__ CUtensorMap kmap, const __grid_consta
             return I.n > 0;
         };
         if (warp >= 8) {
-            asm volatile("setmaxnreg.dec.sync.aligned.u32 88;\n" ::);
+            if constexpr (D == 128) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;\n" ::);
         if (warp == 10) {
             // ------------------------------------------------ items
             line_walk walk;
@@ -990,24 +1007,40 @@ k_paged_attn_tiles(const __grid_constant__ CUtensorMap kmap, const __grid_consta
             bool ok = true;
             while (ok && next_item()) {
                 const int seen = first_owned(I, L);
-                for (int t = 0; ok && t < I.n; t++) {
+                // the page (out of bounds: zeros) and its row that this lane copies of tile t
+                auto place = [&](int t, int & row) {
                     const int64_t key = (int64_t) I.key0 + t * B_KEYS + lane * box;
                     int64_t page = -1;
-                    if (lane < boxes && key < I.kv && key + box > seen) page = page_of(P, I.seq, key);
-                    if (page < 0) page = P.n_pages;          // out of bounds: zeros
-                    const int row = (int) (key & ((1 << P.page_shift) - 1));
+                    if (t < I.n && lane < boxes && key < I.kv && key + box > seen) page = page_of(P, I.seq, key);
+                    row = (int) (key & ((1 << P.page_shift) - 1));
+                    return (int) (page < 0 ? P.n_pages : page);
+                };
+                auto copy = [&](const CUtensorMap * map, int page, int row) {
+                    const uint32_t b = n % ST;
+                    if (!bar_wait_warp(kv_empty + 8 * b, ((n / ST) & 1) ^ 1, stop)) return false;
+                    if (lane == 0) bar_expect(kv_full + 8 * b, TB);
+                    __syncwarp();
+                    if (lane < boxes)
 #pragma unroll
-                    for (int kv = 0; kv < 2; kv++, n++) {
-                        const uint32_t b = n % ST;
-                        if (!(ok = bar_wait_warp(kv_empty + 8 * b, ((n / ST) & 1) ^ 1, stop))) break;
-                        if (lane == 0) bar_expect(kv_full + 8 * b, TB);
-                        __syncwarp();
-                        if (lane < boxes)
+                        for (int i = 0; i < HALVES; i++)
+                            tma_page(ring + b * TB + i * HB + lane * box * 128, map, 64 * i, row, I.head, page, kv_full + 8 * b);
+                    n++;
+                    return true;
+                };
+                // in the order of their use: K 0 (K 1), then V 0, K 1 (K 2), V 1, ..
+                // (page ids are looked up a tile ahead)
+                int row[BUFS + 1], page[BUFS + 1];
 #pragma unroll
-                            for (int i = 0; i < HALVES; i++)
-                                tma_page(ring + b * TB + i * HB + lane * box * 128, kv ? &vmap : &kmap, 64 * i, row, I.head,
-                                         (int) page, kv_full + 8 * b);
-                    }
+                for (int t = 0; t <= BUFS; t++) {
+                    page[t] = place(t, row[t]);
+                    if (t < BUFS && t < I.n) ok = ok && copy(&kmap, page[t], row[t]);
+                }
+                for (int t = 0; ok && t < I.n; t++) {
+                    ok = copy(&vmap, page[0], row[0]);
+                    if (t + BUFS < I.n) ok = ok && copy(&kmap, page[BUFS], row[BUFS]);
+#pragma unroll
+                    for (int i = 0; i < BUFS; i++) page[i] = page[i + 1], row[i] = row[i + 1];
+                    page[BUFS] = place(t + BUFS + 1, row[BUFS]);
                 }
             }
             // nothing of this CTA's may be in flight when it ends
@@ -1016,57 +1049,62 @@ k_paged_attn_tiles(const __grid_constant__ CUtensorMap kmap, const __grid_consta
         } else if (warp == 8) {
             // ------------------------------------------------ MMA
             uint32_t n = 0;                                  // ring position of the item's first K
-            uint32_t np[2] = { 0, 0 }, nq[2] = { 0, 0 };     // phases of p_ready and q_full
+            uint32_t tiles[2] = { 0, 0 }, nq[2] = { 0, 0 };  // tiles of each group so far; phases of q_full
             bool ok = true;
             while (ok && next_item()) {
                 const int groups = I.rows - I.r0 > B_ROWS ? 2 : 1;
                 const uint32_t nt = (uint32_t) I.n;
                 if (lane == 0) {
-                    auto qk = [&](int g, uint32_t i) {
-                        const uint32_t kb = ring + (i % ST) * TB, qb = q_sm + g * TB;
+                    auto full = [&](uint32_t i) { return bar_wait(kv_full + 8 * (i % ST), (i / ST) & 1, stop); };
+                    auto k_at = [&](uint32_t j) { return n + (j < BUFS ? j : 2 * j - BUFS + 1); };     // ring positions
+                    auto v_at = [&](uint32_t j) { return n + min(j + BUFS, nt) + j; };
+                    auto qk = [&](int g, uint32_t j) {
+                        const uint32_t kb = ring + k_at(j) % ST * TB, qb = q_sm + g * QB, b = (tiles[g] + j) % BUFS;
 #pragma unroll
-                        for (int k = 0; k < D / 16; k++) {
-                            const uint32_t off = (k / 4) * HB + (k % 4) * 32;
-                            mma_ss(tmem + S_COL + 128 * g, smem_desc(qb + off, 16, 1024), smem_desc(kb + off, 16, 1024),
-                                   idesc_qk, k > 0);
-                        }
-                        mma_commit(s_full + 8 * g);
+                        for (int k = 0; k < D / 16; k++)
+                            mma_ss(tmem + S_COL + 128 * g + 64 * b, smem_desc(qb + (k / 4) * QH + (k % 4) * 32, 16, 1024),
+                                   smem_desc(kb + (k / 4) * HB + (k % 4) * 32, 16, 1024), idesc_qk, k > 0);
+                        mma_commit(s_full + 16 * g + 8 * b);
                     };
-                    ok = bar_wait(kv_full + 8 * (n % ST), (n / ST) & 1, stop);
-                    for (int g = 0; ok && g < groups; g++) {
-                        ok = bar_wait(q_full + 8 * g, nq[g]++ & 1, stop);
-                        tc_after();
-                        if (ok) qk(g, n);
-                    }
-                    if (ok) mma_commit(kv_empty + 8 * (n % ST));
-                    for (uint32_t j = 0; ok && j < nt; j++) {
-                        const uint32_t v = n + 2 * j + 1, k = v + 1;
-                        const uint32_t vb = ring + (v % ST) * TB;
-                        ok = bar_wait(kv_full + 8 * (v % ST), (v / ST) & 1, stop);
+                    for (uint32_t j = 0; ok && j < min(nt, (uint32_t) BUFS); j++) {
+                        ok = full(k_at(j));
                         for (int g = 0; ok && g < groups; g++) {
-#pragma unroll
-                            for (int half = 0; half < 2; half++) {
-                                if (!(ok = ok && bar_wait(p_ready + 16 * g + 8 * half, np[g] & 1, stop))) break;
+                            if (j == 0) ok = bar_wait(q_full + 8 * g, nq[g]++ & 1, stop);
+                            tc_after();
+                            if (ok) qk(g, j);
+                        }
+                        if (ok) mma_commit(kv_empty + 8 * (k_at(j) % ST));
+                    }
+                    for (uint32_t j = 0; ok && j < nt; j++) {
+                        const uint32_t vb = ring + v_at(j) % ST * TB;
+                        ok = full(v_at(j));
+                        for (int g = 0; ok && g < groups; g++) {
+                            const uint32_t at = tiles[g] + j, b = at % BUFS;
+                            auto pv = [&](int part) {
+                                if (!bar_wait(p_ready + 16 * g + 8 * (PARTS == 2 ? part : b), at / BUFS & 1, stop)) return false;
                                 tc_after();
 #pragma unroll
-                                for (int kk = 4 * half; kk < 4 * half + 4; kk++)
-                                    mma_ts(tmem + O_COL + D * g, tmem + S_COL + 128 * g + 8 * kk,
+                                for (int kk = 4 * part; kk < 4 * part + 4; kk++)
+                                    mma_ts(tmem + O_COL + D * g, tmem + S_COL + 128 * g + 64 * b + 8 * kk,
                                            smem_desc(vb + kk * 2048, HB, 1024), idesc_pv, j > 0 || kk > 0);
-                            }
-                            if (!ok) break;
-                            np[g]++;
-                            if (j + 1 < nt) {
-                                if (g == 0 && !(ok = bar_wait(kv_full + 8 * (k % ST), (k / ST) & 1, stop))) break;
-                                qk(g, k);
-                            } else {
-                                mma_commit(o_full + 8 * g);
+                                return true;
+                            };
+                            if (!(ok = pv(0))) break;
+                            if constexpr (PARTS == 2)
+                                if (!(ok = pv(1))) break;
+                            if (j + 1 == nt) mma_commit(o_full + 8 * g);
+                            else if (BUFS == 2) mma_commit(pv_done + 8 * g);
+                            if (j + BUFS < nt) {
+                                if (g == 0 && !(ok = full(k_at(j + BUFS)))) break;
+                                qk(g, j + BUFS);
                             }
                         }
                         if (ok) {
-                            mma_commit(kv_empty + 8 * (v % ST));
-                            if (j + 1 < nt) mma_commit(kv_empty + 8 * (k % ST));
+                            mma_commit(kv_empty + 8 * (v_at(j) % ST));
+                            if (j + BUFS < nt) mma_commit(kv_empty + 8 * (k_at(j + BUFS) % ST));
                         }
                     }
+                    for (int g = 0; g < groups; g++) tiles[g] += nt;
                 }
                 n += 2 * nt;
                 ok = __shfl_sync(0xFFFFFFFFu, ok, 0);
@@ -1079,13 +1117,13 @@ k_paged_attn_tiles(const __grid_constant__ CUtensorMap kmap, const __grid_consta
             __syncwarp();
         }
         } else {
-            asm volatile("setmaxnreg.inc.sync.aligned.u32 208;\n" ::);
+            if constexpr (D == 128) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;\n" ::);
             // ------------------------------------------------ softmax and output
             const int g = warp >> 2, row = tid & 127;
             const uint32_t lanes = (uint32_t) (warp & 3) << 21;      // TMEM lane 32 (warp % 4)
             const uint32_t s_at = tmem + lanes + S_COL + 128 * g, o_at = tmem + lanes + O_COL + D * g;
-            uint32_t ns = 0, no = 0;                                 // phases of s_full and o_full
-            uint32_t n = 0;
+            uint32_t tiles = 0, no = 0, npv = 0;                     // tiles so far; phases of o_full and pv_done
+            uint32_t n = 0;                                          // ring position of the item's first K
             const int win = (int) min(L.window, (int64_t) 0x7FFFFFFF);
             bool ok = true;
             for (; ok; items++) {
@@ -1109,7 +1147,7 @@ k_paged_attn_tiles(const __grid_constant__ CUtensorMap kmap, const __grid_consta
                     const int r = my_row();
                     const uint4 * src = reinterpret_cast<const uint4 *>(q + (int64_t) (X.first + r / L.G) * q_ld +
                                                                         (int64_t) (X.head * L.G + r % L.G) * D);
-                    const uint32_t qb = q_sm + g * TB + row * 128;
+                    const uint32_t qb = q_sm + g * QB + row * 128;
                     const bool live = r < X.rows;
                     uint4 v[D / 8];
 #pragma unroll
@@ -1117,7 +1155,7 @@ k_paged_attn_tiles(const __grid_constant__ CUtensorMap kmap, const __grid_consta
 #pragma unroll
                     for (int i = 0; i < D / 8; i++)
                         asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n"
-                                     :: "r"(qb + (i / 8) * HB + (((i % 8) ^ (row & 7)) << 4)), "r"(v[i].x), "r"(v[i].y),
+                                     :: "r"(qb + (i / 8) * QH + (((i % 8) ^ (row & 7)) << 4)), "r"(v[i].x), "r"(v[i].y),
                                         "r"(v[i].z), "r"(v[i].w) : "memory");
                     asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
                     bar_arrive(q_full + 8 * g);
@@ -1128,24 +1166,26 @@ k_paged_attn_tiles(const __grid_constant__ CUtensorMap kmap, const __grid_consta
                 const int last_win = win ? X.pos0 + (min(X.r0 + B_ROWS * g + B_ROWS, X.rows) - 1) / L.G - win - X.key0 : -1;
                 float m = k_none, l = 0.0f;
                 for (uint32_t j = 0; j < nt; j++) {
-                    if (!(ok = bar_wait_warp(s_full + 8 * g, ns++ & 1, stop))) break;
+                    const uint32_t buf = tiles % BUFS, s_now = s_at + 64 * buf;
+                    if (!(ok = bar_wait_warp(s_full + 16 * g + 8 * buf, tiles / BUFS & 1, stop))) break;
+                    tiles++;
                     tc_after();
-                    uint32_t sv[128];
+                    uint32_t sv[B_KEYS];
 #pragma unroll
-                    for (int i = 0; i < 4; i++) tc_ld32(s_at + 32 * i, sv + 32 * i);
+                    for (int i = 0; i < B_KEYS / 32; i++) tc_ld32(s_now + 32 * i, sv + 32 * i);
                     tc_wait_ld(sv);
                     if ((int) j * B_KEYS + B_KEYS - 1 > first_pos || (int) j * B_KEYS <= last_win) {
                         const int k0 = X.key0 + (int) j * B_KEYS, pos = X.pos0 + my_row() / L.G;
                         const int seen = win ? max(0, X.pos0 - win + 1) : 0, kv = X.kv;
                         const int hi = pos - k0, lo = win ? pos - win + 1 - k0 : 0;     // columns lo .. hi
 #pragma unroll
-                        for (int i = 0; i < 128; i++)
+                        for (int i = 0; i < B_KEYS; i++)
                             if (i > hi || i < lo) sv[i] = 0xFF800000u;
                         // those rows of V may hold anything: weight 0 must meet 0
                         if (k0 + B_KEYS > kv || k0 < seen) {
-                            const uint32_t i = ring0 + 2 * j + 1;
+                            const uint32_t i = ring0 + min(j + BUFS, nt) + j;
                             if (!(ok = bar_wait_warp(kv_full + 8 * (i % ST), (i / ST) & 1, stop))) break;
-                            if (k0 + row >= kv || k0 + row < seen) {
+                            if (row < B_KEYS && (k0 + row >= kv || k0 + row < seen)) {
                                 const uint32_t vb = ring + (i % ST) * TB + row * 128;
 #pragma unroll
                                 for (int c = 0; c < D / 8; c++)
@@ -1157,7 +1197,7 @@ k_paged_attn_tiles(const __grid_constant__ CUtensorMap kmap, const __grid_consta
                     }
                     float t4[4] = { -INFINITY, -INFINITY, -INFINITY, -INFINITY };
 #pragma unroll
-                    for (int i = 0; i < 128; i += 8)
+                    for (int i = 0; i < B_KEYS; i += 8)
 #pragma unroll
                         for (int e = 0; e < 4; e++)
                             t4[e] = max3(t4[e], __uint_as_float(sv[i + 2 * e]), __uint_as_float(sv[i + 2 * e + 1]));
@@ -1167,6 +1207,9 @@ k_paged_attn_tiles(const __grid_constant__ CUtensorMap kmap, const __grid_consta
                         m = mn;
                         l *= f;
                         if (j > 0) {
+                            // with two S, PV of the tile before may be on its way (with one, S came after it)
+                            if (BUFS == 2 && !(ok = bar_wait_warp(pv_done + 8 * g, (npv - 1) & 1, stop))) break;
+                            tc_after();
 #pragma unroll
                             for (int i = 0; i < D / 32; i++) {
                                 uint32_t ov[32];
@@ -1178,11 +1221,10 @@ k_paged_attn_tiles(const __grid_constant__ CUtensorMap kmap, const __grid_consta
                             }
                         }
                     }
-                    // PV of the first 64 keys starts while the others' weights are computed
                     float2 add[2] = { { 0, 0 }, { 0, 0 } };
                     const float2 sc2 = make_float2(scale_log2, scale_log2), m2 = make_float2(-m, -m);
 #pragma unroll
-                    for (int i = 0; i < 2; i++) {
+                    for (int i = 0; i < PARTS; i++) {
                         uint32_t pv[32];
 #pragma unroll
                         for (int e = 0; e < 32; e++) {
@@ -1192,11 +1234,12 @@ k_paged_attn_tiles(const __grid_constant__ CUtensorMap kmap, const __grid_consta
                             add[e & 1] = add2(add[e & 1], w);
                             pv[e] = num<T>::pack(w.x, w.y);
                         }
-                        tc_st32(s_at + 32 * i, pv);
+                        tc_st32(s_now + 32 * i, pv);
                         tc_wait_st();
                         tc_before();
-                        bar_arrive(p_ready + 16 * g + 8 * i);
+                        bar_arrive(p_ready + 16 * g + 8 * (PARTS == 2 ? i : buf));
                     }
+                    npv += j + 1 < nt;         // PV of an item's last tile goes to o_full
                     l += (add[0].x + add[0].y) + (add[1].x + add[1].y);
                 }
                 if (!ok || !(ok = bar_wait_warp(o_full + 8 * g, no++ & 1, stop))) break;
@@ -2470,12 +2513,12 @@ encode_fn tensor_map_encoder() {
     return fn;
 }
 // a cache as (64 of dim, row of the page, kv head, page); false: not to be described
-bool map_cache(CUtensorMap * m, const lnsb_paged_kv & c, void * cache) {
+bool map_cache(CUtensorMap * m, const lnsb_paged_kv & c, void * cache, int keys) {
     const encode_fn encode = tensor_map_encoder();
     if (encode == nullptr) return false;
     const cuuint64_t dims[4] = { (cuuint64_t) c.head_dim, (cuuint64_t) c.page_size, (cuuint64_t) c.n_head_kv, (cuuint64_t) c.n_pages };
     const cuuint64_t strides[3] = { (cuuint64_t) c.row_stride * 2, (cuuint64_t) c.head_stride * 2, (cuuint64_t) c.page_stride * 2 };
-    const cuuint32_t box[4] = { 64, (cuuint32_t) std::min(c.page_size, B_KEYS), 1, 1 }, one[4] = { 1, 1, 1, 1 };
+    const cuuint32_t box[4] = { 64, (cuuint32_t) std::min(c.page_size, keys), 1, 1 }, one[4] = { 1, 1, 1, 1 };
     return encode(m, c.type == LNSB_TYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, cache, dims,
                   strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
@@ -2487,8 +2530,8 @@ int launch_attn_dim(const lnsb_paged_attn_args & a, cudaStream_t s) {
         const int G = a.n_head / a.kv.n_head_kv;
         CUtensorMap km, vm;
         // scale > 0: the tiles take the maximum before the scale
-        if (a.max_q * G > ROWS && a.kv.n_pages > 0 && a.scale > 0.0f && std::isfinite(a.scale) && map_cache(&km, a.kv, a.kv.k_cache) &&
-            map_cache(&vm, a.kv, a.kv.v_cache)) {
+        if (a.max_q * G > ROWS && a.kv.n_pages > 0 && a.scale > 0.0f && std::isfinite(a.scale) && map_cache(&km, a.kv, a.kv.k_cache, b_keys<D>()) &&
+            map_cache(&vm, a.kv, a.kv.v_cache, b_keys<D>())) {
             auto kern = k_paged_attn_tiles<T, D>;
             static bool attr[k_max_devices] = {};
             int st = allow_smem(kern, attr, b_smem<D>());
@@ -2500,6 +2543,8 @@ int launch_attn_dim(const lnsb_paged_attn_args & a, cudaStream_t s) {
             L.rows_above = both ? ROWS : 0;
             L.window = a.window;
             L.G = G;
+            L.key_shift = D == 128 ? 7 : 6;
+            static_assert(b_keys<D>() == (D == 128 ? 1 << 7 : 1 << 6), "keys of a tile");
             unsigned char * w = static_cast<unsigned char *>(a.work) + A_WORK;
             launch_k(kern, dim3(B_CTAS), dim3(B_THREADS), (size_t) b_smem<D>(), s, km, vm, view_of(a.kv), L,
                      static_cast<const T *>(a.q), static_cast<T *>(a.dst), a.q_ld, a.dst_ld, a.scale * k_log2e,
