@@ -190,6 +190,30 @@ def test_offsets_past_32_bits(ks, work):
     _check(ks, work, P, x[:, 2:3].contiguous())
 
 
+@pytest.mark.parametrize("dim", (64, 128, 32))
+@pytest.mark.parametrize("q", (1, 150))
+def test_visible_nan_stays(ks, work, dim, q):
+    """a NaN in a query is that row's alone; one in a key or value that rows see is theirs, and no other sequence's"""
+    P = ref.Paged([q, q], [400, 400], 2, dim, 16, BF16, seed=26)
+    qq = _q(P, 4, dim, BF16, 27)
+    clean = _attn(ks, work, P, qq)
+    assert not torch.isnan(clean).any()
+    bad = qq.clone()
+    bad[q - 1, 1, 3] = float("nan")
+    got = _attn(ks, work, P, bad)
+    assert torch.isnan(got[q - 1, 1]).all()
+    got[q - 1, 1] = clean[q - 1, 1]
+    assert torch.equal(got, clean)
+    for cache in (P.k, P.v):
+        at = (P.host_table[0, 0].item(), 5)
+        old = cache[at].clone()
+        cache[at][0] = float("nan")
+        got = _attn(ks, work, P, qq)
+        cache[at] = old
+        assert torch.isnan(got[:q, :2]).all()                # kv head 0 of the first sequence
+        assert torch.equal(got[q:], clean[q:]) and torch.equal(got[:q, 2:], clean[:q, 2:])
+
+
 # ------------------------------------------------------------------ append
 
 def _cos_sin(rows, half, seed=0):

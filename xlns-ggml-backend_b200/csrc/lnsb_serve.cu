@@ -571,7 +571,7 @@ k_paged_attn_rows(paged P, const T * __restrict__ q, T * __restrict__ dst, const
             }
             if (whole) {
                 const int64_t gr = r0 + r;
-                dst[(S.first + gr / G) * dst_ld + ((int64_t) h * G + gr % G) * D + d] = num<T>::from(den > 0 ? num_ / den : 0.0f);
+                dst[(S.first + gr / G) * dst_ld + ((int64_t) h * G + gr % G) * D + d] = num<T>::from(den != 0 ? num_ / den : 0.0f);
             } else {
                 part[r * D + d] = num_;
                 if (d == 0) {
@@ -603,7 +603,7 @@ k_paged_attn_rows(paged P, const T * __restrict__ q, T * __restrict__ dst, const
                     }
                     const int64_t gr = r0 + r;
                     dst[(S.first + gr / G) * dst_ld + ((int64_t) h * G + gr % G) * D + d] =
-                        num<T>::from(den > 0 ? num_ / den : 0.0f);
+                        num<T>::from(den != 0 ? num_ / den : 0.0f);
                 }
                 if (tid == 0) counters[c0] = 0;
             }
