@@ -1368,8 +1368,8 @@ k_paged_attn_tiles(const __grid_constant__ CUtensorMap kmap, const __grid_consta
 //            32-bit order-preserving keys.
 //
 // Measured: 1 x 49,152 F32 with every filter 16 us, 48 rows of mixed filters 36
-// us, 256 x 131,071 bf16 218 us (greedy rows alone 27, top-k 49-75, top-p alone
-// 185, where three passes take exponentials).
+// us, 256 x 131,071 bf16 151 us (greedy rows alone 25, top-k 27-55, top-p alone
+// 124-134, where three passes take exponentials).
 //
 // Masses are integers of 2^-38 of the largest weight, rounded to nearest: sums
 // are exact in any order, so the result hangs on no order of atomics.
@@ -1693,9 +1693,10 @@ k_sample(const T * __restrict__ logits, int64_t ld, int V, int vecs, int C, cons
         if (at >= 0 && at + E <= V) return __ldg(reinterpret_cast<const uint4 *>(x + at));
         return ends(at);
     };
-    // f(vector, index of its first element) for the row's vectors from .. to - 1; eight on their way at a time
+    // f(vector, index of its first element) for the row's vectors from .. to - 1; from memory two at a
+    // time (eight copies of f spent a third of the time on fetching instructions: 218 against 151 us on 256 x 131,071)
     auto each_vec = [&](int from, int to, auto f) {
-        constexpr int N = HELD ? 1 : 8;
+        constexpr int N = HELD ? 1 : 2;
         for (int i = from; i < to; i += N) {
             uint4 r[N];
 #pragma unroll
