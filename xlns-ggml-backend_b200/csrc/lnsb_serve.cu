@@ -884,7 +884,7 @@ template <class T, int D>
 __global__ void __launch_bounds__(B_THREADS, 1)
 k_paged_attn_tiles(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, paged P, tile_plan L,
                    const T * __restrict__ q, T * __restrict__ dst, int64_t q_ld, int64_t dst_ld, float scale_log2,
-                   int * __restrict__ counters, float * __restrict__ parts, int after_rows) {
+                   int * __restrict__ counters, float * __restrict__ parts) {
     // bytes of a K or V tile, of its 64-dim halves, and of Q's
     constexpr int B_KEYS = b_keys<D>(), BUFS = D == 128 ? 1 : 2, PARTS = B_KEYS / 64;
     constexpr int ST = b_ring<D>(), TB = b_tile_bytes<D>(), HB = B_KEYS * 128, QB = b_q_bytes<D>(), QH = B_ROWS * 128, HALVES = D / 64;
@@ -925,11 +925,9 @@ k_paged_attn_tiles(const __grid_constant__ CUtensorMap kmap, const __grid_consta
         C.stop = 0;
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
-    // behind k_paged_attn_rows of the same call this grid needs not wait at its
-    // start: that kernel let it launch after its own wait, and the two write
-    // different rows
-    if (!after_rows) asm volatile("griddepcontrol.wait;\n" ::: "memory");
-    asm volatile("griddepcontrol.launch_dependents;\n" :::);
+    // behind k_paged_attn_rows of the same call too: only a grid's own wait makes
+    // visible to it what earlier grids wrote (q, the plan, the cache's rows)
+    pdl_entry();
 
     // the line's length
     const int64_t per = (P.n_seqs + B_SUMS - 1) / B_SUMS;
@@ -1342,8 +1340,6 @@ k_paged_attn_tiles(const __grid_constant__ CUtensorMap kmap, const __grid_consta
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;\n" :: "r"(C.tmem));
         if (lane == 0 && C.stop) atomicAdd(&g_paged_errors[1], 1ull);
     }
-    // whoever waits for this grid waits for the rows kernel too
-    if (after_rows) asm volatile("griddepcontrol.wait;\n" ::: "memory");
 }
 
 // ============================ sampling =====================================
@@ -2561,7 +2557,7 @@ int launch_attn_dim(const lnsb_paged_attn_args & a, cudaStream_t s) {
             unsigned char * w = static_cast<unsigned char *>(a.work) + A_WORK;
             launch_k(kern, dim3(B_CTAS), dim3(B_THREADS), (size_t) b_smem<D>(), s, km, vm, view_of(a.kv), L,
                      static_cast<const T *>(a.q), static_cast<T *>(a.dst), a.q_ld, a.dst_ld, a.scale * k_log2e,
-                     reinterpret_cast<int *>(w), reinterpret_cast<float *>(w + B_COUNT_BYTES), both ? 1 : 0);
+                     reinterpret_cast<int *>(w), reinterpret_cast<float *>(w + B_COUNT_BYTES));
             return launch_status();
         }
     }
