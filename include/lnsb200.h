@@ -491,7 +491,8 @@ int lnsb_paged_errors(int64_t * bad_pages, int64_t * timeouts);
 
 /* The next token of every row of logits from one given random number per row.
  * With x = logits[r] (NaN counts as -inf), t = temperature[r] and
- *   w_i = exp((x_i - max x) * (1 / t)),  w_i = 1 where x_i is the maximum,
+ *   w_i = exp((x_i - max x) * (1 / t)),  w_i = 1 where x_i is the maximum
+ *   (1 / t at most the largest float),
  * the tokens in falling order of x, equal ones in order of their index, are
  * cut to the first top_k, of these to the shortest prefix whose sum of w is
  * at least top_p times theirs (one token at least), of these to those with

@@ -9,6 +9,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 #include <cstdint>
 #include <type_traits>
@@ -1417,7 +1418,7 @@ struct sample_row {
                          const float * uniform) {
         const float t = temperature ? temperature[row] : 1.0f;
         greedy = !(t > 0.0f);
-        inv_t = fminf(1.0f / t, 3.4e38f);
+        inv_t = fminf(1.0f / t, FLT_MAX);
         k = top_k ? top_k[row] : 0;
         if (k <= 0 || k > V) k = V;
         top_p = p ? p[row] : 1.0f;
@@ -1973,7 +1974,8 @@ k_sample(const T * __restrict__ logits, int64_t ld, int V, int vecs, int C, cons
     } else if (by_k || by_p || R.min_p > 0.0f) {
         // distance to the maximum in buckets: up to the smallest logit, or to where nothing weighs
         const float reach = fminf(low < top ? top - low : INFINITY, S_RANGE / R.inv_t);
-        const float q = -(S_BUCKETS - 1) / reach;
+        // finite, so that the maximum's own place is 0: below a reach of 2.4e-35 the logits take fewer buckets
+        const float q = -fminf((S_BUCKETS - 1) / reach, FLT_MAX);
         auto place = [&](float v) { return (v - top) * q; };      // NaN, or S_BUCKETS and more: none
         float below = 0.0f;                                       // the list: place < below
         bool list = false;
