@@ -1,0 +1,69 @@
+"""lnsb_paged_attn at the ends of its arguments' ranges, against plain 64-bit forms."""
+import pytest
+import torch
+
+import serve_ref as ref
+
+pytestmark = pytest.mark.gpu
+
+F16, BF16 = torch.float16, torch.bfloat16
+
+
+@pytest.fixture(scope="module")
+def ks():
+    import lnsb200
+    return lnsb200.KernelSet(16, "base")
+
+
+@pytest.fixture(scope="module")
+def work(ks):
+    return ks.paged_attn_work()
+
+
+def _q(P, heads, dim, dtype, seed, scale=1.5):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn((P.tokens, heads, dim), generator=g) * scale).to(dtype).cuda()
+
+
+def _attn(ks, work, P, q, window=0, max_q=None, max_kv=None, scale=None):
+    dst = torch.full_like(q, float("nan"))
+    ks.paged_attn(q, P.k, P.v, P.table, P.q_start, P.kv_len, P.max_q if max_q is None else max_q,
+                  P.max_kv if max_kv is None else max_kv, dst, work, window=window, scale=scale)
+    return dst
+
+
+def _check(P, q, got, window=0, scale=None):
+    want, mag = ref.attention(P, q, q.shape[2] ** -0.5 if scale is None else scale, window)
+    v_max = max([float(P.rows(P.v, s).abs().max()) for s in range(len(P.kv)) if P.kv[s]] + [0.0])
+    bound = ref.attention_bound(q.dtype, want, mag, P.max_kv, v_max)
+    bad = ~((got.double() - want).abs() <= bound)
+    assert not bad.any(), "%d of %d values off, worst %g of the bound" % (
+        int(bad.sum()), bad.numel(), float(((got.double() - want).abs() / bound).max()))
+
+
+# ------------------------------------------------------------------- windows
+
+@pytest.mark.parametrize("heads,kv_heads,dim", [(4, 2, 64), (4, 2, 128), (4, 2, 32)])
+@pytest.mark.parametrize("lengths", [([200], [150]), ([200, 1, 40], [150, 70, 10]), ([300, 30], [1, 7]), ([1, 2], [90, 1])], ids=str)
+def test_window_that_hides_nothing(ks, work, heads, kv_heads, dim, lengths):
+    """a window of the longest sequence and any longer one, up to the type's end, gives the bits of none; also where a
+    sequence has more new tokens than rows"""
+    P = ref.Paged(*lengths, kv_heads, dim, 16, BF16, seed=40)
+    q = _q(P, heads, dim, BF16, 41)
+    plain = _attn(ks, work, P, q)
+    _check(P, q, plain)
+    for window in (P.max_kv, P.max_kv + 1, 1000, 2 ** 31 - 1, 2 ** 31, 2 ** 32, 2 ** 32 + 5, 2 ** 63 - 1):
+        assert torch.equal(_attn(ks, work, P, q, window), plain), window
+    assert ks.paged_errors() == (0, 0)
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", [(4, 2, 64), (4, 2, 128), (4, 2, 32)])
+@pytest.mark.parametrize("window", (1, 2, 33, 100, 149))
+def test_window_with_rows_that_see_nothing(ks, work, heads, kv_heads, dim, window):
+    """windows over sequences with more new tokens than rows"""
+    P = ref.Paged([200, 1, 40, 3], [150, 70, 10, 0], kv_heads, dim, 16, BF16, seed=42)
+    q = _q(P, heads, dim, BF16, 43)
+    got = _attn(ks, work, P, q, window)
+    _check(P, q, got, window)
+    assert (got[:50] == 0).all() and (got[201:231] == 0).all() and (got[241:] == 0).all()
+    assert ks.paged_errors() == (0, 0)

@@ -1131,7 +1131,7 @@ k_paged_attn_tiles(const __grid_constant__ CUtensorMap kmap, const __grid_consta
             const uint32_t s_at = tmem + lanes + S_COL + 128 * g, o_at = tmem + lanes + O_COL + D * g;
             uint32_t tiles = 0, no = 0, npv = 0;                     // tiles so far; phases of o_full and pv_done
             uint32_t n = 0;                                          // ring position of the item's first K
-            const int win = (int) min(L.window, (int64_t) 0x7FFFFFFF);
+            const int win = (int) L.window;                          // below max_kv
             bool ok = true;
             for (; ok; items++) {
                 // the item stays in shared memory: the loop over the keys needs its registers for the scores
@@ -1170,7 +1170,7 @@ k_paged_attn_tiles(const __grid_constant__ CUtensorMap kmap, const __grid_consta
                 // a tile needs a look at its edges where its last key is past the first row's, or its first key before
                 // the last row's window; rows of V that the sequence does not own lie only in such tiles
                 const int first_pos = X.pos0 + (X.r0 + B_ROWS * g) / L.G - X.key0;
-                const int last_win = win ? X.pos0 + (min(X.r0 + B_ROWS * g + B_ROWS, X.rows) - 1) / L.G - win - X.key0 : -1;
+                const int last_win = win ? max(X.pos0 + (min(X.r0 + B_ROWS * g + B_ROWS, X.rows) - 1) / L.G, -1) - X.key0 - win : -1;
                 float m = k_none, l = 0.0f;
                 for (uint32_t j = 0; j < nt; j++) {
                     const uint32_t buf = tiles % BUFS, s_now = s_at + 64 * buf;
@@ -1183,7 +1183,7 @@ k_paged_attn_tiles(const __grid_constant__ CUtensorMap kmap, const __grid_consta
                     tc_wait_ld(sv);
                     if ((int) j * B_KEYS + B_KEYS - 1 > first_pos || (int) j * B_KEYS <= last_win) {
                         const int k0 = X.key0 + (int) j * B_KEYS, pos = X.pos0 + my_row() / L.G;
-                        const int seen = win ? max(0, X.pos0 - win + 1) : 0, kv = X.kv;
+                        const int seen = win ? max(0, max(X.pos0, 0) - win + 1) : 0, kv = X.kv;
                         const int hi = pos - k0, lo = win ? pos - win + 1 - k0 : 0;     // columns lo .. hi
 #pragma unroll
                         for (int i = 0; i < B_KEYS; i++)
@@ -2624,8 +2624,10 @@ int lnsb_paged_attn(const lnsb_paged_attn_args * a, lnsb_stream_t stream) {
     if (c.n_tokens == 0 || c.n_seqs == 0) return 0;
     if (a->q == nullptr || a->dst == nullptr || a->work == nullptr || a->work_bytes < lnsb_paged_attn_work_bytes())
         return LNSB_E_INVALID;
+    lnsb_paged_attn_args b = *a;
+    if (b.window >= c.max_kv) b.window = 0;     // hides no row; the kernels' windows are below 2^31
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    return c.type == LNSB_TYPE_F16 ? launch_attn<__half>(*a, s) : launch_attn<__nv_bfloat16>(*a, s);
+    return c.type == LNSB_TYPE_F16 ? launch_attn<__half>(b, s) : launch_attn<__nv_bfloat16>(b, s);
 }
 
 int lnsb_paged_errors(int64_t * bad_pages, int64_t * timeouts) {
