@@ -67,3 +67,43 @@ def test_window_with_rows_that_see_nothing(ks, work, heads, kv_heads, dim, windo
     _check(P, q, got, window)
     assert (got[:50] == 0).all() and (got[201:231] == 0).all() and (got[241:] == 0).all()
     assert ks.paged_errors() == (0, 0)
+
+
+# -------------------------------------------------------------- large scores
+
+@pytest.mark.parametrize("dtype,size", [(F16, 20000.0), (BF16, 1e6), (BF16, 1e15)])
+@pytest.mark.parametrize("dim", (64, 128, 32))
+@pytest.mark.parametrize("q", (1, 40, 300))
+def test_scores_of_any_size(ks, work, dtype, size, dim, q):
+    """scores far past 2^24, all apart by more than their rounding: each token takes the largest key it sees, whole;
+    rising, falling, and all of them far below zero"""
+    n, page = 700, 32
+    for lo, hi in ((-1.0, 1.0), (1.0, -1.0), (-1.0, -0.25), (-0.25, -1.0)):
+        P = ref.Paged([q], [n], 2, dim, page, dtype, seed=44)
+        # 700 steps of the type's own grid would not fit bfloat16's: 100 levels, and within one the keys are equal
+        level = torch.arange(n) // 7
+        ramp = (lo + (hi - lo) * level / 99.0) * size
+        for i in range(n):
+            P.k[P.host_table[0, i // page], i % page] = ramp[i].to(dtype).cuda()
+        qq = torch.full((q, 4, dim), size, dtype=dtype, device="cuda")
+        got = _attn(ks, work, P, qq)
+        _check(P, qq, got)
+    assert ks.paged_errors() == (0, 0)
+
+
+@pytest.mark.parametrize("dim", (64, 128, 32))
+@pytest.mark.parametrize("q", (1, 300))
+def test_large_scores_that_rise_slowly(ks, work, dim, q):
+    """scores near 1.5 2^27, where floats are 16 apart, rise by 16 (base 2) every 128 keys: the weights stay below
+    half's largest value"""
+    n, page = 1500, 32
+    P = ref.Paged([q], [n], 2, dim, page, F16, seed=45)
+    k = torch.zeros((n, 2, dim))
+    k[:, :, 0] = 12288.0
+    k[:, :, 1] = (torch.arange(n) // 128).float()[:, None]
+    for i in range(n):
+        P.k[P.host_table[0, i // page], i % page] = k[i].half().cuda()
+    qq = torch.zeros((q, 4, dim), dtype=F16, device="cuda")
+    qq[..., 0], qq[..., 1] = 16384.0, 16.0
+    scale = 0.6931471805599453                             # ln 2: the products are the scores to base 2
+    _check(P, qq, _attn(ks, work, P, qq, scale=scale), scale=scale)

@@ -293,7 +293,8 @@ k_paged_append_vec(paged P, const TI * __restrict__ k, const TI * __restrict__ v
 // the line, so the result does not hang on who came when.
 //
 // The maximum is a reference that moves only when a score passes it by more
-// than 8 (in log2): exp2 of the rest stays below 2^8, which both types hold,
+// than 8 (in log2; the difference of near floats is exact, a sum with 8 need
+// not be): exp2 of the rest stays below 2^8, which both types hold,
 // and the quotient does not see the reference.  The sum of the weights comes
 // from the same product as the output, against a column of ones, so it is of
 // the weights as rounded.
@@ -305,7 +306,7 @@ k_paged_append_vec(paged P, const TI * __restrict__ k, const TI * __restrict__ v
 constexpr int ROWS = 16, KEYS = 64, A_CTAS = 2 * k_sms;
 constexpr int MAX_DIM = 256;
 constexpr float k_lag = 8.0f;
-constexpr float k_none = -1e30f;               // the reference of a row that has seen nothing
+constexpr float k_none = -FLT_MAX;             // the reference of a row that has seen nothing
 
 // work: [counters A_CTAS int32][partials A_CTAS * 2 * (ROWS * MAX_DIM + 2 * ROWS) float]
 constexpr int64_t A_PART = ROWS * MAX_DIM + 2 * ROWS;
@@ -510,7 +511,7 @@ k_paged_attn_rows(paged P, const T * __restrict__ q, T * __restrict__ dst, const
                     sc[n][e] = key <= pos[i] && key >= lo[i] ? sc[n][e] * scale_log2 : -INFINITY;
                     top[i] = fmaxf(top[i], sc[n][e]);
                 }
-            if (__any_sync(0xFFFFFFFFu, top[0] > m[0] + k_lag || top[1] > m[1] + k_lag)) {
+            if (__any_sync(0xFFFFFFFFu, top[0] - m[0] > k_lag || top[1] - m[1] > k_lag)) {
 #pragma unroll
                 for (int i = 0; i < 2; i++) {
                     top[i] = fmaxf(top[i], __shfl_xor_sync(0xFFFFFFFFu, top[i], 1));
@@ -1209,7 +1210,7 @@ k_paged_attn_tiles(const __grid_constant__ CUtensorMap kmap, const __grid_consta
                         for (int e = 0; e < 4; e++)
                             t4[e] = max3(t4[e], __uint_as_float(sv[i + 2 * e]), __uint_as_float(sv[i + 2 * e + 1]));
                     const float top = fmaxf(max3(t4[0], t4[1], t4[2]), t4[3]) * scale_log2;
-                    if (__any_sync(0xFFFFFFFFu, top > m + k_lag)) {
+                    if (__any_sync(0xFFFFFFFFu, top - m > k_lag)) {
                         const float mn = fmaxf(m, top), f = ex2(m - mn);
                         m = mn;
                         l *= f;
@@ -1228,8 +1229,19 @@ k_paged_attn_tiles(const __grid_constant__ CUtensorMap kmap, const __grid_consta
                             }
                         }
                     }
+                    // past 2^22 the rounding of the reference's product, which the fused form puts into every exponent,
+                    // passes 1/4: the scores' products are then rounded as well, and the largest is the reference again
+                    float factor = scale_log2;
+                    if (__any_sync(0xFFFFFFFFu, fabsf(m) > 0x1p22f && fabsf(m) < FLT_MAX)) {
+                        if (fabsf(m) > 0x1p22f) {
+                            factor = 1.0f;
+#pragma unroll
+                            for (int i = 0; i < B_KEYS; i++) sv[i] = __float_as_uint(__uint_as_float(sv[i]) * scale_log2);
+                        }
+                        __syncwarp();
+                    }
                     float2 add[2] = { { 0, 0 }, { 0, 0 } };
-                    const float2 sc2 = make_float2(scale_log2, scale_log2), m2 = make_float2(-m, -m);
+                    const float2 sc2 = make_float2(factor, factor), m2 = make_float2(-m, -m);
 #pragma unroll
                     for (int i = 0; i < PARTS; i++) {
                         uint32_t pv[32];
