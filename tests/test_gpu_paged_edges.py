@@ -107,3 +107,37 @@ def test_large_scores_that_rise_slowly(ks, work, dim, q):
     qq[..., 0], qq[..., 1] = 16384.0, 16.0
     scale = 0.6931471805599453                             # ln 2: the products are the scores to base 2
     _check(P, qq, _attn(ks, work, P, qq, scale=scale), scale=scale)
+
+
+# -------------------------------------------------------- what is divided by
+
+@pytest.mark.parametrize("dtype,value", [(F16, 1.9990234375), (BF16, 1.9921875)])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(4, 2, 64), (4, 2, 128), (4, 2, 32)])
+@pytest.mark.parametrize("q", (1, 40, 300))
+@pytest.mark.parametrize("spread", (0.3, 1.5, 6.0))
+def test_equal_values_come_back(ks, work, dtype, value, heads, kv_heads, dim, q, spread):
+    """where all values are one number, every output is that number: the weights as they meet the values are what the
+    output is divided by, in chunks as for single tokens"""
+    P = ref.Paged([q, 1], [900, 333], kv_heads, dim, 16, dtype, seed=46)
+    for s in range(2):
+        for i in range(P.kv[s]):
+            P.v[P.host_table[s, i // 16], i % 16] = value
+    qq = _q(P, heads, dim, dtype, 47, spread)
+    assert (_attn(ks, work, P, qq) == value).all()
+
+
+@pytest.mark.parametrize("dtype,value,over", [(F16, 1.9990234375, 0.00064), (BF16, 1.9921875, 0.00505)])
+@pytest.mark.parametrize("dim", (64, 128, 32))
+@pytest.mark.parametrize("q", (1, 40))
+def test_one_heavy_weight_between_two_numbers(ks, work, dtype, value, over, dim, q):
+    """the same where nearly all weight is one key's, which is 2^7 and almost half a place against the maximum of the
+    tiles before it; enough sequences for several tiles to a CTA"""
+    n, page, seqs = 1024, 128, 64
+    P = ref.Paged([q] * seqs, [n] * seqs, 2, dim, page, dtype, seed=48)
+    P.k[:], P.v[:] = 0.0, value
+    P.k[..., 0] = -60.0
+    P.k[P.host_table[:, 0].long(), 0] = 0.0
+    P.k[P.host_table[:, 1].long(), 5, :, 0], P.k[P.host_table[:, 1].long(), 5, :, 1] = 7.0, over
+    qq = torch.zeros((q * seqs, 4, dim), dtype=dtype, device="cuda")
+    qq[..., :2] = 1.0
+    assert (_attn(ks, work, P, qq, scale=0.6931471805599453) == value).all()   # ln 2: base 2

@@ -39,6 +39,7 @@ template <> struct num<__half> {
         const __half2 h = __floats2half2_rn(lo, hi);
         return *reinterpret_cast<const uint32_t *>(&h);
     }
+    static __device__ __forceinline__ float2 unpack(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2 *>(&v)); }
     static constexpr uint32_t one2 = 0x3C003C00u;
 };
 template <> struct num<__nv_bfloat16> {
@@ -47,6 +48,9 @@ template <> struct num<__nv_bfloat16> {
     static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
         const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
         return *reinterpret_cast<const uint32_t *>(&h);
+    }
+    static __device__ __forceinline__ float2 unpack(uint32_t v) {
+        return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xFFFF0000u));
     }
     static constexpr uint32_t one2 = 0x3F803F80u;
 };
@@ -627,7 +631,9 @@ k_paged_attn_rows(paged P, const T * __restrict__ q, T * __restrict__ dst, const
 // S = Q K^T of a group lands in TMEM, one row a lane; the group's 128 threads
 // read one row each, so maximum and sum need no other thread, and write the
 // weights back into the same columns as the 16-bit A operand of P V, whose sum
-// O stays in TMEM.
+// O stays in TMEM.  They add up the weights as rounded, as the rows kernel does
+// (sums of the weights in 32 bits are 1-2 % faster, and off by a heavy weight's
+// rounding).
 //
 // Head dim 64 leaves TMEM for two S of 64 keys to each group: while its softmax
 // works on one, the next is ready, so it waits for no product (45 us where one
@@ -1249,9 +1255,8 @@ k_paged_attn_tiles(const __grid_constant__ CUtensorMap kmap, const __grid_consta
                         for (int e = 0; e < 32; e++) {
                             const float2 x = fma2(make_float2(__uint_as_float(sv[64 * i + 2 * e]), __uint_as_float(sv[64 * i + 2 * e + 1])),
                                                   sc2, m2);
-                            const float2 w = make_float2(ex2(x.x), ex2(x.y));
-                            add[e & 1] = add2(add[e & 1], w);
-                            pv[e] = num<T>::pack(w.x, w.y);
+                            pv[e] = num<T>::pack(ex2(x.x), ex2(x.y));
+                            add[e & 1] = add2(add[e & 1], num<T>::unpack(pv[e]));
                         }
                         tc_st32(s_now + 32 * i, pv);
                         tc_wait_st();
