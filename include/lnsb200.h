@@ -463,7 +463,7 @@ int lnsb_paged_append(const lnsb_paged_append_args * args, lnsb_stream_t stream)
  * q and dst are of the cache's type, rows 16-byte aligned (pointers, q_ld and
  * dst_ld multiples of 8).  Products and the softmax's sums are 32-bit floats;
  * the weights p are rounded to the cache's type for the product with v, and
- * their sum is that of the rounded ones.
+ * their sum is that of the rounded ones (F16: to 2^-32 of the largest).
  *
  * work: lnsb_paged_attn_work_bytes() bytes of device memory, 16-byte aligned,
  * zero before its first use; every call leaves it ready for the next.  Calls

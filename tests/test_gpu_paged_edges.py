@@ -141,3 +141,32 @@ def test_one_heavy_weight_between_two_numbers(ks, work, dtype, value, over, dim,
     qq = torch.zeros((q * seqs, 4, dim), dtype=dtype, device="cuda")
     qq[..., :2] = 1.0
     assert (_attn(ks, work, P, qq, scale=0.6931471805599453) == value).all()   # ln 2: base 2
+
+
+# ------------------------------------------------------------- light weights
+
+@pytest.mark.parametrize("dim", (64, 128, 32))
+@pytest.mark.parametrize("q", (1, 40, 300))
+@pytest.mark.parametrize("lo,hi", [(26.0, 26.0), (18.0, 30.0)])
+def test_many_light_weights_in_half(ks, work, dim, q, lo, hi):
+    """one key outweighs each of 20,000 others by 2^18 to 2^30; its value is 0, theirs is 1.  Half's last place below its
+    normal numbers is 2^-24, and the largest weight is 2^7 at least: a weight is off by 2^-32 of the largest, or by u.
+    64 sequences share the pages, so that a CTA takes many tiles"""
+    n, page, seqs = 20000, 1024, 64
+    P = ref.Paged([q], [n], 1, dim, page, F16, seed=49, junk=0.0)
+    g = torch.Generator().manual_seed(50)
+    P.k[:], P.v[:] = 0.0, 1.0
+    P.k[..., 0, 0] = -(lo + (hi - lo) * torch.rand(P.k.shape[:2], generator=g)).half().cuda()
+    first = P.host_table[0, 0].item()
+    P.k[first, 0], P.v[first, 0] = 0.0, 0.0
+    qq = torch.zeros((q, 2, dim), dtype=F16, device="cuda")
+    qq[..., 0] = 1.0
+    scale = 0.6931471805599453                             # ln 2: base 2
+    want, mag = ref.attention(P, qq, scale)
+    u = ref.UNIT[F16]
+    bound = (2 * u + 2.0 ** -12) * mag * 1.01 + u * want.abs() * 1.01 + n * 2.0 ** -32 + 2.0 ** -24
+    P.table, P.kv_len = P.table.repeat(seqs, 1), P.kv_len.repeat(seqs)
+    P.q_start = torch.arange(seqs + 1, dtype=torch.int32, device="cuda") * q
+    got = _attn(ks, work, P, qq.repeat(seqs, 1, 1), scale=scale).view(seqs, q, 2, dim).double()
+    assert float(want.min()) > 1e-4
+    assert ((got - want).abs() <= bound).all(), float(((got - want).abs() / bound).max())

@@ -41,6 +41,7 @@ template <> struct num<__half> {
     }
     static __device__ __forceinline__ float2 unpack(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2 *>(&v)); }
     static constexpr uint32_t one2 = 0x3C003C00u;
+    static constexpr float head = 7.0f;         // the largest weight is 2^7 at least, where its reference is set
 };
 template <> struct num<__nv_bfloat16> {
     static __device__ __forceinline__ float to(__nv_bfloat16 v) { return __bfloat162float(v); }
@@ -53,6 +54,7 @@ template <> struct num<__nv_bfloat16> {
         return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xFFFF0000u));
     }
     static constexpr uint32_t one2 = 0x3F803F80u;
+    static constexpr float head = 0.0f;
 };
 
 // two floats in one instruction
@@ -298,8 +300,10 @@ k_paged_append_vec(paged P, const TI * __restrict__ k, const TI * __restrict__ v
 //
 // The maximum is a reference that moves only when a score passes it by more
 // than 8 (in log2; the difference of near floats is exact, a sum with 8 need
-// not be): exp2 of the rest stays below 2^8, which both types hold,
-// and the quotient does not see the reference.  The sum of the weights comes
+// not be): exp2 of the rest stays below 2^8, and the quotient does not see the
+// reference.  Half's numbers end at 2^-24, where BF16's go on: there it is 7
+// below the score that sets it, so that weights down to 2^-32 of the largest
+// count, and none passes 2^15.  The sum of the weights comes
 // from the same product as the output, against a column of ones, so it is of
 // the weights as rounded.
 //
@@ -388,6 +392,7 @@ k_paged_attn_rows(paged P, const T * __restrict__ q, T * __restrict__ dst, const
                   const T * __restrict__ vc, int64_t q_ld, int64_t dst_ld, int G, float scale_log2, int64_t window,
                   int64_t rows_most, int * __restrict__ counters, float * __restrict__ parts) {
     constexpr int ST = a_stages<D>(), SB = a_stage_bytes<D>(), CPR = D / 8, KS = D / 16;
+    constexpr float head = num<T>::head, lag = k_lag + head;
     extern __shared__ __align__(128) unsigned char sm[];
     __shared__ int64_t s_scan[128];
     __shared__ int s_last;
@@ -512,15 +517,15 @@ k_paged_attn_rows(paged P, const T * __restrict__ q, T * __restrict__ dst, const
                 for (int e = 0; e < 4; e++) {
                     const int64_t key = k0 + n * 8 + (lane % 4) * 2 + (e & 1);
                     const int i = e >> 1;
-                    sc[n][e] = key <= pos[i] && key >= lo[i] ? sc[n][e] * scale_log2 : -INFINITY;
+                    sc[n][e] = key <= pos[i] && key >= lo[i] ? __fmul_rn(sc[n][e], scale_log2) : -INFINITY;
                     top[i] = fmaxf(top[i], sc[n][e]);
                 }
-            if (__any_sync(0xFFFFFFFFu, top[0] - m[0] > k_lag || top[1] - m[1] > k_lag)) {
+            if (__any_sync(0xFFFFFFFFu, top[0] - m[0] > lag || top[1] - m[1] > lag)) {
 #pragma unroll
                 for (int i = 0; i < 2; i++) {
                     top[i] = fmaxf(top[i], __shfl_xor_sync(0xFFFFFFFFu, top[i], 1));
                     top[i] = fmaxf(top[i], __shfl_xor_sync(0xFFFFFFFFu, top[i], 2));
-                    const float mn = fmaxf(m[i], top[i]), f = ex2(m[i] - mn);
+                    const float mn = fmaxf(m[i], top[i] - head), f = ex2(m[i] - mn);
                     m[i] = mn;
                     l[2 * i] *= f;
 #pragma unroll
@@ -897,6 +902,7 @@ k_paged_attn_tiles(const __grid_constant__ CUtensorMap kmap, const __grid_consta
     constexpr int B_KEYS = b_keys<D>(), BUFS = D == 128 ? 1 : 2, PARTS = B_KEYS / 64;
     constexpr int ST = b_ring<D>(), TB = b_tile_bytes<D>(), HB = B_KEYS * 128, QB = b_q_bytes<D>(), QH = B_ROWS * 128, HALVES = D / 64;
     constexpr bool BF = std::is_same<T, __nv_bfloat16>::value;
+    constexpr float head = num<T>::head, lag = k_lag + head;
     // f32 sums of 16-bit operands, 128 rows; B of PV is [key][dim], keys outside
     constexpr uint32_t fmt = (1u << 4) | ((BF ? 1u : 0u) << 7) | ((BF ? 1u : 0u) << 10) | (8u << 24);
     constexpr uint32_t idesc_qk = fmt | ((B_KEYS / 8) << 17), idesc_pv = fmt | (1u << 16) | ((D / 8) << 17);
@@ -1215,9 +1221,9 @@ k_paged_attn_tiles(const __grid_constant__ CUtensorMap kmap, const __grid_consta
 #pragma unroll
                         for (int e = 0; e < 4; e++)
                             t4[e] = max3(t4[e], __uint_as_float(sv[i + 2 * e]), __uint_as_float(sv[i + 2 * e + 1]));
-                    const float top = fmaxf(max3(t4[0], t4[1], t4[2]), t4[3]) * scale_log2;
-                    if (__any_sync(0xFFFFFFFFu, top - m > k_lag)) {
-                        const float mn = fmaxf(m, top), f = ex2(m - mn);
+                    const float top = __fmul_rn(fmaxf(max3(t4[0], t4[1], t4[2]), t4[3]), scale_log2);     // rounded: never fused
+                    if (__any_sync(0xFFFFFFFFu, top - m > lag)) {
+                        const float mn = fmaxf(m, top - head), f = ex2(m - mn);
                         m = mn;
                         l *= f;
                         if (j > 0) {
@@ -1242,7 +1248,7 @@ k_paged_attn_tiles(const __grid_constant__ CUtensorMap kmap, const __grid_consta
                         if (fabsf(m) > 0x1p22f) {
                             factor = 1.0f;
 #pragma unroll
-                            for (int i = 0; i < B_KEYS; i++) sv[i] = __float_as_uint(__uint_as_float(sv[i]) * scale_log2);
+                            for (int i = 0; i < B_KEYS; i++) sv[i] = __float_as_uint(__fmul_rn(__uint_as_float(sv[i]), scale_log2));
                         }
                         __syncwarp();
                     }
