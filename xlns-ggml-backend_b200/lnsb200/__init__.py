@@ -266,12 +266,17 @@ class KernelSet:
         if not (v.shape == k.shape and v.dtype is ty and ty in _type_ids and kv[15] == n_head_kv and kv[16] == D
                 and _rows_ok(ks, n_head_kv, D) and _rows_ok(vs, n_head_kv, D)):
             raise ValueError("k and v must be [n_tokens][n_head_kv][head_dim] of one type (F32, F16, BF16), heads contiguous")
+        dev = k_cache.get_device()
+        if not dev == k.get_device() == v.get_device():
+            raise ValueError(_elsewhere)
         cs = qp = op = None
         n_dims = n_head = q_ld = o_ld = 0
         if cos_sin is not None:
             rows, half, two = cos_sin.shape
             if not (cos_sin.dtype is _f32 and two == 2 and rows >= max_kv and cos_sin.is_contiguous()):
                 raise ValueError("cos_sin must be contiguous F32 [rows >= max_kv][n_dims / 2][2]")
+            if cos_sin.get_device() != dev:
+                raise ValueError(_elsewhere)
             n_dims, cs = 2 * half, cos_sin.data_ptr() if half else None
         if q is not None:
             n, n_head, d = q.shape
@@ -279,6 +284,8 @@ class KernelSet:
             if not (q_out is not None and q_out.shape == q.shape and q.dtype is ty and q_out.dtype is k_cache.dtype and n == T
                     and d == D and _rows_ok(qs, n_head, D) and _rows_ok(qos, n_head, D)):
                 raise ValueError("q must be [n_tokens][n_head][head_dim] of k's type, q_out the same of the caches' type")
+            if not dev == q.get_device() == q_out.get_device():
+                raise ValueError(_elsewhere)
             q_ld, o_ld, qp, op = _ld(qs, T, n_head, D), _ld(qos, T, n_head, D), q.data_ptr(), q_out.data_ptr()
         a = _lib.PagedAppendArgs(*kv, k.data_ptr(), v.data_ptr(), qp, op, cs, _ld(ks, T, n_head_kv, D), _ld(vs, T, n_head_kv, D),
                                  q_ld, o_ld, _type_ids[ty], n_head, n_dims, 1 if neox else 0)
@@ -301,6 +308,8 @@ class KernelSet:
         if not (q.dtype is ty and dst.dtype is ty and dst.shape == q.shape and kv[16] == D and _rows_ok(qs, n_head, D)
                 and _rows_ok(ds, n_head, D)):
             raise ValueError("q and dst must be [n_tokens][n_head][head_dim] of the caches' type, heads contiguous")
+        if not k_cache.get_device() == q.get_device() == dst.get_device() == work.get_device():
+            raise ValueError(_elsewhere)
         a = _lib.PagedAttnArgs(*kv, q.data_ptr(), dst.data_ptr(), work.data_ptr(), work.nbytes, _ld(qs, T, n_head, D),
                                _ld(ds, T, n_head, D), max_q, window, n_head, D ** -0.5 if scale is None else scale)
         st = self.lib.lnsb_paged_attn(ctypes.byref(a), _raw_stream(stream))
@@ -323,9 +332,13 @@ class KernelSet:
         ld, step = logits.stride()
         if not ((step == 1 or V == 1) and logits.dtype in _type_ids):
             raise ValueError("logits must be F32, F16 or BF16 with contiguous rows")
-        a = _lib.SampleArgs(logits.data_ptr(), _row_ptr(temperature, _f32, R), _row_ptr(top_k, _i32, R), _row_ptr(top_p, _f32, R),
-                            _row_ptr(min_p, _f32, R), _row_ptr(u, _f32, R), _row_ptr(token, _i32, R), _row_ptr(prob, _f32, R),
-                            ld if R > 1 else V, R, V, _type_ids[logits.dtype])
+        d = logits.get_device()
+        a = _lib.SampleArgs(logits.data_ptr(), _row_ptr(temperature, _f32, R, d), _row_ptr(top_k, _i32, R, d),
+                            _row_ptr(top_p, _f32, R, d), _row_ptr(min_p, _f32, R, d), _row_ptr(u, _f32, R, d),
+                            _row_ptr(token, _i32, R, d), _row_ptr(prob, _f32, R, d), ld if R > 1 else V, R, V,
+                            _type_ids[logits.dtype])
+        if d < 0 or d != _current_device():
+            raise ValueError(_elsewhere)
         st = self.lib.lnsb_sample(ctypes.byref(a), _raw_stream(stream))
         if st:
             _lib.check(self.lib, "lnsb_sample", st)
@@ -333,16 +346,17 @@ class KernelSet:
 
 # torch's types, looked up at the first use (the module itself does not import torch)
 _type_ids = {}
-_f32 = _i32 = _current_stream = None
+_f32 = _i32 = _current_stream = _current_device = None
 
 
 def _load_types():
-    global _f32, _i32, _current_stream
+    global _f32, _i32, _current_stream, _current_device
     import torch
     try:                                # the same handle without a Stream object: 0.2 us, not 3
         raw, device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
-        _current_stream = lambda: raw(device())  # noqa: E731
+        _current_stream, _current_device = lambda: raw(device()), device
     except AttributeError:
+        _current_device = torch.cuda.current_device
         _current_stream = lambda: torch.cuda.current_stream().cuda_stream  # noqa: E731
     _f32, _i32 = torch.float32, torch.int32
     _type_ids.update({_f32: _lib.TYPES["f32"], torch.float16: _lib.TYPES["f16"], torch.bfloat16: _lib.TYPES["bf16"]})
@@ -363,11 +377,16 @@ def _ld(st, tokens, heads, D):
     return st[0] if tokens > 1 else heads * D
 
 
-def _row_ptr(t, dtype, rows):
+_elsewhere = "every tensor must be on the current CUDA device"
+
+
+def _row_ptr(t, dtype, rows, dev):
     if t is None:
         return None
     if not (t.dtype is dtype and t.numel() == rows and t.is_contiguous()):
         raise ValueError("u, prob, temperature, top_p, min_p must be F32 [n_rows], token and top_k int32 [n_rows]")
+    if t.get_device() != dev:
+        raise ValueError(_elsewhere)
     return t.data_ptr()
 
 
@@ -384,6 +403,10 @@ def _paged_kv(k_cache, v_cache, page_table, q_start, kv_len, max_kv, n_tokens):
     if not (page_table.dtype is _i32 and q_start.dtype is _i32 and kv_len.dtype is _i32 and q_start.numel() == n_seqs + 1
             and kv_len.numel() == n_seqs and page_table.is_contiguous() and q_start.is_contiguous() and kv_len.is_contiguous()):
         raise ValueError("page_table [n_seqs][pages], q_start [n_seqs + 1] and kv_len [n_seqs] must be contiguous int32")
+    dev = k_cache.get_device()
+    if not (0 <= dev == v_cache.get_device() == page_table.get_device() == q_start.get_device() == kv_len.get_device()
+            and dev == _current_device()):
+        raise ValueError(_elsewhere)
     return (k_cache.data_ptr(), v_cache.data_ptr(), st[0], st[1], st[2], page_table.data_ptr(), q_start.data_ptr(),
             kv_len.data_ptr(), table_ld, n_pages, n_tokens, max_kv, n_seqs, _type_ids[ty], page_size, n_head_kv, head_dim, 0)
 
