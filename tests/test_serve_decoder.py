@@ -1,0 +1,168 @@
+"""The paged decoder's host side, on the CPU: a model's ops and kernels are stand-ins that write down what they are given
+and on which stream."""
+import contextlib
+
+import pytest
+import torch
+
+from lnsb200.serve import PagedDecoder
+
+CFG = dict(n_layer=2, n_embd=8, n_head=2, n_head_kv=1, head_dim=4, n_ff=8, vocab=11, eps=1e-5)
+
+
+class Stream:
+    def __init__(self, name, log):
+        self.name, self.log = name, log
+
+    def wait_stream(self, other):
+        self.log.append(("wait", self.name, other.name))
+
+
+class Cuda:
+    """torch.cuda's part in it: which stream is current"""
+
+    def __init__(self, log):
+        self.now, self.log = Stream("current", log), log
+
+    def current_stream(self, device=None):
+        return self.now
+
+    @contextlib.contextmanager
+    def stream(self, s):
+        before, self.now = self.now, s
+        try:
+            yield
+        finally:
+            self.now = before
+
+
+class Torch:
+    """torch, with each call that makes or moves device data written down with the stream it runs on"""
+
+    def __init__(self, log):
+        self.cuda, self.log = Cuda(log), log
+
+    def __getattr__(self, name):
+        v = getattr(torch, name)
+        if name in ("tensor", "as_tensor", "empty", "empty_like", "zeros", "rand"):
+            def call(*a, **kw):
+                self.log.append((name, self.cuda.now.name))
+                return v(*a, **kw)
+            return call
+        return v
+
+
+class Kernels:
+    def __init__(self, ops):
+        self.ops, self.log = ops, ops.log
+
+    def paged_attn_work(self, device=None):
+        self.log.append(("work", self.ops.torch.cuda.now.name))
+        return torch.zeros(64, dtype=torch.uint8)
+
+    def _call(self, name, stream):
+        now = self.ops.torch.cuda.now
+        self.log.append((name, (stream or now).name))
+        assert stream in (None, now)
+        if name == self.ops.fail:
+            raise RuntimeError("out of memory")
+
+    def paged_append(self, k, v, kc, vc, table, q_start, kv_len, max_kv, q=None, q_out=None, cos_sin=None, stream=None):
+        self._call("append", stream)
+        self.ops.plans.append((table.tolist(), q_start.tolist(), kv_len.tolist()))
+
+    def paged_attn(self, q, kc, vc, table, q_start, kv_len, max_q, max_kv, dst, work, stream=None):
+        self._call("attn", stream)
+        dst.zero_()
+
+    def f16_to_f32(self, src, dst, n, stream=None):
+        self._call("to f32", stream)
+        dst.copy_(src.view(dst.shape))
+
+    def sample(self, logits, u, token, prob, t, k, p, m, stream=None):
+        self._call("sample", stream)
+        token.copy_(logits.argmax(1))
+        prob.fill_(1.0)
+
+
+class Ops:
+    def __init__(self, stream=None, n_ctx=32):
+        self.log, self.plans, self.fail = [], [], None
+        self.torch, self.cfg, self.n_ctx, self.dev = Torch(self.log), CFG, n_ctx, torch.device("cpu")
+        self.stream = Stream(stream, self.log) if stream else None
+        self.rope_cs, self.ks = torch.zeros(n_ctx, 2, 2), Kernels(self)
+
+    def _op(self, name, out):
+        self.log.append((name, self.torch.cuda.now.name))
+        if name == self.fail:
+            raise RuntimeError("out of memory")
+        return out
+
+    def embed(self, ids):
+        assert all(0 <= i < CFG["vocab"] for i in ids)
+        return self._op("embed", torch.zeros(len(ids), CFG["n_embd"]))
+
+    def w(self, il, name):
+        return name
+
+    def rms_norm(self, x, eps, name=None):
+        return self._op("norm", x.clone())
+
+    def mul(self, x, w):
+        return self._op("mul", x.clone())
+
+    def add(self, a, b):
+        return self._op("add", a + b)
+
+    def swiglu(self, gate, up):
+        return self._op("swiglu", gate * up)
+
+    def linear(self, w, x, name=None, src=None):
+        out = torch.zeros(x.shape[0], CFG["vocab"] if w == "output" else CFG["n_embd"])
+        out[:, 3] = 1.0
+        return self._op("linear", out)
+
+    def linears(self, il, ws, x, names=None, src=None):
+        n = {"wq": 8, "wk": 4, "wv": 4, "w_up": 8, "w_gate": 8}
+        return [self._op("linears", torch.zeros(x.shape[0], n[w])) for w in ws]
+
+
+# -------------------------------------------------------------------- streams
+
+def _ran(log):
+    return {e[1] for e in log if e[0] != "wait"}
+
+
+@pytest.mark.parametrize("u", (None, [0.5, 0.5]))
+def test_everything_runs_on_the_models_stream(u):
+    """kernels, copies, random numbers and allocations: a tensor made, read or freed on another stream would not be
+    ordered with the kernels"""
+    ops = Ops("side")
+    dec = PagedDecoder(ops, n_pages=8, page_size=4)
+    a, b = dec.open(), dec.open()
+    assert dec.step([(a, [1, 2, 3]), (b, [4])], u=u, temperature=[0.5, 0.7], top_p=0.9) == [3, 3]
+    assert _ran(ops.log) == {"side"}
+    # the model's stream waits for the current one before the step's first work, and the current one for it behind the last
+    work = [i for i, e in enumerate(ops.log) if e[0] != "wait"]
+    first, last = ops.log.index(("embed", "side")), work[-1]
+    assert ("wait", "side", "current") in ops.log[:first]
+    assert ("wait", "current", "side") in ops.log[last:]
+    assert ops.torch.cuda.now.name == "current"
+
+
+def test_the_stream_is_left_after_an_error():
+    ops = Ops("side")
+    dec = PagedDecoder(ops, n_pages=8, page_size=4)
+    a = dec.open()
+    ops.fail = "attn"
+    with pytest.raises(RuntimeError, match="out of memory"):
+        dec.step([(a, [1, 2])])
+    assert ops.torch.cuda.now.name == "current" and ops.log[-1] == ("wait", "current", "side")
+
+
+def test_without_a_stream_the_current_one():
+    ops = Ops()
+    dec = PagedDecoder(ops, n_pages=8, page_size=4)
+    a = dec.open()
+    assert dec.step([(a, [1, 2, 3])]) == [3]
+    assert _ran(ops.log) == {"current"} and not [e for e in ops.log if e[0] == "wait"]

@@ -13,6 +13,8 @@ host takes out of LNS with LNS_DISABLE_OPS=rope,kq,kq_soft_max,kqv), through
     tokens = dec.step([(s, p) for s, p in zip(seqs, prompts)], temperature=0.8, top_p=0.95)
     tokens = dec.step([(s, [t]) for s, t in zip(seqs, tokens)], temperature=0.8, top_p=0.95)
 """
+import contextlib
+
 __all__ = ["PagePool", "PagedDecoder"]
 
 
@@ -54,17 +56,40 @@ class PagePool:
 
 class PagedDecoder:
     """One cache per layer and one pool of pages over a model's ops (`model.GpuOps`); the rotation's table bounds a
-    sequence's length (ops.n_ctx)."""
+    sequence's length (ops.n_ctx).  All device work runs on the ops' stream, between what the caller's current stream
+    was given before a call and what it is given after it; the ops without one use the current stream."""
 
     def __init__(self, ops, n_pages, page_size=16):
         torch, cfg = ops.torch, ops.cfg
         self.ops, self.cfg, self.ks, self.torch = ops, cfg, ops.ks, torch
         self.pool = PagePool(n_pages, page_size)
         shape = (n_pages, page_size, cfg["n_head_kv"], cfg["head_dim"])
-        # zeros: rows that no sequence has written are never seen, but a reader of the cache may look
-        self.kc = [torch.zeros(shape, dtype=torch.float16, device=ops.dev) for _ in range(cfg["n_layer"])]
-        self.vc = [torch.zeros(shape, dtype=torch.float16, device=ops.dev) for _ in range(cfg["n_layer"])]
-        self.work = self.ks.paged_attn_work(ops.dev)
+        with self._on_stream():
+            # zeros: rows that no sequence has written are never seen, but a reader of the cache may look
+            self.kc = [torch.zeros(shape, dtype=torch.float16, device=ops.dev) for _ in range(cfg["n_layer"])]
+            self.vc = [torch.zeros(shape, dtype=torch.float16, device=ops.dev) for _ in range(cfg["n_layer"])]
+            self.work = self.ks.paged_attn_work(ops.dev)
+
+    @contextlib.contextmanager
+    def _on_stream(self):
+        """the ops' stream, behind the current one's work and before its next"""
+        cuda, mine = self.torch.cuda, self.ops.stream
+        now = None if mine is None else cuda.current_stream(self.ops.dev)
+        if mine is None or mine == now:
+            yield
+            return
+        mine.wait_stream(now)
+        try:
+            with cuda.stream(mine):
+                yield
+        finally:
+            now.wait_stream(mine)
+
+    def _handed_over(self, *tensors):
+        """tensors of the ops' stream that the caller's current stream will read"""
+        for t in tensors:
+            if t.is_cuda:
+                t.record_stream(self.torch.cuda.current_stream(self.ops.dev))
 
     def open(self):
         return self.pool.open()
@@ -77,6 +102,12 @@ class PagedDecoder:
 
     def forward(self, batch):
         """logits (F32, [len(batch)][vocab]) of the last of the new tokens of each (sequence, tokens) of `batch`"""
+        with self._on_stream():
+            logits = self._forward(batch)
+        self._handed_over(logits)
+        return logits
+
+    def _forward(self, batch):
         torch, ops, cfg, ks, stream = self.torch, self.ops, self.cfg, self.ks, self.ops.stream
         H, HKV, D = cfg["n_head"], cfg["n_head_kv"], cfg["head_dim"]
         if not batch or any(len(t) == 0 for _, t in batch):
@@ -118,11 +149,13 @@ class PagedDecoder:
         u: the random numbers, or None to draw them"""
         torch, n = self.torch, logits.shape[0]
         each = lambda v, t: torch.as_tensor(v, dtype=t, device=self.ops.dev).expand(n).contiguous()  # noqa: E731
-        u = torch.rand(n, device=self.ops.dev) if u is None else each(u, torch.float32)
-        token = torch.empty(n, dtype=torch.int32, device=self.ops.dev)
-        prob = torch.empty(n, dtype=torch.float32, device=self.ops.dev)
-        self.ks.sample(logits, u, token, prob, each(temperature, torch.float32), each(top_k, torch.int32),
-                       each(top_p, torch.float32), each(min_p, torch.float32), stream=self.ops.stream)
+        with self._on_stream():
+            u = torch.rand(n, device=self.ops.dev) if u is None else each(u, torch.float32)
+            token = torch.empty(n, dtype=torch.int32, device=self.ops.dev)
+            prob = torch.empty(n, dtype=torch.float32, device=self.ops.dev)
+            self.ks.sample(logits, u, token, prob, each(temperature, torch.float32), each(top_k, torch.int32),
+                           each(top_p, torch.float32), each(min_p, torch.float32), stream=self.ops.stream)
+        self._handed_over(token, prob)
         return token, prob
 
     def step(self, batch, u=None, **sampling):
