@@ -166,3 +166,53 @@ def test_without_a_stream_the_current_one():
     a = dec.open()
     assert dec.step([(a, [1, 2, 3])]) == [3]
     assert _ran(ops.log) == {"current"} and not [e for e in ops.log if e[0] == "wait"]
+
+
+# ------------------------------------------------------ a step that goes wrong
+
+def _state(dec):
+    p = dec.pool
+    return dict(p.length), {s: list(v) for s, v in p.pages.items()}, list(p.free)
+
+
+@pytest.mark.parametrize("fail", ("embed", "norm", "mul", "linears", "append", "attn", "to f32", "linear", "add", "swiglu", "sample"))
+def test_a_failed_step_leaves_the_pool(fail):
+    """whatever call raises: the sequences keep their rows and pages, and the step can be taken again, in smaller pieces"""
+    ops = Ops()
+    dec = PagedDecoder(ops, n_pages=8, page_size=4)
+    a, b = dec.open(), dec.open()
+    dec.step([(a, [1, 2, 3]), (b, [4])])
+    before = _state(dec)
+    ops.fail = fail
+    with pytest.raises(RuntimeError, match="out of memory"):
+        dec.step([(a, [5, 6, 7, 8, 9, 1]), (b, [2, 3, 4, 5])])
+    assert _state(dec) == before
+    ops.fail, ops.plans = None, []
+    assert dec.step([(b, [2, 3])]) == [3]
+    table, q_start, kv_len = ops.plans[0]
+    assert q_start == [0, 2] and kv_len == [3] and table == [dec.pool.pages[b]]
+    assert dec.pool.length == {a: 3, b: 3}
+
+
+@pytest.mark.parametrize("bad", (dict(u=[0.1, 0.2]), dict(top_k="many"), dict(temperature=[1.0, 2.0, 3.0])), ids=str)
+def test_parameters_that_do_not_fit_leave_the_pool(bad):
+    dec = PagedDecoder(Ops(), n_pages=8, page_size=4)
+    seqs = [dec.open(), dec.open(), dec.open(), dec.open()]
+    before = _state(dec)
+    with pytest.raises((RuntimeError, ValueError, TypeError)):
+        dec.step([(s, [1, 2]) for s in seqs], **bad)
+    assert _state(dec) == before
+
+
+def test_forward_alone_too():
+    ops = Ops()
+    dec = PagedDecoder(ops, n_pages=8, page_size=4)
+    a = dec.open()
+    before = _state(dec)
+    ops.fail = "attn"
+    with pytest.raises(RuntimeError):
+        dec.forward([(a, [1, 2, 3, 4, 5])])
+    assert _state(dec) == before
+    ops.fail = None
+    assert dec.forward([(a, [1, 2, 3, 4, 5])]).shape == (1, CFG["vocab"])
+    assert dec.pool.length == {a: 5}

@@ -49,6 +49,13 @@ class PagePool:
                 self.pages[s].append(self.free.pop())
             self.length[s] += n
 
+    def shrink(self, grown):
+        """takes a grow back: the last n rows of each (sequence, n), and the pages that held nothing else"""
+        for s, n in reversed(grown):
+            self.length[s] -= n
+            while len(self.pages[s]) > -(-self.length[s] // self.page_size):
+                self.free.append(self.pages[s].pop())
+
     def close(self, s):
         self.free.extend(reversed(self.pages.pop(s)))
         del self.length[s]
@@ -100,22 +107,41 @@ class PagedDecoder:
     def _i32(self, v):
         return self.torch.tensor(v, dtype=self.torch.int32, device=self.ops.dev)
 
+    def _grow(self, batch):
+        """room in the pool for the new tokens of a batch"""
+        if not batch or any(len(t) == 0 for _, t in batch):
+            raise ValueError("every sequence of a batch needs a token")
+        if any(self.pool.length.get(s, 0) + len(t) > self.ops.n_ctx for s, t in batch):
+            raise ValueError("a sequence would pass %d rows" % self.ops.n_ctx)
+        grown = [(s, len(t)) for s, t in batch]
+        self.pool.grow(grown)
+        return grown
+
+    @contextlib.contextmanager
+    def _or_shrink(self, grown):
+        """the rows of a step that raises are not the sequences': the next step writes them anew"""
+        try:
+            yield
+        except BaseException:
+            self.pool.shrink(grown)
+            raise
+
     def forward(self, batch):
-        """logits (F32, [len(batch)][vocab]) of the last of the new tokens of each (sequence, tokens) of `batch`"""
+        """logits (F32, [len(batch)][vocab]) of the last of the new tokens of each (sequence, tokens) of `batch`; if it
+        raises, the sequences are as they were"""
+        with self._or_shrink(self._grow(batch)):
+            return self._forward(batch)
+
+    def _forward(self, batch):
         with self._on_stream():
-            logits = self._forward(batch)
+            logits = self._graph(batch)
         self._handed_over(logits)
         return logits
 
-    def _forward(self, batch):
+    def _graph(self, batch):
         torch, ops, cfg, ks, stream = self.torch, self.ops, self.cfg, self.ks, self.ops.stream
         H, HKV, D = cfg["n_head"], cfg["n_head_kv"], cfg["head_dim"]
-        if not batch or any(len(t) == 0 for _, t in batch):
-            raise ValueError("every sequence of a batch needs a token")
         pool = self.pool
-        if any(pool.length.get(s, 0) + len(t) > ops.n_ctx for s, t in batch):
-            raise ValueError("a sequence would pass %d rows" % ops.n_ctx)
-        pool.grow([(s, len(t)) for s, t in batch])
         start = [0]
         for _, t in batch:
             start.append(start[-1] + len(t))
@@ -159,5 +185,7 @@ class PagedDecoder:
         return token, prob
 
     def step(self, batch, u=None, **sampling):
-        """forward, then sample: the next token of each sequence of the batch, on the host"""
-        return self.sample(self.forward(batch), u, **sampling)[0].tolist()
+        """forward, then sample: the next token of each sequence of the batch, on the host; if it raises, the sequences
+        are as they were"""
+        with self._or_shrink(self._grow(batch)):
+            return self.sample(self._forward(batch), u, **sampling)[0].tolist()
