@@ -216,3 +216,18 @@ def test_forward_alone_too():
     ops.fail = None
     assert dec.forward([(a, [1, 2, 3, 4, 5])]).shape == (1, CFG["vocab"])
     assert dec.pool.length == {a: 5}
+
+
+# ------------------------------------------------------------------ token ids
+
+@pytest.mark.parametrize("ids", ([-1], [1, CFG["vocab"]], [2 ** 40, 1], [3, -2 ** 31]), ids=str)
+def test_tokens_outside_the_vocabulary(ids):
+    """refused on the host before anything grows or runs: -1 is what a row without a finite logit samples"""
+    ops = Ops()
+    dec = PagedDecoder(ops, n_pages=8, page_size=4)
+    a, b = dec.open(), dec.open()
+    before, log = _state(dec), list(ops.log)
+    for call in (dec.step, dec.forward):
+        with pytest.raises(ValueError, match="vocab"):
+            call([(b, [1]), (a, ids)])
+    assert _state(dec) == before and ops.log == log

@@ -111,6 +111,9 @@ class PagedDecoder:
         """room in the pool for the new tokens of a batch"""
         if not batch or any(len(t) == 0 for _, t in batch):
             raise ValueError("every sequence of a batch needs a token")
+        vocab = self.cfg["vocab"]
+        if any(not 0 <= i < vocab for _, t in batch for i in t):     # -1: a row without a logit above -inf sampled it
+            raise ValueError("a token is outside the vocabulary of %d" % vocab)
         if any(self.pool.length.get(s, 0) + len(t) > self.ops.n_ctx for s, t in batch):
             raise ValueError("a sequence would pass %d rows" % self.ops.n_ctx)
         grown = [(s, len(t)) for s, t in batch]
