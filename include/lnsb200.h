@@ -484,7 +484,8 @@ int lnsb_paged_attn(const lnsb_paged_attn_args * args, lnsb_stream_t stream);
 int64_t lnsb_paged_attn_work_bytes(void);
 
 /* since the last call, on the current device: page ids outside the cache met
- * by lnsb_paged_append and lnsb_paged_attn, and waits inside lnsb_paged_attn
+ * by lnsb_paged_append (one for each token) and lnsb_paged_attn (one at least
+ * for each such page that a call reads), and waits inside lnsb_paged_attn
  * that ran out (its output is then invalid, and its work has to be zeroed
  * again); either may be NULL.  Reads and
  * clears both counts (synchronises with the device). */

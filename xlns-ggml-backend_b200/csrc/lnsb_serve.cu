@@ -104,10 +104,10 @@ __device__ __forceinline__ seq_span span_of(const paged & P, int s) {
     return { a, b - a, min(max((int64_t) P.kv_len[s], (int64_t) 0), P.max_kv) };
 }
 // page id of a row below kv_len, or -1 (counted) for one outside the cache
-__device__ __forceinline__ int64_t page_of(const paged & P, int s, int64_t row) {
+__device__ __forceinline__ int64_t page_of(const paged & P, int s, int64_t row, bool count = true) {
     const int64_t id = P.table[s * P.table_ld + (row >> P.page_shift)];
     if (id >= 0 && id < P.n_pages) return id;
-    atomicAdd(&g_paged_errors[0], 1ull);
+    if (count) atomicAdd(&g_paged_errors[0], 1ull);
     return -1;
 }
 
@@ -141,7 +141,7 @@ __global__ void k_paged_append(paged P, const TI * __restrict__ k, const TI * __
         const bool to_cache = is_v || h >= n_head;
         int64_t at = 0;
         if (to_cache) {
-            const int64_t id = page_of(P, lo, row);
+            const int64_t id = page_of(P, lo, row, r == n_head * per);      // counted by the token's first key element
             if (id < 0) continue;
             at = id * P.page_stride + (row & ((1 << P.page_shift) - 1)) * P.row_stride +
                  (is_v ? h : h - n_head) * P.head_stride;
