@@ -487,8 +487,8 @@ int64_t lnsb_paged_attn_work_bytes(void);
  * by lnsb_paged_append (one for each token) and lnsb_paged_attn (one at least
  * for each such page that a call reads), and waits inside lnsb_paged_attn
  * that ran out (its output is then invalid, and its work has to be zeroed
- * again); either may be NULL.  Reads and
- * clears both counts (synchronises with the device). */
+ * again); either may be NULL.  Hands out both counts, each event to one caller
+ * of the process (synchronises with the device). */
 int lnsb_paged_errors(int64_t * bad_pages, int64_t * timeouts);
 
 /* The next token of every row of logits from one given random number per row.

@@ -31,3 +31,30 @@ def test_a_token_without_a_page_counts_once(ks, n_dims, offset, with_q):
                     q_out=torch.zeros(50, 3, 64, dtype=torch.float16, device="cuda") if with_q else None, cos_sin=cs)
     assert ks.paged_errors() == (16, 0)
     assert ks.paged_errors() == (0, 0)
+
+
+def test_no_count_is_lost(ks):
+    """one thread launches, others read and clear all the while: what they were given adds up"""
+    P = ref.Paged([20], [20], 1, 64, 8, torch.float16, seed=61, junk=0.0)
+    P.table[0, 1] = 99
+    x = torch.zeros((20, 2, 64), device="cuda")
+    ks.paged_errors()
+    steps, seen, done = 3000, [0, 0, 0], threading.Event()
+
+    def launch():
+        for _ in range(steps):
+            ks.paged_append(x[:, :1], x[:, 1:], P.k, P.v, P.table, P.q_start, P.kv_len, 20)
+        done.set()
+
+    def read(i):
+        while not done.is_set():
+            seen[i] += ks.paged_errors()[0]
+
+    threads = [threading.Thread(target=launch)] + [threading.Thread(target=read, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    seen[2] = ks.paged_errors()[0]
+    assert sum(seen) == 8 * steps, seen

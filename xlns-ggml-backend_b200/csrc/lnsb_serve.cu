@@ -12,6 +12,7 @@
 #include <cfloat>
 #include <cmath>
 #include <cstdint>
+#include <mutex>
 #include <type_traits>
 
 #include "lnsb200.h"
@@ -2654,11 +2655,23 @@ int lnsb_paged_attn(const lnsb_paged_attn_args * a, lnsb_stream_t stream) {
 }
 
 int lnsb_paged_errors(int64_t * bad_pages, int64_t * timeouts) {
-    unsigned long long v[2] = {}, zero[2] = {};
-    cudaError_t e = cudaDeviceSynchronize();
-    if (e == cudaSuccess) e = cudaMemcpyFromSymbol(v, g_paged_errors, sizeof(v));
-    if (e == cudaSuccess) e = cudaMemcpyToSymbol(g_paged_errors, zero, sizeof(zero));
+    // the device's counts only grow, also while they are read; what was handed out is kept here
+    static std::mutex lock;
+    static unsigned long long given[k_max_devices][2];
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess) e = cudaDeviceSynchronize();
     if (e != cudaSuccess) return (int) e;
+    if (dev < 0 || dev >= k_max_devices) return LNSB_E_NO_DEVICE;
+    const std::lock_guard<std::mutex> hold(lock);
+    unsigned long long v[2] = {};
+    e = cudaMemcpyFromSymbol(v, g_paged_errors, sizeof(v));
+    if (e != cudaSuccess) return (int) e;
+    for (int i = 0; i < 2; i++) {
+        const unsigned long long before = v[i] < given[dev][i] ? 0 : given[dev][i];     // 0: the device was reset
+        given[dev][i] = v[i];
+        v[i] -= before;
+    }
     if (bad_pages) *bad_pages = (int64_t) v[0];
     if (timeouts) *timeouts = (int64_t) v[1];
     return 0;
