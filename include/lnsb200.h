@@ -467,7 +467,9 @@ int lnsb_paged_append(const lnsb_paged_append_args * args, lnsb_stream_t stream)
  *
  * work: lnsb_paged_attn_work_bytes() bytes of device memory, 16-byte aligned,
  * zero before its first use; every call leaves it ready for the next.  Calls
- * that can overlap on the GPU need one each. */
+ * that can overlap on the GPU need one each.  Its last 8 bytes count, as an
+ * int64, the waits that ran out in the calls that used it: where they are not
+ * 0, those calls' outputs are invalid, and work has to be zeroed again. */
 typedef struct {
     lnsb_paged_kv kv;
     const void *  q;              /* [n_tokens][n_head][head_dim] */
@@ -482,12 +484,16 @@ typedef struct {
 } lnsb_paged_attn_args;
 int lnsb_paged_attn(const lnsb_paged_attn_args * args, lnsb_stream_t stream);
 int64_t lnsb_paged_attn_work_bytes(void);
+/* the most SM clock cycles that a wait inside lnsb_paged_attn may take before
+ * the call gives up, for the process's later calls: 2^31 at first, about a
+ * second, and at most; 0: as soon as one is not over at once */
+int lnsb_paged_attn_wait_limit(int64_t cycles);
 
 /* since the last call, on the current device: page ids outside the cache met
  * by lnsb_paged_append (one for each token) and lnsb_paged_attn (one at least
  * for each such page that a call reads), and waits inside lnsb_paged_attn
- * that ran out (its output is then invalid, and its work has to be zeroed
- * again); either may be NULL.  Hands out both counts, each event to one caller
+ * that ran out (in any call of the process: work tells a caller about its own);
+ * either may be NULL.  Hands out both counts, each event to one caller
  * of the process (synchronises with the device). */
 int lnsb_paged_errors(int64_t * bad_pages, int64_t * timeouts);
 

@@ -58,3 +58,48 @@ def test_no_count_is_lost(ks):
     torch.cuda.synchronize()
     seen[2] = ks.paged_errors()[0]
     assert sum(seen) == 8 * steps, seen
+
+
+@pytest.mark.parametrize("dim", (64, 128))
+def test_waits_that_run_out(ks, dim):
+    """with a limit of nothing the first wait for memory gives up: the call ends, both counts say so, and with work
+    zeroed and the limit back the next call is right"""
+    import test_gpu_paged as paged
+    P = ref.Paged([300, 40], [1100, 500], 2, dim, 16, torch.bfloat16, seed=62)
+    q = paged._q(P, 8, dim, torch.bfloat16, 63)
+    work, other = ks.paged_attn_work(), ks.paged_attn_work()
+    paged._check(ks, work, P, q)
+    ks.paged_attn_wait_limit(0)
+    try:
+        for i in range(3):
+            paged._attn(ks, work, P, q)
+            torch.cuda.synchronize()
+            assert ks.paged_errors()[1] > 0 and ks.paged_attn_timeouts(work) > 0
+    finally:
+        ks.paged_attn_wait_limit(1 << 31)
+    assert ks.paged_attn_timeouts(other) == 0
+    paged._check(ks, other, P, q)
+    work.zero_()
+    paged._check(ks, work, P, q)
+    assert ks.paged_attn_timeouts(work) == 0
+
+
+def test_the_decoder_raises_and_goes_on(ks):
+    from lnsb200 import model, serve
+    cfg = dict(n_layer=1, n_embd=192, n_head=3, n_head_kv=1, head_dim=64, n_ff=256, vocab=320, rope_base=10000.0, eps=1e-5)
+    ops = model.GpuOps(cfg, model.init_weights(cfg, seed=3), mode="base", n_ctx=128, fmt=32)
+    prompt = model.prompt_ids(cfg, 50, seed=4)
+    dec = serve.PagedDecoder(ops, n_pages=16)
+    s = dec.open()
+    want = dec.step([(s, prompt)], temperature=0.0)
+    dec.close(s)
+    s = dec.open()
+    ops.ks.paged_attn_wait_limit(0)
+    try:
+        with pytest.raises(RuntimeError, match="ran out"):
+            dec.step([(s, prompt)], temperature=0.0)
+    finally:
+        ops.ks.paged_attn_wait_limit(1 << 31)
+    assert dec.pool.length[s] == 0
+    assert dec.step([(s, prompt)], temperature=0.0) == want
+    ops.ks.paged_errors()

@@ -60,6 +60,10 @@ class Kernels:
         self.log.append(("work", self.ops.torch.cuda.now.name))
         return torch.zeros(64, dtype=torch.uint8)
 
+    def paged_attn_timeouts(self, work):
+        self.log.append(("timeouts", self.ops.torch.cuda.now.name))
+        return work[-8:].view(torch.int64).item()
+
     def _call(self, name, stream):
         now = self.ops.torch.cuda.now
         self.log.append((name, (stream or now).name))
@@ -74,6 +78,9 @@ class Kernels:
     def paged_attn(self, q, kc, vc, table, q_start, kv_len, max_q, max_kv, dst, work, stream=None):
         self._call("attn", stream)
         dst.zero_()
+        if self.ops.timeout:
+            work[-8:].view(torch.int64).add_(1)
+            work[0] = 1                                     # a counter left half way
 
     def f16_to_f32(self, src, dst, n, stream=None):
         self._call("to f32", stream)
@@ -87,7 +94,7 @@ class Kernels:
 
 class Ops:
     def __init__(self, stream=None, n_ctx=32):
-        self.log, self.plans, self.fail = [], [], None
+        self.log, self.plans, self.fail, self.timeout = [], [], None, False
         self.torch, self.cfg, self.n_ctx, self.dev = Torch(self.log), CFG, n_ctx, torch.device("cpu")
         self.stream = Stream(stream, self.log) if stream else None
         self.rope_cs, self.ks = torch.zeros(n_ctx, 2, 2), Kernels(self)
@@ -231,3 +238,35 @@ def test_tokens_outside_the_vocabulary(ids):
         with pytest.raises(ValueError, match="vocab"):
             call([(b, [1]), (a, ids)])
     assert _state(dec) == before and ops.log == log
+
+
+# ----------------------------------------------------------- waits that ran out
+
+def test_an_attention_that_gave_up():
+    """the step raises and takes its rows back, and the workspace is clean for the next"""
+    ops = Ops()
+    dec = PagedDecoder(ops, n_pages=8, page_size=4)
+    a = dec.open()
+    assert dec.step([(a, [1, 2, 3])]) == [3]
+    before = _state(dec)
+    ops.timeout = True
+    with pytest.raises(RuntimeError, match="ran out"):
+        dec.step([(a, [4, 5, 6])])
+    assert _state(dec) == before and not dec.work.any()
+    dec.forward([(a, [4])])
+    with pytest.raises(RuntimeError, match="ran out"):
+        dec.check()
+    ops.timeout = False
+    dec.check()
+    assert dec.step([(a, [5])]) == [3]
+
+
+def test_one_decoders_timeout_is_its_own():
+    slow, fine = Ops(), Ops()
+    a, b = PagedDecoder(slow, n_pages=8, page_size=4), PagedDecoder(fine, n_pages=8, page_size=4)
+    slow.timeout = True
+    sa, sb = a.open(), b.open()
+    a.forward([(sa, [1])])
+    assert b.step([(sb, [1, 2])]) == [3]
+    with pytest.raises(RuntimeError, match="ran out"):
+        a.check()

@@ -9,6 +9,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cfloat>
 #include <cmath>
 #include <cstdint>
@@ -669,16 +670,20 @@ k_paged_attn_rows(paged P, const T * __restrict__ q, T * __restrict__ dst, const
 // the CTAs cut into equal shares; each warp joins its own 32 rows of a cut
 // item, so no warp waits for another outside the mbarriers.
 //
-// Every wait gives up after k_wait_cycles: the CTA then drains what it has in
-// flight, frees its TMEM and counts a timeout.
+// Every wait gives up after a limit (lnsb_paged_attn_wait_limit): the CTA then
+// drains what it has in flight, frees its TMEM and counts a timeout, for the
+// device and in `work`.
 
 constexpr int B_ROWS = 128, B_TILE = 256, B_THREADS = 384, B_SUMS = 256, B_ITEMS = 4, B_CTAS = k_sms;
-constexpr long long k_wait_cycles = 1ll << 31;
+constexpr uint32_t k_wait_cycles = 1u << 31;
 
+// work, behind the rows kernel's: counters, partials, and the waits that ran out
 // partials: [slot][group][warp][d / 4][lane] float4, then [warp][lane] (m, l)
 constexpr int64_t B_PART = (int64_t) B_TILE * (128 + 2);
 constexpr int64_t B_COUNT_BYTES = ((int64_t) B_CTAS * 8 * 4 + 255) / 256 * 256;
 constexpr int64_t B_WORK = B_COUNT_BYTES + (int64_t) B_CTAS * 2 * B_PART * 4;
+constexpr int64_t WORK_BYTES = A_WORK + B_WORK + 8;
+static_assert(B_WORK % 8 == 0, "the count's place");
 
 // ---- mbarriers, TMA, tcgen05 ----
 __device__ __forceinline__ void bar_init(uint32_t bar, uint32_t count) {
@@ -696,23 +701,27 @@ __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
                  : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
     return ok != 0;
 }
+struct give_up {
+    int      stop;                   // a wait has run out
+    uint32_t limit;                  // cycles
+};
 // false: the CTA gives up (this wait ran out, or another one did)
-__device__ __forceinline__ bool bar_wait_slow(uint32_t bar, uint32_t parity, volatile int * stop) {
-    const long long t0 = clock64();
+__device__ __forceinline__ bool bar_wait_slow(uint32_t bar, uint32_t parity, volatile give_up * stop) {
+    const uint32_t t0 = (uint32_t) clock();
     while (!bar_try(bar, parity)) {
-        if (*stop) return false;
-        if (clock64() - t0 > k_wait_cycles) {
-            *stop = 1;
+        if (stop->stop) return false;
+        if ((uint32_t) clock() - t0 > stop->limit) {
+            stop->stop = 1;
             return false;
         }
     }
     return true;
 }
-__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int * stop) {
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile give_up * stop) {
     return bar_try(bar, parity) || bar_wait_slow(bar, parity, stop);
 }
 // the same for a whole warp: all its lanes go on, or none
-__device__ __forceinline__ bool bar_wait_warp(uint32_t bar, uint32_t parity, volatile int * stop) {
+__device__ __forceinline__ bool bar_wait_warp(uint32_t bar, uint32_t parity, volatile give_up * stop) {
     return __all_sync(0xFFFFFFFFu, bar_wait(bar, parity, stop));
 }
 __device__ __forceinline__ void tma_page(uint32_t dst, const CUtensorMap * map, int d, int row, int head, int page, uint32_t bar) {
@@ -886,8 +895,8 @@ struct tile_control {                // behind the tiles
     int64_t   sums[B_SUMS];
     tile_item item[B_ITEMS];
     uint64_t  bar[2 * 10 + 2 * B_ITEMS + 15];
+    give_up   stop;
     uint32_t  tmem;
-    int       stop;
 };
 template <int D> __host__ __device__ constexpr int b_smem() {
     return 2 * b_q_bytes<D>() + b_ring<D>() * b_tile_bytes<D>() + (int) sizeof(tile_control);
@@ -898,7 +907,7 @@ template <class T, int D>
 __global__ void __launch_bounds__(B_THREADS, 1)
 k_paged_attn_tiles(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, paged P, tile_plan L,
                    const T * __restrict__ q, T * __restrict__ dst, int64_t q_ld, int64_t dst_ld, float scale_log2,
-                   int * __restrict__ counters, float * __restrict__ parts) {
+                   int * __restrict__ counters, float * __restrict__ parts, uint32_t wait_cycles, unsigned long long * __restrict__ ran_out) {
     // bytes of a K or V tile, of its 64-dim halves, and of Q's
     constexpr int B_KEYS = b_keys<D>(), BUFS = D == 128 ? 1 : 2, PARTS = B_KEYS / 64;
     constexpr int ST = b_ring<D>(), TB = b_tile_bytes<D>(), HB = B_KEYS * 128, QB = b_q_bytes<D>(), QH = B_ROWS * 128, HALVES = D / 64;
@@ -916,7 +925,7 @@ k_paged_attn_tiles(const __grid_constant__ CUtensorMap kmap, const __grid_consta
     const uint32_t bars = smem_addr(C.bar);
     const uint32_t kv_full = bars, kv_empty = bars + 8 * ST, q_full = kv_empty + 8 * ST, s_full = q_full + 16,
                    p_ready = s_full + 32, o_full = p_ready + 32, pv_done = o_full + 16, it_full = pv_done + 16, it_empty = it_full + 8 * B_ITEMS, drained = it_empty + 8 * B_ITEMS;
-    volatile int * stop = &C.stop;
+    volatile give_up * stop = &C.stop;
 
     if (tid == 0) {
         for (int i = 0; i < ST; i++) {
@@ -937,7 +946,8 @@ k_paged_attn_tiles(const __grid_constant__ CUtensorMap kmap, const __grid_consta
             bar_init(it_empty + 8 * i, 10);                  // warps 0 .. 9
         }
         bar_init(drained, 1);
-        C.stop = 0;
+        C.stop.limit = wait_cycles;
+        C.stop.stop = 0;
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
     // behind k_paged_attn_rows of the same call too: only a grid's own wait makes
@@ -1065,7 +1075,7 @@ k_paged_attn_tiles(const __grid_constant__ CUtensorMap kmap, const __grid_consta
                 }
             }
             // nothing of this CTA's may be in flight when it ends
-            int none = 0;
+            give_up none = { 0, k_wait_cycles };
             for (uint32_t i = n > ST ? n - ST : 0; i < n; i++) (void) bar_wait(kv_full + 8 * (i % ST), (i / ST) & 1, &none);
         } else if (warp == 8) {
             // ------------------------------------------------ MMA
@@ -1131,7 +1141,7 @@ k_paged_attn_tiles(const __grid_constant__ CUtensorMap kmap, const __grid_consta
                 ok = __shfl_sync(0xFFFFFFFFu, ok, 0);
             }
             if (lane == 0) {
-                int none = 0;
+                give_up none = { 0, k_wait_cycles };
                 mma_commit(drained);
                 (void) bar_wait(drained, 0, &none);
             }
@@ -1363,7 +1373,10 @@ k_paged_attn_tiles(const __grid_constant__ CUtensorMap kmap, const __grid_consta
     __syncthreads();
     if (work && warp == 8) {
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;\n" :: "r"(C.tmem));
-        if (lane == 0 && C.stop) atomicAdd(&g_paged_errors[1], 1ull);
+        if (lane == 0 && C.stop.stop) {
+            atomicAdd(&g_paged_errors[1], 1ull);
+            atomicAdd(ran_out, 1ull);
+        }
     }
 }
 
@@ -2519,6 +2532,8 @@ int launch_sample_rows(const lnsb_sample_args & a, cudaStream_t s) {
     return launch_sample<T, 512, false>(a, 1, vecs(512, 1), s);
 }
 
+std::atomic<uint32_t> wait_limit{ k_wait_cycles };   // of lnsb_paged_attn's later calls
+
 constexpr float k_log2e = 1.44269504088896340736f;
 
 template <class T, int D>
@@ -2583,7 +2598,8 @@ int launch_attn_dim(const lnsb_paged_attn_args & a, cudaStream_t s) {
             unsigned char * w = static_cast<unsigned char *>(a.work) + A_WORK;
             launch_k(kern, dim3(B_CTAS), dim3(B_THREADS), (size_t) b_smem<D>(), s, km, vm, view_of(a.kv), L,
                      static_cast<const T *>(a.q), static_cast<T *>(a.dst), a.q_ld, a.dst_ld, a.scale * k_log2e,
-                     reinterpret_cast<int *>(w), reinterpret_cast<float *>(w + B_COUNT_BYTES));
+                     reinterpret_cast<int *>(w), reinterpret_cast<float *>(w + B_COUNT_BYTES),
+                     wait_limit.load(), reinterpret_cast<unsigned long long *>(w + B_WORK));
             return launch_status();
         }
     }
@@ -2632,7 +2648,13 @@ int lnsb_paged_append(const lnsb_paged_append_args * a, lnsb_stream_t stream) {
     }
 }
 
-int64_t lnsb_paged_attn_work_bytes(void) { return A_WORK + B_WORK; }
+int64_t lnsb_paged_attn_work_bytes(void) { return WORK_BYTES; }
+
+int lnsb_paged_attn_wait_limit(int64_t cycles) {
+    if (cycles < 0) return LNSB_E_INVALID;
+    wait_limit.store((uint32_t) std::min<int64_t>(cycles, k_wait_cycles));
+    return 0;
+}
 
 int lnsb_paged_attn(const lnsb_paged_attn_args * a, lnsb_stream_t stream) {
     if (a == nullptr) return LNSB_E_INVALID;

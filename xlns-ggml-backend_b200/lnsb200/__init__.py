@@ -316,6 +316,17 @@ class KernelSet:
         if st:
             _lib.check(self.lib, "lnsb_paged_attn", st)
 
+    def paged_attn_timeouts(self, work):
+        """waits that ran out in the calls that used this workspace (read on the current stream): if there are any, those
+        calls' outputs are invalid, and the workspace has to be zeroed"""
+        import torch
+        n = self.lib.lnsb_paged_attn_work_bytes()
+        return work.view(torch.uint8)[n - 8:n].view(torch.int64).item()
+
+    def paged_attn_wait_limit(self, cycles):
+        """the most SM clock cycles that a wait inside paged_attn may take (lnsb_paged_attn_wait_limit)"""
+        _lib.check(self.lib, "lnsb_paged_attn_wait_limit", self.lib.lnsb_paged_attn_wait_limit(cycles))
+
     def paged_errors(self):
         """(page ids outside the cache, waits that ran out) since the last call, on the current device"""
         b, t = ctypes.c_int64(), ctypes.c_int64()

@@ -159,6 +159,7 @@ SIGNATURES = [
     ("lnsb_paged_append", ctypes.c_int, [ctypes.POINTER(PagedAppendArgs), _VP]),
     ("lnsb_paged_attn", ctypes.c_int, [ctypes.POINTER(PagedAttnArgs), _VP]),
     ("lnsb_paged_attn_work_bytes", _I64, []),
+    ("lnsb_paged_attn_wait_limit", ctypes.c_int, [_I64]),
     ("lnsb_paged_errors", ctypes.c_int, [ctypes.POINTER(_I64), ctypes.POINTER(_I64)]),
     ("lnsb_sample", ctypes.c_int, [ctypes.POINTER(SampleArgs), _VP]),
     ("lnsb_monte_get_state", ctypes.c_int, [ctypes.POINTER(ctypes.c_uint16)]),

@@ -131,7 +131,8 @@ class PagedDecoder:
 
     def forward(self, batch):
         """logits (F32, [len(batch)][vocab]) of the last of the new tokens of each (sequence, tokens) of `batch`; if it
-        raises, the sequences are as they were"""
+        raises, the sequences are as they were.  The work is on its way when this returns: `check` says whether it went
+        well"""
         with self._or_shrink(self._grow(batch)):
             return self._forward(batch)
 
@@ -173,6 +174,16 @@ class PagedDecoder:
         h = ops.mul(ops.rms_norm(last, cfg["eps"], "norm"), ops.w(None, "output_norm"))
         return ops.linear(ops.w(None, "output"), h, "result_output", "result_norm")
 
+    def check(self):
+        """raises RuntimeError if a wait inside the attention ran out since the last check: what came out of it and the
+        rows written since are invalid (waits for the device)"""
+        with self._on_stream():
+            n = self.ks.paged_attn_timeouts(self.work)
+            if n:
+                self.work.zero_()
+        if n:
+            raise RuntimeError("%d waits inside the attention ran out" % n)
+
     def sample(self, logits, u=None, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
         """next tokens (int32 on the device) and their probabilities; each parameter one number, or one for each row;
         u: the random numbers, or None to draw them"""
@@ -191,4 +202,6 @@ class PagedDecoder:
         """forward, then sample: the next token of each sequence of the batch, on the host; if it raises, the sequences
         are as they were"""
         with self._or_shrink(self._grow(batch)):
-            return self.sample(self._forward(batch), u, **sampling)[0].tolist()
+            tokens = self.sample(self._forward(batch), u, **sampling)[0].tolist()
+            self.check()
+            return tokens
