@@ -170,3 +170,66 @@ def test_many_light_weights_in_half(ks, work, dim, q, lo, hi):
     got = _attn(ks, work, P, qq.repeat(seqs, 1, 1), scale=scale).view(seqs, q, 2, dim).double()
     assert float(want.min()) > 1e-4
     assert ((got - want).abs() <= bound).all(), float(((got - want).abs() / bound).max())
+
+
+# ------------------------------------------------------------ many sequences
+
+@pytest.mark.parametrize("seqs", (129, 300, 700))
+@pytest.mark.parametrize("kind", ("tokens", "chunks", "mixed"))
+@pytest.mark.parametrize("heads,kv_heads,dim", [(2, 1, 64), (4, 2, 128), (2, 2, 16)])
+@pytest.mark.parametrize("window", (0, 40))
+def test_many_sequences(ks, work, seqs, kind, heads, kv_heads, dim, window):
+    """more sequences than one thread or lane looks at, idle ones first, last and in long runs"""
+    g = torch.Generator().manual_seed(seqs)
+    kv = torch.randint(0, 150, (seqs,), generator=g).tolist()
+    most = {"tokens": 1, "chunks": 60, "mixed": 60}[kind]
+    q = torch.randint(0 if kind == "tokens" else 2, most + 1, (seqs,), generator=g).tolist()
+    if kind == "mixed":
+        q = [n if i % 3 == 0 else n % 3 for i, n in enumerate(q)]
+    for lo, hi in ((0, 5), (40, 75), (seqs - 9, seqs)):
+        q[lo:hi] = [0] * (hi - lo)
+    P = ref.Paged(q, kv, kv_heads, dim, 16, BF16, seed=51)
+    x = _q(P, heads, dim, BF16, 52)
+    _check(P, x, _attn(ks, work, P, x, window), window)
+    assert ks.paged_errors() == (0, 0)
+
+
+def test_one_sequence_among_thousands_of_idle_ones(ks, work):
+    for seqs in (5000, 65536):
+        for at in (0, seqs // 2 + 3, seqs - 1):
+            q, kv = [0] * seqs, [0] * seqs
+            q[at], kv[at] = 50, 333
+            P = ref.Paged([50], [333], 2, 64, 16, BF16, seed=53)
+            start = torch.zeros(seqs + 1, dtype=torch.int32, device="cuda")
+            start[at + 1:] = 50
+            lens, table = torch.zeros(seqs, dtype=torch.int32, device="cuda"), P.table.new_full((seqs, P.table.shape[1]), -1)
+            lens[at], table[at] = 333, P.table[0]
+            x = _q(P, 4, 64, BF16, 54)
+            dst = torch.full_like(x, float("nan"))
+            ks.paged_attn(x, P.k, P.v, table, start, lens, 50, 333, dst, work)
+            _check(P, x, dst)
+
+
+# ----------------------------------------------------------------- the bounds
+
+@pytest.mark.parametrize("heads,kv_heads,dim", [(4, 2, 64), (8, 2, 128), (4, 2, 32)])
+@pytest.mark.parametrize("lengths", [([1, 1, 0], [70, 500, 3]), ([40, 1, 130], [40, 700, 300]), ([90], [400])], ids=str)
+def test_any_bound_on_the_new_tokens(ks, work, heads, kv_heads, dim, lengths):
+    """max_q chooses the kernels and limits nothing, below the real one too"""
+    P = ref.Paged(*lengths, kv_heads, dim, 16, BF16, seed=55)
+    x = _q(P, heads, dim, BF16, 56)
+    for max_q in (0, 1, 16, 1000, 2 ** 31 - 1, 2 ** 62, 2 ** 63 - 1):
+        _check(P, x, _attn(ks, work, P, x, max_q=max_q))
+    for max_kv in (P.max_kv + 1, P.table.shape[1] * 16):
+        _check(P, x, _attn(ks, work, P, x, max_kv=max_kv))
+    assert ks.paged_errors() == (0, 0)
+
+
+@pytest.mark.parametrize("dim", (64, 32))
+def test_a_bound_on_the_rows_below_the_real_one(ks, work, dim):
+    """kv_len above max_kv is taken as max_kv"""
+    P = ref.Paged([40, 1], [300, 90], 2, dim, 16, BF16, seed=57)
+    x = _q(P, 4, dim, BF16, 58)
+    got = _attn(ks, work, P, x, max_kv=200)
+    P.kv = [200, 90]
+    _check(P, x, got)
