@@ -33,3 +33,24 @@ def test_steps_on_another_stream_than_the_current():
         assert ops.ks.paged_errors() == (0, 0)
     assert runs[0][1] == runs[1][1]
     assert all(torch.equal(a, b) for a, b in zip(runs[0][0], runs[1][0]))
+
+
+@pytest.mark.parametrize("fused", (True, False))
+def test_the_model_on_another_stream_than_the_current(fused):
+    """the same of the graph with its own cache: a prompt, then steps, with work ahead on either stream"""
+    from lnsb200 import model
+    weights, runs = model.init_weights(TINY, seed=5), []
+    for stream in (None, torch.cuda.Stream()):
+        ops = model.GpuOps(TINY, weights, mode="sum32", n_ctx=64, stream=stream, fmt=32)
+        ops.fused = fused
+        busy = torch.zeros(1 << 26, device="cuda")
+        ids, pos, out = model.prompt_ids(TINY, 9, seed=6), 0, []
+        for i in range(6):
+            for s in (torch.cuda.current_stream(), stream):
+                if s is not None:
+                    with torch.cuda.stream(s):
+                        busy.add_(1.0).mul_(0.5)
+            out.append(model.forward(ops, TINY, ids, pos).clone())
+            pos, ids = pos + len(ids), [int(out[-1].argmax())]
+        runs.append(out)
+    assert all(torch.equal(a, b) for a, b in zip(*runs))

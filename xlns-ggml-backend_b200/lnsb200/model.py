@@ -33,6 +33,7 @@ Weights are drawn in a fixed order from numpy default_rng(seed) N(0, 0.02),
 F32; the norm weights are 1.0.  The prompt is `prompt_len` ids from a separate
 default_rng(seed).integers(0, vocab).
 """
+import contextlib
 import math
 
 import numpy as np
@@ -83,9 +84,41 @@ def rope_table(n_ctx, n_dims, base):
     return out
 
 
+@contextlib.contextmanager
+def on_stream(ops):
+    """the ops' own stream (ops.stream; none: the current one), behind the current
+    stream's work and before its next"""
+    mine = getattr(ops, "stream", None)
+    now = None if mine is None else ops.torch.cuda.current_stream(ops.dev)
+    if mine is None or mine == now:
+        yield
+        return
+    mine.wait_stream(now)
+    try:
+        with ops.torch.cuda.stream(mine):
+            yield
+    finally:
+        now.wait_stream(mine)
+
+
+def handed_over(ops, *tensors):
+    """tensors made in on_stream that the current stream will read"""
+    if getattr(ops, "stream", None) is not None:
+        for t in tensors:
+            if t.is_cuda:
+                t.record_stream(ops.torch.cuda.current_stream(ops.dev))
+
+
 def forward(ops, cfg, ids, pos0):
     """logits (F32, [vocab]) of the last of `ids`, which sit at positions
     pos0 .. pos0 + len(ids) - 1; the KV cache holds positions < pos0."""
+    with on_stream(ops):
+        logits = _forward(ops, cfg, ids, pos0)
+    handed_over(ops, logits)
+    return logits
+
+
+def _forward(ops, cfg, ids, pos0):
     if getattr(ops, "fused", False) and (ids.numel() if hasattr(ids, "numel") else len(ids)) == 1:
         return ops.forward_fused(cfg, ids, pos0)            # a decode step: the fused ops
     T, E = (ids.numel() if hasattr(ids, "numel") else len(ids)), cfg["n_embd"]

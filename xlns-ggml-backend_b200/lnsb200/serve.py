@@ -15,6 +15,8 @@ host takes out of LNS with LNS_DISABLE_OPS=rope,kq,kq_soft_max,kqv), through
 """
 import contextlib
 
+from .model import handed_over, on_stream
+
 __all__ = ["PagePool", "PagedDecoder"]
 
 
@@ -71,32 +73,11 @@ class PagedDecoder:
         self.ops, self.cfg, self.ks, self.torch = ops, cfg, ops.ks, torch
         self.pool = PagePool(n_pages, page_size)
         shape = (n_pages, page_size, cfg["n_head_kv"], cfg["head_dim"])
-        with self._on_stream():
+        with on_stream(ops):
             # zeros: rows that no sequence has written are never seen, but a reader of the cache may look
             self.kc = [torch.zeros(shape, dtype=torch.float16, device=ops.dev) for _ in range(cfg["n_layer"])]
             self.vc = [torch.zeros(shape, dtype=torch.float16, device=ops.dev) for _ in range(cfg["n_layer"])]
             self.work = self.ks.paged_attn_work(ops.dev)
-
-    @contextlib.contextmanager
-    def _on_stream(self):
-        """the ops' stream, behind the current one's work and before its next"""
-        cuda, mine = self.torch.cuda, self.ops.stream
-        now = None if mine is None else cuda.current_stream(self.ops.dev)
-        if mine is None or mine == now:
-            yield
-            return
-        mine.wait_stream(now)
-        try:
-            with cuda.stream(mine):
-                yield
-        finally:
-            now.wait_stream(mine)
-
-    def _handed_over(self, *tensors):
-        """tensors of the ops' stream that the caller's current stream will read"""
-        for t in tensors:
-            if t.is_cuda:
-                t.record_stream(self.torch.cuda.current_stream(self.ops.dev))
 
     def open(self):
         return self.pool.open()
@@ -137,9 +118,9 @@ class PagedDecoder:
             return self._forward(batch)
 
     def _forward(self, batch):
-        with self._on_stream():
+        with on_stream(self.ops):
             logits = self._graph(batch)
-        self._handed_over(logits)
+        handed_over(self.ops, logits)
         return logits
 
     def _graph(self, batch):
@@ -177,7 +158,7 @@ class PagedDecoder:
     def check(self):
         """raises RuntimeError if a wait inside the attention ran out since the last check: what came out of it and the
         rows written since are invalid (waits for the device)"""
-        with self._on_stream():
+        with on_stream(self.ops):
             n = self.ks.paged_attn_timeouts(self.work)
             if n:
                 self.work.zero_()
@@ -189,13 +170,13 @@ class PagedDecoder:
         u: the random numbers, or None to draw them"""
         torch, n = self.torch, logits.shape[0]
         each = lambda v, t: torch.as_tensor(v, dtype=t, device=self.ops.dev).expand(n).contiguous()  # noqa: E731
-        with self._on_stream():
+        with on_stream(self.ops):
             u = torch.rand(n, device=self.ops.dev) if u is None else each(u, torch.float32)
             token = torch.empty(n, dtype=torch.int32, device=self.ops.dev)
             prob = torch.empty(n, dtype=torch.float32, device=self.ops.dev)
             self.ks.sample(logits, u, token, prob, each(temperature, torch.float32), each(top_k, torch.int32),
                            each(top_p, torch.float32), each(min_p, torch.float32), stream=self.ops.stream)
-        self._handed_over(token, prob)
+        handed_over(self.ops, token, prob)
         return token, prob
 
     def step(self, batch, u=None, **sampling):
