@@ -1008,145 +1008,145 @@ k_paged_attn_tiles(const __grid_constant__ CUtensorMap kmap, const __grid_consta
         };
         if (warp >= 8) {
             if constexpr (D == 128) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;\n" ::);
-        if (warp == 10) {
-            // ------------------------------------------------ items
-            line_walk walk;
-            walk.sums = C.sums;
-            walk.per = per;
-            walk.W = W;
-            walk.N = N;
-            walk.x = W * blockIdx.x / N;
-            walk.x_end = W * (blockIdx.x + 1) / N;
-            walk.base = walk.run_base = 0;
-            walk.seq_len = -1;
-            walk.run = walk.s = 0;
-            do {
-                const uint32_t i = items % B_ITEMS;
-                walk.next(P, L, I);
-                if (!bar_wait_warp(it_empty + 8 * i, ((items / B_ITEMS) & 1) ^ 1, stop)) break;
-                if (lane == 0) {
-                    C.item[i] = I;
-                    bar_arrive(it_full + 8 * i);
-                }
-                __syncwarp();
-                items++;
-            } while (I.n > 0);
-        } else if (warp == 9) {
-            // ------------------------------------------------ K and V pages
-            const int box = min(1 << P.page_shift, B_KEYS), boxes = B_KEYS / box;
-            uint32_t n = 0;                                  // buffers filled
-            bool ok = true;
-            while (ok && next_item()) {
-                const int seen = first_owned(I, L);
-                // the page (out of bounds: zeros) and its row that this lane copies of tile t
-                auto place = [&](int t, int & row) {
-                    const int64_t key = (int64_t) I.key0 + t * B_KEYS + lane * box;
-                    int64_t page = -1;
-                    if (t < I.n && lane < boxes && key < I.kv && key + box > seen) page = page_of(P, I.seq, key);
-                    row = (int) (key & ((1 << P.page_shift) - 1));
-                    return (int) (page < 0 ? P.n_pages : page);
-                };
-                auto copy = [&](const CUtensorMap * map, int page, int row) {
-                    const uint32_t b = n % ST;
-                    if (!bar_wait_warp(kv_empty + 8 * b, ((n / ST) & 1) ^ 1, stop)) return false;
-                    if (lane == 0) bar_expect(kv_full + 8 * b, TB);
-                    __syncwarp();
-                    if (lane < boxes)
-#pragma unroll
-                        for (int i = 0; i < HALVES; i++)
-                            tma_page(ring + b * TB + i * HB + lane * box * 128, map, 64 * i, row, I.head, page, kv_full + 8 * b);
-                    n++;
-                    return true;
-                };
-                // in the order of their use: K 0 (K 1), then V 0, K 1 (K 2), V 1, ..
-                // (page ids are looked up a tile ahead)
-                int row[BUFS + 1], page[BUFS + 1];
-#pragma unroll
-                for (int t = 0; t <= BUFS; t++) {
-                    page[t] = place(t, row[t]);
-                    if (t < BUFS && t < I.n) ok = ok && copy(&kmap, page[t], row[t]);
-                }
-                for (int t = 0; ok && t < I.n; t++) {
-                    ok = copy(&vmap, page[0], row[0]);
-                    if (t + BUFS < I.n) ok = ok && copy(&kmap, page[BUFS], row[BUFS]);
-#pragma unroll
-                    for (int i = 0; i < BUFS; i++) page[i] = page[i + 1], row[i] = row[i + 1];
-                    page[BUFS] = place(t + BUFS + 1, row[BUFS]);
-                }
-            }
-            // nothing of this CTA's may be in flight when it ends
-            give_up none = { 0, k_wait_cycles };
-            for (uint32_t i = n > ST ? n - ST : 0; i < n; i++) (void) bar_wait(kv_full + 8 * (i % ST), (i / ST) & 1, &none);
-        } else if (warp == 8) {
-            // ------------------------------------------------ MMA
-            uint32_t n = 0;                                  // ring position of the item's first K
-            uint32_t tiles[2] = { 0, 0 }, nq[2] = { 0, 0 };  // tiles of each group so far; phases of q_full
-            bool ok = true;
-            while (ok && next_item()) {
-                const int groups = I.rows - I.r0 > B_ROWS ? 2 : 1;
-                const uint32_t nt = (uint32_t) I.n;
-                if (lane == 0) {
-                    auto full = [&](uint32_t i) { return bar_wait(kv_full + 8 * (i % ST), (i / ST) & 1, stop); };
-                    auto k_at = [&](uint32_t j) { return n + (j < BUFS ? j : 2 * j - BUFS + 1); };     // ring positions
-                    auto v_at = [&](uint32_t j) { return n + min(j + BUFS, nt) + j; };
-                    auto qk = [&](int g, uint32_t j) {
-                        const uint32_t kb = ring + k_at(j) % ST * TB, qb = q_sm + g * QB, b = (tiles[g] + j) % BUFS;
-#pragma unroll
-                        for (int k = 0; k < D / 16; k++)
-                            mma_ss(tmem + S_COL + 128 * g + 64 * b, smem_desc(qb + (k / 4) * QH + (k % 4) * 32, 16, 1024),
-                                   smem_desc(kb + (k / 4) * HB + (k % 4) * 32, 16, 1024), idesc_qk, k > 0);
-                        mma_commit(s_full + 16 * g + 8 * b);
-                    };
-                    for (uint32_t j = 0; ok && j < min(nt, (uint32_t) BUFS); j++) {
-                        ok = full(k_at(j));
-                        for (int g = 0; ok && g < groups; g++) {
-                            if (j == 0) ok = bar_wait(q_full + 8 * g, nq[g]++ & 1, stop);
-                            tc_after();
-                            if (ok) qk(g, j);
-                        }
-                        if (ok) mma_commit(kv_empty + 8 * (k_at(j) % ST));
+            if (warp == 10) {
+                // ------------------------------------------------ items
+                line_walk walk;
+                walk.sums = C.sums;
+                walk.per = per;
+                walk.W = W;
+                walk.N = N;
+                walk.x = W * blockIdx.x / N;
+                walk.x_end = W * (blockIdx.x + 1) / N;
+                walk.base = walk.run_base = 0;
+                walk.seq_len = -1;
+                walk.run = walk.s = 0;
+                do {
+                    const uint32_t i = items % B_ITEMS;
+                    walk.next(P, L, I);
+                    if (!bar_wait_warp(it_empty + 8 * i, ((items / B_ITEMS) & 1) ^ 1, stop)) break;
+                    if (lane == 0) {
+                        C.item[i] = I;
+                        bar_arrive(it_full + 8 * i);
                     }
-                    for (uint32_t j = 0; ok && j < nt; j++) {
-                        const uint32_t vb = ring + v_at(j) % ST * TB;
-                        ok = full(v_at(j));
-                        for (int g = 0; ok && g < groups; g++) {
-                            const uint32_t at = tiles[g] + j, b = at % BUFS;
-                            auto pv = [&](int part) {
-                                if (!bar_wait(p_ready + 16 * g + 8 * (PARTS == 2 ? part : b), at / BUFS & 1, stop)) return false;
-                                tc_after();
+                    __syncwarp();
+                    items++;
+                } while (I.n > 0);
+            } else if (warp == 9) {
+                // ------------------------------------------------ K and V pages
+                const int box = min(1 << P.page_shift, B_KEYS), boxes = B_KEYS / box;
+                uint32_t n = 0;                                  // buffers filled
+                bool ok = true;
+                while (ok && next_item()) {
+                    const int seen = first_owned(I, L);
+                    // the page (out of bounds: zeros) and its row that this lane copies of tile t
+                    auto place = [&](int t, int & row) {
+                        const int64_t key = (int64_t) I.key0 + t * B_KEYS + lane * box;
+                        int64_t page = -1;
+                        if (t < I.n && lane < boxes && key < I.kv && key + box > seen) page = page_of(P, I.seq, key);
+                        row = (int) (key & ((1 << P.page_shift) - 1));
+                        return (int) (page < 0 ? P.n_pages : page);
+                    };
+                    auto copy = [&](const CUtensorMap * map, int page, int row) {
+                        const uint32_t b = n % ST;
+                        if (!bar_wait_warp(kv_empty + 8 * b, ((n / ST) & 1) ^ 1, stop)) return false;
+                        if (lane == 0) bar_expect(kv_full + 8 * b, TB);
+                        __syncwarp();
+                        if (lane < boxes)
 #pragma unroll
-                                for (int kk = 4 * part; kk < 4 * part + 4; kk++)
-                                    mma_ts(tmem + O_COL + D * g, tmem + S_COL + 128 * g + 64 * b + 8 * kk,
-                                           smem_desc(vb + kk * 2048, HB, 1024), idesc_pv, j > 0 || kk > 0);
-                                return true;
-                            };
-                            if (!(ok = pv(0))) break;
-                            if constexpr (PARTS == 2)
-                                if (!(ok = pv(1))) break;
-                            if (j + 1 == nt) mma_commit(o_full + 8 * g);
-                            else if (BUFS == 2) mma_commit(pv_done + 8 * g);
-                            if (j + BUFS < nt) {
-                                if (g == 0 && !(ok = full(k_at(j + BUFS)))) break;
-                                qk(g, j + BUFS);
+                            for (int i = 0; i < HALVES; i++)
+                                tma_page(ring + b * TB + i * HB + lane * box * 128, map, 64 * i, row, I.head, page, kv_full + 8 * b);
+                        n++;
+                        return true;
+                    };
+                    // in the order of their use: K 0 (K 1), then V 0, K 1 (K 2), V 1, ..
+                    // (page ids are looked up a tile ahead)
+                    int row[BUFS + 1], page[BUFS + 1];
+#pragma unroll
+                    for (int t = 0; t <= BUFS; t++) {
+                        page[t] = place(t, row[t]);
+                        if (t < BUFS && t < I.n) ok = ok && copy(&kmap, page[t], row[t]);
+                    }
+                    for (int t = 0; ok && t < I.n; t++) {
+                        ok = copy(&vmap, page[0], row[0]);
+                        if (t + BUFS < I.n) ok = ok && copy(&kmap, page[BUFS], row[BUFS]);
+#pragma unroll
+                        for (int i = 0; i < BUFS; i++) page[i] = page[i + 1], row[i] = row[i + 1];
+                        page[BUFS] = place(t + BUFS + 1, row[BUFS]);
+                    }
+                }
+                // nothing of this CTA's may be in flight when it ends
+                give_up none = { 0, k_wait_cycles };
+                for (uint32_t i = n > ST ? n - ST : 0; i < n; i++) (void) bar_wait(kv_full + 8 * (i % ST), (i / ST) & 1, &none);
+            } else if (warp == 8) {
+                // ------------------------------------------------ MMA
+                uint32_t n = 0;                                  // ring position of the item's first K
+                uint32_t tiles[2] = { 0, 0 }, nq[2] = { 0, 0 };  // tiles of each group so far; phases of q_full
+                bool ok = true;
+                while (ok && next_item()) {
+                    const int groups = I.rows - I.r0 > B_ROWS ? 2 : 1;
+                    const uint32_t nt = (uint32_t) I.n;
+                    if (lane == 0) {
+                        auto full = [&](uint32_t i) { return bar_wait(kv_full + 8 * (i % ST), (i / ST) & 1, stop); };
+                        auto k_at = [&](uint32_t j) { return n + (j < BUFS ? j : 2 * j - BUFS + 1); };     // ring positions
+                        auto v_at = [&](uint32_t j) { return n + min(j + BUFS, nt) + j; };
+                        auto qk = [&](int g, uint32_t j) {
+                            const uint32_t kb = ring + k_at(j) % ST * TB, qb = q_sm + g * QB, b = (tiles[g] + j) % BUFS;
+#pragma unroll
+                            for (int k = 0; k < D / 16; k++)
+                                mma_ss(tmem + S_COL + 128 * g + 64 * b, smem_desc(qb + (k / 4) * QH + (k % 4) * 32, 16, 1024),
+                                       smem_desc(kb + (k / 4) * HB + (k % 4) * 32, 16, 1024), idesc_qk, k > 0);
+                            mma_commit(s_full + 16 * g + 8 * b);
+                        };
+                        for (uint32_t j = 0; ok && j < min(nt, (uint32_t) BUFS); j++) {
+                            ok = full(k_at(j));
+                            for (int g = 0; ok && g < groups; g++) {
+                                if (j == 0) ok = bar_wait(q_full + 8 * g, nq[g]++ & 1, stop);
+                                tc_after();
+                                if (ok) qk(g, j);
+                            }
+                            if (ok) mma_commit(kv_empty + 8 * (k_at(j) % ST));
+                        }
+                        for (uint32_t j = 0; ok && j < nt; j++) {
+                            const uint32_t vb = ring + v_at(j) % ST * TB;
+                            ok = full(v_at(j));
+                            for (int g = 0; ok && g < groups; g++) {
+                                const uint32_t at = tiles[g] + j, b = at % BUFS;
+                                auto pv = [&](int part) {
+                                    if (!bar_wait(p_ready + 16 * g + 8 * (PARTS == 2 ? part : b), at / BUFS & 1, stop)) return false;
+                                    tc_after();
+#pragma unroll
+                                    for (int kk = 4 * part; kk < 4 * part + 4; kk++)
+                                        mma_ts(tmem + O_COL + D * g, tmem + S_COL + 128 * g + 64 * b + 8 * kk,
+                                               smem_desc(vb + kk * 2048, HB, 1024), idesc_pv, j > 0 || kk > 0);
+                                    return true;
+                                };
+                                if (!(ok = pv(0))) break;
+                                if constexpr (PARTS == 2)
+                                    if (!(ok = pv(1))) break;
+                                if (j + 1 == nt) mma_commit(o_full + 8 * g);
+                                else if (BUFS == 2) mma_commit(pv_done + 8 * g);
+                                if (j + BUFS < nt) {
+                                    if (g == 0 && !(ok = full(k_at(j + BUFS)))) break;
+                                    qk(g, j + BUFS);
+                                }
+                            }
+                            if (ok) {
+                                mma_commit(kv_empty + 8 * (v_at(j) % ST));
+                                if (j + BUFS < nt) mma_commit(kv_empty + 8 * (k_at(j + BUFS) % ST));
                             }
                         }
-                        if (ok) {
-                            mma_commit(kv_empty + 8 * (v_at(j) % ST));
-                            if (j + BUFS < nt) mma_commit(kv_empty + 8 * (k_at(j + BUFS) % ST));
-                        }
+                        for (int g = 0; g < groups; g++) tiles[g] += nt;
                     }
-                    for (int g = 0; g < groups; g++) tiles[g] += nt;
+                    n += 2 * nt;
+                    ok = __shfl_sync(0xFFFFFFFFu, ok, 0);
                 }
-                n += 2 * nt;
-                ok = __shfl_sync(0xFFFFFFFFu, ok, 0);
+                if (lane == 0) {
+                    give_up none = { 0, k_wait_cycles };
+                    mma_commit(drained);
+                    (void) bar_wait(drained, 0, &none);
+                }
+                __syncwarp();
             }
-            if (lane == 0) {
-                give_up none = { 0, k_wait_cycles };
-                mma_commit(drained);
-                (void) bar_wait(drained, 0, &none);
-            }
-            __syncwarp();
-        }
         } else {
             if constexpr (D == 128) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;\n" ::);
             // ------------------------------------------------ softmax and output
@@ -2092,100 +2092,100 @@ k_sample(const T * __restrict__ logits, int64_t ld, int V, int vecs, int C, cons
 #pragma unroll
                 for (int j = 0; j < PB; j++) c[j] = M.hist[PB * tid + j];
             }
-                // each bucket's mass lies between count x its ends' weights; 1e-4 for the rounding of places and sums
-                const float step = R.inv_t / -q, ratio = expf(-step), w_first_bucket = expf(-step * (PB * tid));
-                float least = 0, most = 0, all_least, all_most, wb = w_first_bucket;
+            // each bucket's mass lies between count x its ends' weights; 1e-4 for the rounding of places and sums
+            const float step = R.inv_t / -q, ratio = expf(-step), w_first_bucket = expf(-step * (PB * tid));
+            float least = 0, most = 0, all_least, all_most, wb = w_first_bucket;
 #pragma unroll
-                for (int j = 0; j < PB; j++) {
-                    most += c[j] * wb;
-                    wb *= ratio;
-                    least += c[j] * wb;
+            for (int j = 0; j < PB; j++) {
+                most += c[j] * wb;
+                wb *= ratio;
+                least += c[j] * wb;
+            }
+            float * fs = reinterpret_cast<float *>(M.scan);
+            const float least_upto = block_scan<WARPS>(least, fs, all_least);
+            float lower = least_upto - least, upper = block_scan<WARPS>(most, fs, all_most) - most;
+            int b1 = S_BUCKETS, b2 = S_BUCKETS;
+            wb = w_first_bucket;
+#pragma unroll
+            for (int j = 0; j < PB; j++) {
+                upper += c[j] * wb;
+                wb *= ratio;
+                lower += c[j] * wb;
+                if (upper * 1.0001f >= R.top_p * all_least * 0.9999f) b1 = min(b1, PB * tid + j);
+                if (lower * 0.9999f >= R.top_p * all_most * 1.0001f) b2 = min(b2, PB * tid + j);
+            }
+            b1 = __reduce_min_sync(0xFFFFFFFFu, b1);
+            b2 = __reduce_min_sync(0xFFFFFFFFu, b2);
+            if (lane == 0) {
+                atomicMin(&M.b1, b1);
+                atomicMin(&M.b2, b2);
+            }
+            __syncthreads();
+            b1 = M.b1 == S_BUCKETS ? 0 : M.b1;
+            b2 = min(M.b2, S_BUCKETS - 1);
+            // all down to the cut's buckets, if they are few, else the cut's buckets
+            uint32_t upto = 0;
+#pragma unroll
+            for (int j = 0; j < PB; j++) upto += PB * tid + j <= b2 ? c[j] : 0u;
+            upto = block_sum<WARPS>(upto, reinterpret_cast<uint32_t *>(M.scan));
+            const float from = upto <= S_LIST ? 0.0f : (float) b1, to = (float) b2 + 1.0f;
+            ull all_m = 0, above_m = 0, above;
+            uint32_t klo = 0xFFFFFFFFu, khi = 0;
+            each_vec(w_first, w_first + vecs, [&](const uint4 & r, int at) {
+                uint32_t hi = 0, lo = 0, ahi = 0, alo = 0;
+                int an = 0;
+                bool some = false;
+#pragma unroll
+                for (int e = 0; e < E; e += 2) {
+                    const float2 d = R.distance2(vec16<T>::at(r, e), vec16<T>::at(r, e + 1)), b2 = mul2(d, make_float2(q, q));
+                    uint32_t h[2], l[2];
+                    mass_parts2(R.weight2(d), h, l);
+#pragma unroll
+                    for (int j = 0; j < 2; j++) {
+                        const float b = j ? b2.y : b2.x;
+                        const bool over = b < from;
+                        hi += h[j];
+                        lo += l[j];
+                        ahi += over ? h[j] : 0u;
+                        alo += over ? l[j] : 0u;
+                        an += over;
+                        some |= !over && b < to;
+                    }
                 }
-                float * fs = reinterpret_cast<float *>(M.scan);
-                const float least_upto = block_scan<WARPS>(least, fs, all_least);
-                float lower = least_upto - least, upper = block_scan<WARPS>(most, fs, all_most) - most;
-                int b1 = S_BUCKETS, b2 = S_BUCKETS;
-                wb = w_first_bucket;
+                all_m += mass_sum(hi, lo, E);
+                above_m += mass_sum(ahi, alo, an);
+                if (some) {
 #pragma unroll
-                for (int j = 0; j < PB; j++) {
-                    upper += c[j] * wb;
-                    wb *= ratio;
-                    lower += c[j] * wb;
-                    if (upper * 1.0001f >= R.top_p * all_least * 0.9999f) b1 = min(b1, PB * tid + j);
-                    if (lower * 0.9999f >= R.top_p * all_most * 1.0001f) b2 = min(b2, PB * tid + j);
-                }
-                b1 = __reduce_min_sync(0xFFFFFFFFu, b1);
-                b2 = __reduce_min_sync(0xFFFFFFFFu, b2);
-                if (lane == 0) {
-                    atomicMin(&M.b1, b1);
-                    atomicMin(&M.b2, b2);
-                }
-                __syncthreads();
-                b1 = M.b1 == S_BUCKETS ? 0 : M.b1;
-                b2 = min(M.b2, S_BUCKETS - 1);
-                // all down to the cut's buckets, if they are few, else the cut's buckets
-                uint32_t upto = 0;
-#pragma unroll
-                for (int j = 0; j < PB; j++) upto += PB * tid + j <= b2 ? c[j] : 0u;
-                upto = block_sum<WARPS>(upto, reinterpret_cast<uint32_t *>(M.scan));
-                const float from = upto <= S_LIST ? 0.0f : (float) b1, to = (float) b2 + 1.0f;
-                ull all_m = 0, above_m = 0, above;
-                uint32_t klo = 0xFFFFFFFFu, khi = 0;
-                each_vec(w_first, w_first + vecs, [&](const uint4 & r, int at) {
-                    uint32_t hi = 0, lo = 0, ahi = 0, alo = 0;
-                    int an = 0;
-                    bool some = false;
-#pragma unroll
-                    for (int e = 0; e < E; e += 2) {
-                        const float2 d = R.distance2(vec16<T>::at(r, e), vec16<T>::at(r, e + 1)), b2 = mul2(d, make_float2(q, q));
-                        uint32_t h[2], l[2];
-                        mass_parts2(R.weight2(d), h, l);
-#pragma unroll
-                        for (int j = 0; j < 2; j++) {
-                            const float b = j ? b2.y : b2.x;
-                            const bool over = b < from;
-                            hi += h[j];
-                            lo += l[j];
-                            ahi += over ? h[j] : 0u;
-                            alo += over ? l[j] : 0u;
-                            an += over;
-                            some |= !over && b < to;
+                    for (int e = 0; e < E; e++) {
+                        const float v = vec16<T>::at(r, e), b = place(v);
+                        if (b >= from && b < to) {
+                            klo = min(klo, order_key(v));
+                            khi = max(khi, order_key(v));
+                            if (*(volatile int *) &M.n <= S_LIST) push(v, at + e);
                         }
                     }
-                    all_m += mass_sum(hi, lo, E);
-                    above_m += mass_sum(ahi, alo, an);
-                    if (some) {
+                }
+            });
+            klo = __reduce_min_sync(0xFFFFFFFFu, klo);
+            khi = __reduce_max_sync(0xFFFFFFFFu, khi);
+            if (lane == 0) {
+                atomicMin(&M.key_lo, klo);
+                atomicMax(&M.key_hi, khi);
+            }
+            {
+                ull m = above_m;
 #pragma unroll
-                        for (int e = 0; e < E; e++) {
-                            const float v = vec16<T>::at(r, e), b = place(v);
-                            if (b >= from && b < to) {
-                                klo = min(klo, order_key(v));
-                                khi = max(khi, order_key(v));
-                                if (*(volatile int *) &M.n <= S_LIST) push(v, at + e);
-                            }
-                        }
-                    }
-                });
-                klo = __reduce_min_sync(0xFFFFFFFFu, klo);
-                khi = __reduce_max_sync(0xFFFFFFFFu, khi);
-                if (lane == 0) {
-                    atomicMin(&M.key_lo, klo);
-                    atomicMax(&M.key_hi, khi);
-                }
-                {
-                    ull m = above_m;
-#pragma unroll
-                    for (int d = 16; d; d >>= 1) m += __shfl_xor_sync(0xFFFFFFFFu, m, d);
-                    if (lane == 0) M.part_mass[warp] = m;
-                }
-                cluster_sum(all_m, above_m, whole, above);
-                const int n = listed();
-                if (n <= S_LIST) {
-                    if (finish(n, above, from > 0.0f, true)) return;
-                    found = true;
-                    parts_known = R.min_p <= 0.0f;
-                }
-                if (tid == 0) M.above = above;
+                for (int d = 16; d; d >>= 1) m += __shfl_xor_sync(0xFFFFFFFFu, m, d);
+                if (lane == 0) M.part_mass[warp] = m;
+            }
+            cluster_sum(all_m, above_m, whole, above);
+            const int n = listed();
+            if (n <= S_LIST) {
+                if (finish(n, above, from > 0.0f, true)) return;
+                found = true;
+                parts_known = R.min_p <= 0.0f;
+            }
+            if (tid == 0) M.above = above;
         }
         if (list) {
             smem & M0 = peer(0);               // into CTA 0's list
