@@ -2580,8 +2580,8 @@ int launch_attn_dim(const lnsb_paged_attn_args & a, cudaStream_t s) {
         const int G = a.n_head / a.kv.n_head_kv;
         CUtensorMap km, vm;
         // scale > 0: the tiles take the maximum before the scale
-        if (a.max_q * G > ROWS && a.kv.n_pages > 0 && a.scale > 0.0f && std::isfinite(a.scale) && map_cache(&km, a.kv, a.kv.k_cache, b_keys<D>()) &&
-            map_cache(&vm, a.kv, a.kv.v_cache, b_keys<D>())) {
+        if (a.max_q > ROWS / G && a.kv.n_pages > 0 && a.scale > 0.0f && std::isfinite(a.scale) &&
+            map_cache(&km, a.kv, a.kv.k_cache, b_keys<D>()) && map_cache(&vm, a.kv, a.kv.v_cache, b_keys<D>())) {
             auto kern = k_paged_attn_tiles<T, D>;
             static bool attr[k_max_devices] = {};
             int st = allow_smem(kern, attr, b_smem<D>());
