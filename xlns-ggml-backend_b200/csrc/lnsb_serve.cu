@@ -116,7 +116,9 @@ __device__ __forceinline__ int64_t page_of(const paged & P, int s, int64_t row, 
 // ============================ append =======================================
 
 // Any alignment and any n_dims: one thread a rotated pair, copied element or v
-// element.
+// element.  Each looks its token up for itself, and nothing is loaded wide: 333
+// us where the kernel below takes 56.  It is there for rows that do not allow
+// that one's 16-byte accesses; a decoder's do.
 template <class TI, class TC>
 __global__ void k_paged_append(paged P, const TI * __restrict__ k, const TI * __restrict__ v, const TI * __restrict__ q,
                                TC * __restrict__ q_out, const float * __restrict__ cos_sin, int64_t k_ld, int64_t v_ld,
@@ -195,7 +197,7 @@ __device__ __forceinline__ void store8(T * p, const float (&x)[8]) {
 // takes 8 elements (NEOX: 8 of each half of the pairs), a block `tokens`
 // tokens.  Its inputs are on their way while the first threads look up where
 // the block's tokens go.  HBM bounds it: 8,592 tokens of 32/8 heads of 128 from
-// F32 56 us, 5.7 TB/s (the element-wise kernel 333 us); one token 2.0 us.
+// F32 56 us, 5.7 TB/s (the element-wise kernel 333 us); one token 2.2 us.
 template <class TI, class TC, bool NEOX>
 __global__ void __launch_bounds__(256)
 k_paged_append_vec(paged P, const TI * __restrict__ k, const TI * __restrict__ v, const TI * __restrict__ q,
@@ -309,9 +311,15 @@ k_paged_append_vec(paged P, const TI * __restrict__ k, const TI * __restrict__ v
 // from the same product as the output, against a column of ones, so it is of
 // the weights as rounded.
 //
-// Measured: 64 ragged sequences of up to 8,192 rows, 32/8 heads of 128 (1.2 GB)
-// 204 us, 5.9 TB/s; one token over 131,072 rows 107 us, 5.0 TB/s; one token
-// over 200 rows 8.4 us.
+// The weights are rounded to the cache's type because the tensor cores take
+// operands of one 16-bit type; two parts of each would double the products with
+// V.  Against 64 bits the outputs are off by 2.1e-3 in BF16 and 2.3e-4 in F16
+// (root mean square, relative), where rounding the outputs alone gives 1.7e-3
+// and 2.2e-4.
+//
+// Measured, replayed from a CUDA graph: 64 ragged sequences of up to 8,192 rows,
+// 32/8 heads of 128 (1.2 GB) 205 us, 5.9 TB/s; one token over 131,072 rows 109
+// us, 4.9 TB/s; one token over 200 rows 8.3 us.
 
 constexpr int ROWS = 16, KEYS = 64, A_CTAS = 2 * k_sms;
 constexpr int MAX_DIM = 256;
@@ -644,14 +652,16 @@ k_paged_attn_rows(paged P, const T * __restrict__ q, T * __restrict__ dst, const
 //
 // Head dim 64 leaves TMEM for two S of 64 keys to each group: while its softmax
 // works on one, the next is ready, so it waits for no product (45 us where one
-// S of 128 keys takes 57, on 16 sequences of up to 512 new tokens in a window
-// of 1,024).  At 128 the products are what counts, and QK over 64 keys reads
-// shared memory for Q as long as over 128: one S of 128 keys (720 us where two
-// of 64 take 998, on the two chunks below), and PV of
-// its first 64 keys starts under the weights of the others.
+// S of 128 keys took 57 when the two were compared, on 16 sequences of up to 512
+// new tokens in a window of 1,024).  At 128 the products are what counts, and QK
+// over 64 keys reads shared memory for Q as long as over 128: one S of 128 keys
+// (720 us where two of 64 took 998, on the two chunks below), and PV of its first
+// 64 keys starts under the weights of the others.
 //
-// Measured: two chunks, 3,927 tokens over 26,803 rows in all, 32/8
-// heads of 128, 720 us (1,108 TFLOP/s); 512 tokens over 8,192 rows 84 us.
+// Measured, replayed from a CUDA graph: two chunks, 3,927 tokens over 26,803 rows
+// in all, 32/8 heads of 128, 734 us (1,087 TFLOP/s; 847 us call after call);
+// 512 tokens over 8,192 rows 85 us; the 16 sequences 47 us, behind the rows
+// kernel, whose CTAs leave no registers for this kernel's to start beside them.
 //
 //   warps 0-3, 4-7  group 0, group 1: Q into shared memory, softmax, output
 //   warp 8          one thread issues every MMA: PV of a group's tile j, then
@@ -1402,8 +1412,9 @@ k_paged_attn_tiles(const __grid_constant__ CUtensorMap kmap, const __grid_consta
 //            32-bit order-preserving keys.
 //
 // Measured: 1 x 49,152 F32 with every filter 16 us, 48 rows of mixed filters 36
-// us, 256 x 131,071 bf16 151 us (greedy rows alone 25, top-k 27-55, top-p alone
-// 124-134, where three passes take exponentials).
+// us, 256 x 131,071 bf16 152 us (greedy rows alone 24, no filter 50, top-k 25-54,
+// top-p alone 118-135: beside one pass of exponentials, as without a filter, it
+// scans for the smallest logit and counts distances, one atomic a logit).
 //
 // Masses are integers of 2^-38 of the largest weight, rounded to nearest: sums
 // are exact in any order, so the result hangs on no order of atomics.
@@ -2579,13 +2590,19 @@ int launch_attn_dim(const lnsb_paged_attn_args & a, cudaStream_t s) {
     if constexpr (D == 64 || D == 128) {
         const int G = a.n_head / a.kv.n_head_kv;
         CUtensorMap km, vm;
+        // More than 16 rows go to the tiles: the rows kernel reads K and V again for every 16.  64 sequences over 4,096
+        // rows, 8 kv heads of 128: 16 rows each 226 us by tiles and 189 by rows, 20 to 32 rows 227 and 346, 256 rows
+        // 338 and 2,820; at head dim 64 (4 kv heads) 104 and 88, 105 and 146, 165 and 804.  (One sequence of 9 to 16 rows
+        // leaves the rows kernel few warps to a key: 34 us by tiles and 67 by rows over 2,048 rows.  There the rule is wrong
+        // by up to two times, and so at head dim 64 from 64 rows on, where one short sequence takes 40 by tiles, 33 by rows.)
         // scale > 0: the tiles take the maximum before the scale
         if (a.max_q > ROWS / G && a.kv.n_pages > 0 && a.scale > 0.0f && std::isfinite(a.scale) &&
             map_cache(&km, a.kv, a.kv.k_cache, b_keys<D>()) && map_cache(&vm, a.kv, a.kv.v_cache, b_keys<D>())) {
             auto kern = k_paged_attn_tiles<T, D>;
             static bool attr[k_max_devices] = {};
             int st = allow_smem(kern, attr, b_smem<D>());
-            // sequences of few rows go to the rows kernel; one sequence alone does not split
+            // sequences of few rows go to the rows kernel; one sequence alone does not split (which of several have
+            // few is known on the device only: a launch without such rows ends at the plan)
             const bool both = a.kv.n_seqs > 1;
             if (st == 0 && both) st = launch_rows<T, D>(a, ROWS, s);
             if (st != 0) return st;
